@@ -40,6 +40,7 @@ typedef struct {
     uint64_t* enc_desc;
     long long enc_desc_cap;
     unsigned long long* enc_dbg;   /* DC_DEBUG_STAMPS: [tile][8] encoder phase stamps */
+    unsigned* d_kv_status;           /* sticky status of the key/value cache operators (dc_kv_status) */
     unsigned long long* d_total;
     unsigned* d_enc_err;
     unsigned* d_enc_flag;            /* the pack kernel's scan-published flag (encode epoch) */
@@ -195,6 +196,7 @@ int dc_set_encode_stream(void* stream) {
 int dc_abi_status(void) { return G.abi_rc; }
 void dc_abi_set_status(int rc) { G.abi_rc = rc; }      /* the double ABI (dc_host64.c) reports through it too */
 int dc_set_error(int code, const char* msg) { return seterr(code, "%s", msg); }
+unsigned* dc_kv_status_word(void) { return G.d_kv_status; }   /* (dc_host_lowbit.c) */
 void* dc_get_stream(void) { return (void*)G.st; }
 void dc_set_abs_error_bound(double bound) { absErrBound = bound; absErrorBound_binary = -100; }
 double dc_get_abs_error_bound(void) { return absErrBound; }
@@ -298,6 +300,8 @@ int dc_init(int device) {
     HIPCHK(hipMalloc((void**)&G.d_x2n, sizeof x2n));
     HIPCHK(hipMemcpy(G.d_crctab, tab, sizeof tab, hipMemcpyHostToDevice));
     HIPCHK(hipMemcpy(G.d_x2n, x2n, sizeof x2n, hipMemcpyHostToDevice));
+    HIPCHK(hipMalloc((void**)&G.d_kv_status, 64));
+    HIPCHK(hipMemset(G.d_kv_status, 0, 64));
     G.dec_epoch = 1;
     G.inited = 1;
     return DC_OK;

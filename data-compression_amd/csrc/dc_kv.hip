@@ -1,0 +1,711 @@
+// dc_kv.hip -- a key/value cache held in 4 or 8 bits: quantised as it is written, read back, and attended to as it is
+// held (no float copy of it in HBM).
+//
+// A row is the D keys (or values) of one token and one head.  With n = 2^BITS - 1 it is stored as D codes and one word,
+// its step s (a bfloat16, low half) and its zero point z (int16, high half):
+//     x^_i = s (z + code_i),   |x_i - x^_i| <= s / 2 (up to f32's rounding of the row's span),
+//     s = the smallest bfloat16 >= max(span / n, amax / 32512, 2^-100),  z = rint(lo / s),
+//     code_i = clamp(rint(x_i / s) - z, 0, n)           (rint: to nearest, ties to even, of the exact quotient).
+// s (z + code) has at most 8 + 15 significant bits, so it is exact in f32 and the only rounding on the way back is the
+// one to the output's type.  A row with a value that is not finite has s = NaN and reads back as NaN.
+//
+// A page holds P tokens (a multiple of 16) of every head; per head: the keys' codes [token][D], the values' codes
+// [block of 16 tokens][16 units of D/16 values][16 tokens], the keys' words [token], the values' words [token].  Both
+// code layouts put what one lane of the attention's matrix instructions needs into consecutive bytes, so that a wave
+// reads a block of 16 tokens of either as one contiguous piece.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include "dc_shared.h"
+#include "../../include/dc_gpu.h"
+
+namespace {
+
+using dc::KvArgs;
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+static __device__ __forceinline__ float asf(uint32_t u) { return __uint_as_float(u); }
+static __device__ __forceinline__ uint32_t asu(float f) { return __float_as_uint(f); }
+
+// ---- element types ------------------------------------------------------------------------------------------------
+struct F32 {
+    typedef float T;
+    static __device__ __forceinline__ float to(T x) { return x; }
+    static __device__ __forceinline__ T from(float x) { return x; }
+    static constexpr float MOST = 3.402823466e38f;
+};
+struct F16 {
+    typedef _Float16 T;
+    static __device__ __forceinline__ float to(T x) { return (float)x; }
+    static __device__ __forceinline__ T from(float x) { return (_Float16)x; }
+    static constexpr float MOST = 65504.0f;
+};
+struct BF16 {
+    typedef uint16_t T;
+    static __device__ __forceinline__ float to(T x) { return asf((uint32_t)x << 16); }
+    static __device__ __forceinline__ T from(float x) {                 // to nearest, ties to even
+        const __bf16 y = (__bf16)x;
+        return __builtin_bit_cast(uint16_t, y);
+    }
+    static constexpr float MOST = 3.38953139e38f;
+};
+
+// N values at p, moved in pieces of A bytes (what the alignment allows)
+template <class T, int N, int A> static __device__ __forceinline__ void load_n(const T* p, T* x) {
+    constexpr int BYTES = N * (int)sizeof(T);
+    if constexpr (A >= 16 && BYTES % 16 == 0) {
+        for (int i = 0; i < BYTES / 16; i++) ((uint4*)x)[i] = ((const uint4*)p)[i];
+    } else if constexpr (A >= 8 && BYTES % 8 == 0) {
+        for (int i = 0; i < BYTES / 8; i++) ((uint2*)x)[i] = ((const uint2*)p)[i];
+    } else if constexpr (A >= 4 && BYTES % 4 == 0) {
+        for (int i = 0; i < BYTES / 4; i++) ((uint32_t*)x)[i] = ((const uint32_t*)p)[i];
+    } else if constexpr (A >= 2 && BYTES % 2 == 0) {
+        for (int i = 0; i < BYTES / 2; i++) ((uint16_t*)x)[i] = ((const uint16_t*)p)[i];
+    } else {
+        for (int i = 0; i < BYTES; i++) ((uint8_t*)x)[i] = ((const uint8_t*)p)[i];
+    }
+}
+template <class T, int N, int A> static __device__ __forceinline__ void store_n(T* p, const T* x) {
+    constexpr int BYTES = N * (int)sizeof(T);
+    if constexpr (A >= 16 && BYTES % 16 == 0) {
+        for (int i = 0; i < BYTES / 16; i++) ((uint4*)p)[i] = ((const uint4*)x)[i];
+    } else if constexpr (A >= 8 && BYTES % 8 == 0) {
+        for (int i = 0; i < BYTES / 8; i++) ((uint2*)p)[i] = ((const uint2*)x)[i];
+    } else if constexpr (A >= 4 && BYTES % 4 == 0) {
+        for (int i = 0; i < BYTES / 4; i++) ((uint32_t*)p)[i] = ((const uint32_t*)x)[i];
+    } else if constexpr (A >= 2 && BYTES % 2 == 0) {
+        for (int i = 0; i < BYTES / 2; i++) ((uint16_t*)p)[i] = ((const uint16_t*)x)[i];
+    } else {
+        for (int i = 0; i < BYTES; i++) ((uint8_t*)p)[i] = ((const uint8_t*)x)[i];
+    }
+}
+
+// n / d by the host's reciprocal m = floor(2^64 / d) + 1 (d = 1: m = 0): exact for n d < 2^64
+static __device__ __forceinline__ uint32_t div_by(uint32_t n, unsigned long long m) {
+    return m ? (uint32_t)__umul64hi((unsigned long long)n, m) : n;
+}
+
+// the row's lanes are 16 neighbours: rotations within a DPP row
+template <int N> static __device__ __forceinline__ float ror16(float x) {
+    return asf((uint32_t)__builtin_amdgcn_update_dpp(0, (int)asu(x), 0x120 + N, 0xF, 0xF, false));
+}
+static __device__ __forceinline__ float min16(float x) {
+    x = fminf(x, ror16<8>(x)); x = fminf(x, ror16<4>(x)); x = fminf(x, ror16<2>(x)); return fminf(x, ror16<1>(x));
+}
+static __device__ __forceinline__ float max16(float x) {
+    x = fmaxf(x, ror16<8>(x)); x = fmaxf(x, ror16<4>(x)); x = fmaxf(x, ror16<2>(x)); return fmaxf(x, ror16<1>(x));
+}
+
+// the smallest bfloat16 c with c * n >= v, from an estimate of v / n that is not above it (c n is exact: 8 + 8 bits)
+static __device__ __forceinline__ float step_up(float v, float inv_n, float n) {
+    float c = asf(asu(v * inv_n * 0.9999990f) & 0xFFFF0000u);
+    for (int i = 0; i < 2; i++) c = c * n < v ? asf(asu(c) + 0x10000u) : c;
+    return c;
+}
+
+// rint(x / s) of the exact quotient: an estimate within one, put right by the remainder (exact, as r s has 24 bits)
+static __device__ __forceinline__ float rint_div(float x, float s, float inv, float half) {
+    float r = rintf(x * inv);
+    const float d = fmaf(-r, s, x), a = fabsf(d);
+    const bool up = a > half || (a == half && ((int)r & 1));
+    return up ? r + copysignf(1.0f, d) : r;
+}
+
+struct Row { long long page; int at; bool ok, bad; };
+
+// position pos of sequence b: its page and place, ok if it is inside the cache
+static __device__ __forceinline__ Row locate(const KvArgs& a, int b, long long pos) {
+    Row r;
+    const bool in = pos >= 0 && pos < a.capacity;
+    const uint32_t p = in ? (uint32_t)pos : 0u, slot = div_by(p, a.page_inv);
+    r.at = (int)(p - slot * (uint32_t)a.page);
+    r.page = a.table ? (long long)a.table[(long long)b * a.table_stride + slot] : (long long)b;
+    r.ok = in && r.page >= 0 && r.page < a.pages;
+    return r;
+}
+
+// ---- write -----------------------------------------------------------------------------------------------------------
+// 16 lanes per row, each with the D/16 consecutive values whose codes are one unit of the layout; min and max over the
+// row's lanes, then the codes.  One read of the input, one write of the codes: HBM bound for long inputs, launch bound
+// for single tokens.
+template <class E, int D, int BITS, bool VEC> __global__ __launch_bounds__(256) void kv_write(KvArgs a) {
+    constexpr int N = D / 16, U = N * BITS / 8, ROW = 16 * U;
+    constexpr int BYTES = N * (int)sizeof(typename E::T);
+    constexpr int AL = VEC ? (BYTES & -BYTES) : (int)sizeof(typename E::T);
+    const long long row = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+    const int c = threadIdx.x & 15;
+    if (row >= a.rows) return;                              // (a whole row's lanes leave together)
+    const int kv = (int)(row & 1);
+    const uint32_t th = (uint32_t)(row >> 1), bt = div_by(th, a.heads_inv), h = th - bt * a.heads;
+    const uint32_t b = div_by(bt, a.tokens_inv), t = bt - b * a.tokens;
+    if (a.lens && (int)t >= a.lens[b]) return;
+    const Row r = locate(a, (int)b, (long long)a.start[b] + t);
+    if (!r.ok) {
+        if (c == 0) atomicOr(a.status, 1u);
+        return;
+    }
+    const typename E::T* src = kv ? (const typename E::T*)a.v + b * a.vs[0] + t * a.vs[1] + h * a.vs[2]
+                                  : (const typename E::T*)a.k + b * a.ks[0] + t * a.ks[1] + h * a.ks[2];
+    alignas(16) typename E::T raw[N];
+    load_n<typename E::T, N, AL>(src + c * N, raw);
+    float x[N], lo, hi;
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        x[i] = E::to(raw[i]);
+        lo = i ? fminf(lo, x[i]) : x[i];
+        hi = i ? fmaxf(hi, x[i]) : x[i];
+        top = max(top, asu(x[i]) & 0x7FFFFFFFu);
+    }
+    const unsigned long long odd = __ballot(top >= 0x7F800000u);
+    const bool bad = (odd >> (threadIdx.x & 48)) & 0xFFFFull;
+    lo = min16(lo);
+    hi = max16(hi);
+    constexpr float CODES = (float)((1 << BITS) - 1);
+    const float half_span = 0.5f * hi - 0.5f * lo;
+    float s = fmaxf(step_up(half_span, 2.0f / CODES, 0.5f * CODES), step_up(fmaxf(hi, -lo), 1.0f / 32512.0f, 32512.0f));
+    s = fmaxf(s, 7.888609052210118e-31f);                   // 2^-100
+    const float inv = __builtin_amdgcn_rcpf(s), half = 0.5f * s;
+    const float z = rint_div(lo, s, inv, half);
+    alignas(16) uint8_t out[U];
+#pragma unroll
+    for (int i = 0; i < N; i += 8 / BITS) {
+        uint32_t q = 0;
+        for (int j = 0; j < 8 / BITS; j++) {
+            const float f = fminf(fmaxf(rint_div(x[i + j], s, inv, half) - z, 0.0f), CODES);
+            q |= (uint32_t)(int)f << (j * BITS);
+        }
+        out[i * BITS / 8] = bad ? (uint8_t)0 : (uint8_t)q;
+    }
+    uint8_t* base = a.data + (r.page * a.heads + h) * a.head_bytes;
+    uint8_t* dst = kv ? base + (long long)a.page * ROW + (r.at >> 4) * (16 * ROW) + c * (16 * U) + (r.at & 15) * U
+                      : base + (long long)r.at * ROW + c * U;
+    store_n<uint8_t, U, (U & -U)>(dst, out);
+    if (c == 0) {
+        const uint32_t w = bad ? 0x7FC0u : (asu(s) >> 16) | ((uint32_t)(int)z << 16);
+        *(uint32_t*)(base + 2ll * a.page * ROW + (kv ? 4ll * a.page : 0) + 4ll * r.at) = w;
+    }
+}
+
+// ---- read ------------------------------------------------------------------------------------------------------------
+template <class E, int D, int BITS, bool VEC> __global__ __launch_bounds__(256) void kv_read(KvArgs a) {
+    constexpr int N = D / 16, U = N * BITS / 8, ROW = 16 * U;
+    constexpr int BYTES = N * (int)sizeof(typename E::T);
+    constexpr int AL = VEC ? (BYTES & -BYTES) : (int)sizeof(typename E::T);
+    const long long row = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+    const int c = threadIdx.x & 15;
+    if (row >= a.rows) return;
+    const int kv = (int)(row & 1);
+    const uint32_t th = (uint32_t)(row >> 1), bt = div_by(th, a.heads_inv), h = th - bt * a.heads;
+    const uint32_t b = div_by(bt, a.tokens_inv), t = bt - b * a.tokens;
+    if (a.lens && (int)t >= a.lens[b]) return;
+    const Row r = locate(a, (int)b, (long long)a.start[b] + t);
+    typename E::T* dst = kv ? (typename E::T*)a.v + b * a.vs[0] + t * a.vs[1] + h * a.vs[2]
+                            : (typename E::T*)a.k + b * a.ks[0] + t * a.ks[1] + h * a.ks[2];
+    alignas(16) typename E::T out[N];
+    if (r.ok) {
+        const uint8_t* base = a.data + (r.page * a.heads + h) * a.head_bytes;
+        const uint8_t* src = kv ? base + (long long)a.page * ROW + (r.at >> 4) * (16 * ROW) + c * (16 * U) + (r.at & 15) * U
+                                : base + (long long)r.at * ROW + c * U;
+        alignas(16) uint8_t in[U];
+        load_n<uint8_t, U, (U & -U)>(src, in);
+        const uint32_t w = *(const uint32_t*)(base + 2ll * a.page * ROW + (kv ? 4ll * a.page : 0) + 4ll * r.at);
+        const float s = asf(w << 16);
+        const int z = (int)w >> 16;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int code = BITS == 8 ? in[i] : (in[i / 2] >> ((i & 1) * 4)) & 15;
+            const float x = s * (float)(z + code);
+            out[i] = E::from(x != x ? x : fminf(fmaxf(x, -E::MOST), E::MOST));
+        }
+    } else {
+        if (c == 0) atomicOr(a.status, 1u);
+#pragma unroll
+        for (int i = 0; i < N; i++) out[i] = E::from(asf(0x7FC00000u));
+    }
+    store_n<typename E::T, N, AL>(dst + c * N, out);
+}
+
+// ---- attention ---------------------------------------------------------------------------------------------------------
+// O = softmax(scale q k^T) v^ over the positions a query sees.  With k^ = s (z + code), code' = code - 2^(BITS-1) and
+// z' = z + 2^(BITS-1):
+//     q . k^_t = ks_t (q . code'_t + kz'_t sum(q)),      O_d = sum_t (p_t vs_t) (code'_td + vz'_t):
+// the matrix instructions see the codes alone, as f16 whole numbers (exact), and a token's step and zero point enter as
+// two multiply-adds on its score and as a factor of its weight.  The queries of a group of heads that share keys are the
+// columns of mfma 16x16x32: A = 16 tokens' codes, B = 16 queries.  The score tile's lane layout (token = 4 (lane / 16) +
+// r, query = lane % 16) is that of the weights' operand in the second product if its 32 tokens are taken in the order
+// (block of 16, r) for each group of lanes, and the values' layout in the cache has that order: no data crosses lanes.
+//
+// The weights w_t = p_t vs_t go into the product as f16.  A running maximum of log2(p_t) + exponent(vs_t) keeps the
+// largest of them in [1, 2^9], whatever the steps are; the sum of p_t is kept in f32 with the same reference.  f16 has 11
+// bits: each w_t is off by 2^-12 of itself at most, below half a unit of what bf16 or f16 outputs round to.  Queries are
+// scaled to 2^10..2^11 by a power of two (exact); elements 2^-24 of a row's largest lose bits.
+static __device__ __forceinline__ float over_groups_max(float x) {     // over the 4 groups of 16 lanes
+    auto p = __builtin_amdgcn_permlane32_swap((int)asu(x), (int)asu(x), false, false);
+    x = fmaxf(asf((uint32_t)p[0]), asf((uint32_t)p[1]));
+    auto q = __builtin_amdgcn_permlane16_swap((int)asu(x), (int)asu(x), false, false);
+    return fmaxf(asf((uint32_t)q[0]), asf((uint32_t)q[1]));
+}
+static __device__ __forceinline__ float over_groups_sum(float x) {
+    auto p = __builtin_amdgcn_permlane32_swap((int)asu(x), (int)asu(x), false, false);
+    x = asf((uint32_t)p[0]) + asf((uint32_t)p[1]);
+    auto q = __builtin_amdgcn_permlane16_swap((int)asu(x), (int)asu(x), false, false);
+    return asf((uint32_t)q[0]) + asf((uint32_t)q[1]);
+}
+
+union Frag { h8 v; h2 p[4]; uint32_t u[4]; };
+union Two { h2 h; uint32_t u; };
+static __device__ __forceinline__ uint32_t h2_sub(uint32_t x, float c) {
+    Two t;
+    t.u = x;
+    t.h = t.h - (h2){(_Float16)c, (_Float16)c};
+    return t.u;
+}
+
+// whole numbers as f16: 1024 + n and 64 + n are n's bits behind a constant exponent
+// 4 bits: nibbles 0..3 of both halves of x -> pairs o[0..3], less 8
+static __device__ __forceinline__ void pairs4(uint32_t x, uint32_t* o, int n) {
+    const uint32_t y = x >> 8;
+    o[0] = h2_sub((x & 0x000F000Fu) | 0x64006400u, 1032.0f);
+    if (n > 1) o[1] = h2_sub((x & 0x00F000F0u) | 0x54005400u, 72.0f);
+    if (n > 2) o[2] = h2_sub((y & 0x000F000Fu) | 0x64006400u, 1032.0f);
+    if (n > 3) o[3] = h2_sub((y & 0x00F000F0u) | 0x54005400u, 72.0f);
+}
+// 8 bits: bytes 0..1 of both halves, less 128
+static __device__ __forceinline__ void pairs8(uint32_t x, uint32_t* o) {
+    o[0] = h2_sub((x & 0x00FF00FFu) | 0x64006400u, 1152.0f);
+    o[1] = h2_sub(((x >> 8) & 0x00FF00FFu) | 0x64006400u, 1152.0f);
+}
+// the 16 bits at byte offset o of w[] (offsets are known when this is compiled); those at two offsets, one per half
+static __device__ __forceinline__ uint32_t at16(const uint32_t* w, int o) {
+    return (o & 3) == 3 ? __builtin_amdgcn_alignbyte(w[o / 4 + 1], w[o / 4], 3) : w[o / 4] >> (8 * (o & 3));
+}
+static __device__ __forceinline__ uint32_t pair16(const uint32_t* w, int oa, int ob) {
+    const uint32_t x = oa & 3, y = ob & 3;
+    if (x == 3 || y == 3) return __builtin_amdgcn_perm(at16(w, ob), at16(w, oa), 0x05040100u);
+    return __builtin_amdgcn_perm(w[ob / 4], w[oa / 4], x | (x + 1) << 8 | (y + 4) << 16 | (y + 5) << 24);
+}
+
+// the d (within 8) that element e of a key operand holds
+template <int BITS> static __device__ __forceinline__ constexpr int key_order(int e) {
+    if constexpr (BITS == 4) return (e >> 1) + 4 * (e & 1);
+    else return (e & 4) + ((e >> 1) & 1) + 2 * (e & 1);
+}
+
+template <int U> struct Stage {         // what a lane holds of 32 tokens: 2 blocks of 16
+    uint32_t k[2][U], v[2][U + 1];      // (one word more: a 16-bit piece may end in it; never used)
+    u4 kw[2], vw[2];
+};
+
+template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_attention(KvArgs a) {
+    constexpr int N = D / 16, U = N * BITS / 8, ROW = 16 * U, KS = D / 32, COLS = 16 * NT;
+    constexpr float BIAS = (float)(1 << (BITS - 1));
+    constexpr bool ALL = D * NT <= 256;                     // every wave its own sums in LDS, or one after the other
+    __shared__ float acc_lds[(ALL ? 4 : 1) * N * 16 * COLS];
+    __shared__ float ml[3][4][COLS];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, g = lane >> 4;
+    // block -> (split, tile of query rows, head, sequence)
+    uint32_t x = blockIdx.x;
+    const uint32_t split = x % a.splits; x /= a.splits;
+    const uint32_t tile = x % a.tiles; x /= a.tiles;
+    const uint32_t h = x % a.heads, b = x / a.heads;
+    int context = a.start[b];
+    if (context < 0 || context > a.capacity) {
+        if (threadIdx.x == 0) atomicOr(a.status, 1u);
+        context = context < 0 ? 0 : (int)a.capacity;
+    }
+    const int len = a.lens ? min(max(a.lens[b], 0), a.tokens) : a.tokens;
+    const int rows = len * a.group;
+    const int row0 = tile * COLS;
+    if (row0 >= rows) return;
+    // what each query row of the tile sees: positions < sees
+    int sees[NT], most = 0;
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        const int rw = row0 + nt * 16 + col;
+        const int i = (int)div_by((uint32_t)rw, a.group_inv);
+        sees[nt] = rw < rows ? (a.causal ? max(context - len + 1 + i, 0) : context) : 0;
+    }
+    {
+        const int last = (int)div_by((uint32_t)(min(row0 + COLS, rows) - 1), a.group_inv);
+        most = a.causal ? max(context - len + 1 + last, 0) : context;
+    }
+    const int chunk = ((context + (int)a.splits - 1) / (int)a.splits + 127) & ~127;
+    const long long lo64 = (long long)split * chunk;
+    const int lo = lo64 < most ? (int)lo64 : most, hi = (int)min((long long)most, lo64 + chunk);
+
+    // queries, as f16 in the keys' order; their sum; the factor that takes a score to log2 units
+    Frag q[NT][KS];
+    float qsum[NT], unit[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        const int rw = row0 + nt * 16 + col;
+        const bool on = rw < rows;
+        const int i = (int)div_by((uint32_t)(on ? rw : 0), a.group_inv), gi = (on ? rw : 0) - i * a.group;
+        const long long at = b * a.ks[0] + (long long)i * a.ks[1] + (long long)(h * a.group + gi) * a.ks[2] + g * (D / 4);
+        float f[D / 4], big = 0.0f;
+        uint32_t top = 0;
+        if (a.dtype == DC_BF16) {
+            const uint16_t* p = (const uint16_t*)a.k + at;
+            alignas(16) uint16_t raw[D / 4];
+            if (a.vec) load_n<uint16_t, D / 4, 16>(p, raw);
+            else load_n<uint16_t, D / 4, 2>(p, raw);
+#pragma unroll
+            for (int j = 0; j < D / 4; j++) f[j] = on ? BF16::to(raw[j]) : 0.0f;
+        } else {
+            const _Float16* p = (const _Float16*)a.k + at;
+            alignas(16) _Float16 raw[D / 4];
+            if (a.vec) load_n<_Float16, D / 4, 16>(p, raw);
+            else load_n<_Float16, D / 4, 2>(p, raw);
+#pragma unroll
+            for (int j = 0; j < D / 4; j++) f[j] = on ? (float)raw[j] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < D / 4; j++) top = max(top, asu(f[j]) & 0x7FFFFFFFu);
+        big = over_groups_max(asf(min(top, 0x7F7FFFFFu)));
+        const int e = min(264 - (int)(asu(big) >> 23), 253);            // 2^(10 - exponent of the largest)
+        const float up = asf((uint32_t)e << 23), down = asf((uint32_t)(254 - e) << 23);
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < KS; j++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const _Float16 v = (_Float16)(f[j * 8 + key_order<BITS>(k)] * up);
+                q[nt][j].v[k] = v;
+                sum += (float)v;
+            }
+        qsum[nt] = over_groups_sum(sum);
+        unit[nt] = a.scale * 1.44269504088896340736f * down;
+    }
+
+    f4 acc[NT][N];
+    float M[NT], L[NT], Z[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        M[nt] = -1e30f;
+        L[nt] = Z[nt] = 0.0f;
+        for (int i = 0; i < N; i++) acc[nt][i] = (f4){0, 0, 0, 0};
+    }
+
+    const int* table = a.table ? a.table + (long long)b * a.table_stride : nullptr;
+    const uint32_t blocks = (uint32_t)a.page >> 4;
+    // the page and place of the block of 16 tokens from t on (t < hi); -1: not in the cache
+    auto page_of = [&](int t, uint32_t& in) -> long long {
+        const uint32_t blk = (uint32_t)t >> 4, slot = div_by(blk, a.blocks_inv);
+        in = blk - slot * blocks;
+        const long long p = table ? (long long)table[slot] : (long long)b;
+        return p >= 0 && p < a.pages ? p : -1;
+    };
+    auto fetch = [&](Stage<U>& s, const long long* page, const uint32_t* in) {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const uint8_t* base = a.data + ((page[j] < 0 ? 0 : page[j]) * a.heads + h) * a.head_bytes;
+            const uint8_t* codes = base + (long long)in[j] * (16 * ROW) + col * ROW + g * (4 * U);
+            load_n<uint32_t, U, 4 * (U & -U)>((const uint32_t*)codes, s.k[j]);
+            load_n<uint32_t, U, 4 * (U & -U)>((const uint32_t*)(codes + (long long)a.page * ROW), s.v[j]);
+            const uint8_t* words = base + 2ll * a.page * ROW + in[j] * 64 + g * 16;
+            s.kw[j] = *(const u4*)words;
+            s.vw[j] = *(const u4*)(words + 4ll * a.page);
+        }
+    };
+    Stage<U> cur, nxt;
+    long long pg[2];
+    uint32_t in[2];
+    bool hole[2], hole_nxt[2];
+    const int first = lo + wave * 32;
+    auto find = [&](int t) {                                // the second block may lie past the end: then the first again
+        pg[0] = page_of(t, in[0]);
+        if (t + 16 < hi) pg[1] = page_of(t + 16, in[1]);
+        else { pg[1] = pg[0]; in[1] = in[0]; }
+    };
+    if (first < hi) {
+        find(first);
+        hole[0] = pg[0] < 0; hole[1] = pg[1] < 0;
+        fetch(cur, pg, in);
+        if (first + 128 < hi) find(first + 128);
+    }
+    for (int t0 = first; t0 < hi; t0 += 128) {
+        if (t0 + 128 < hi) {
+            hole_nxt[0] = pg[0] < 0; hole_nxt[1] = pg[1] < 0;
+            fetch(nxt, pg, in);
+            if (t0 + 256 < hi) find(t0 + 256);
+        }
+        if ((hole[0] || hole[1]) && lane == 0) atomicOr(a.status, 1u);
+        // scores
+        f4 s[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) s[nt][0] = s[nt][1] = (f4){0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int st = 0; st < KS; st++) {
+                Frag k;
+                if constexpr (BITS == 4) pairs4(cur.k[j][st], k.u, 4);
+                else {
+                    pairs8(cur.k[j][2 * st], k.u);
+                    pairs8(cur.k[j][2 * st + 1], k.u + 2);
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+                    s[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k.v, q[nt][st].v, s[nt][j], 0, 0, 0);
+            }
+        // the tokens' words
+        float ks[8], kz[8], ve[8], vm[8], vi[8], vz[8];
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int t = 4 * j + r;
+                const uint32_t kw = cur.kw[j][r], vw = cur.vw[j][r], e = (vw >> 7) & 0xFFu;
+                ks[t] = asf(kw << 16);
+                kz[t] = (float)((int)kw >> 16) + BIAS;
+                ve[t] = e == 255u ? asf(0x7FC00000u) : (float)((int)e - 127);
+                vm[t] = asf(((vw & 0x7Fu) << 16) | 0x3F800000u);
+                vi[t] = asf((254u - min(e, 254u)) << 23);
+                vz[t] = (float)((int)vw >> 16) + BIAS;
+            }
+        Frag w[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            float ref[8], mx = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int left = hole[j] ? -1 : sees[nt] - (t0 + 16 * j + 4 * g);    // tokens of this lane that are seen
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int t = 4 * j + r;
+                    const float y = fmaf(fmaf(kz[t], qsum[nt], s[nt][j][r]) * unit[nt], ks[t], ve[t]);
+                    ref[t] = r < left ? y : -INFINITY;
+                    mx = fmaxf(mx, ref[t]);
+                }
+            }
+            mx = over_groups_max(mx);
+            if (__any(mx > M[nt] + 8.0f)) {                 // (weights stay below 2^9)
+                const float m = fmaxf(M[nt], mx), al = __builtin_amdgcn_exp2f(M[nt] - m);
+                M[nt] = m;
+                L[nt] *= al;
+                Z[nt] *= al;
+                for (int i = 0; i < N; i++) acc[nt][i] *= al;
+            }
+#pragma unroll
+            for (int t = 0; t < 8; t++) {
+                const float p = __builtin_amdgcn_exp2f(ref[t] - M[nt]);
+                const _Float16 wt = (_Float16)(p * vm[t]);
+                L[nt] = fmaf(p, vi[t], L[nt]);
+                Z[nt] = fmaf((float)wt, vz[t], Z[nt]);
+                w[nt].v[t] = wt;
+            }
+        }
+        // values: unit col, tokens 4 g .. 4 g + 3 of both blocks
+#pragma unroll
+        for (int i0 = 0; i0 < N; i0 += 16 / BITS) {         // 16 bits of each token at a time
+            constexpr int PER = 16 / BITS;
+            const int n = N - i0 < PER ? N - i0 : PER, o = i0 * BITS / 8;
+            uint32_t got[4][PER];
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+                    const uint32_t y = pair16(cur.v[j], 2 * r * U + o, (2 * r + 1) * U + o);
+                    if constexpr (BITS == 4) pairs4(y, got[2 * j + r], n);
+                    else pairs8(y, got[2 * j + r]);
+                }
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                if (i >= n) break;
+                Frag f;
+                for (int k = 0; k < 4; k++) f.u[k] = got[k][i];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+                    acc[nt][i0 + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.v, w[nt].v, acc[nt][i0 + i], 0, 0, 0);
+            }
+        }
+        cur = nxt;
+        hole[0] = hole_nxt[0]; hole[1] = hole_nxt[1];
+    }
+
+    // the four waves' sums, in a fixed order
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        L[nt] = over_groups_sum(L[nt]);
+        Z[nt] = over_groups_sum(Z[nt]);
+        if (g == 0) {
+            ml[0][wave][nt * 16 + col] = M[nt];
+            ml[1][wave][nt * 16 + col] = L[nt];
+            ml[2][wave][nt * 16 + col] = Z[nt];
+        }
+    }
+    __syncthreads();
+    float f[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        float m = ml[0][0][nt * 16 + col];
+        for (int v = 1; v < 4; v++) m = fmaxf(m, ml[0][v][nt * 16 + col]);
+        f[nt] = __builtin_amdgcn_exp2f(M[nt] - m);
+    }
+    for (int v = 0; v < (ALL ? 1 : 4); v++) {
+        if (ALL || wave == v)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int i = 0; i < N; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        float* p = &acc_lds[(((ALL ? wave : 0) * NT + nt) * N + i) * 256 + (g * 4 + r) * 16 + col];
+                        const float y = acc[nt][i][r] * f[nt];
+                        *p = ALL || v == 0 ? y : *p + y;
+                    }
+        __syncthreads();
+    }
+    // 16 columns x 16 units: a thread writes the N values of its unit
+    const int oc = threadIdx.x & 15, ou = threadIdx.x >> 4;
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        const int rw = row0 + nt * 16 + oc;
+        if (rw >= rows) continue;
+        float m = ml[0][0][nt * 16 + oc], l = 0.0f, z = 0.0f;
+        for (int v = 1; v < 4; v++) m = fmaxf(m, ml[0][v][nt * 16 + oc]);
+        for (int v = 0; v < 4; v++) {
+            const float sc = __builtin_amdgcn_exp2f(ml[0][v][nt * 16 + oc] - m);
+            l = fmaf(ml[1][v][nt * 16 + oc], sc, l);
+            z = fmaf(ml[2][v][nt * 16 + oc], sc, z);
+        }
+        float o[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            float y = z;
+            for (int v = 0; v < (ALL ? 4 : 1); v++) y += acc_lds[((v * NT + nt) * N + i) * 256 + ou * 16 + oc];
+            o[i] = y;
+        }
+        const int i = (int)div_by((uint32_t)rw, a.group_inv), gi = rw - i * a.group;
+        if (a.splits > 1) {                                 // unnormalised, with its maximum and sum
+            const long long at = ((((long long)b * a.heads + h) * a.row_slots + rw) * a.splits + split);
+            float* p = a.part + at * D + ou * N;
+            for (int k = 0; k < N; k++) p[k] = o[k];
+            if (ou == 0) {
+                a.part_ml[2 * at] = m;
+                a.part_ml[2 * at + 1] = l;
+            }
+            continue;
+        }
+        const bool none = (a.causal ? context - len + 1 + i : context) <= 0;
+        const float inv = 1.0f / l;
+        const long long at = b * a.vs[0] + (long long)i * a.vs[1] + (long long)(h * a.group + gi) * a.vs[2] + ou * N;
+        if (a.dtype == DC_BF16) {
+            uint16_t* p = (uint16_t*)a.v + at;
+            for (int k = 0; k < N; k++) p[k] = BF16::from(none ? 0.0f : o[k] * inv);
+        } else {
+            _Float16* p = (_Float16*)a.v + at;
+            for (int k = 0; k < N; k++) p[k] = (_Float16)(none ? 0.0f : o[k] * inv);
+        }
+        if (a.lse && ou == 0)
+            a.lse[((long long)b * a.tokens + i) * a.heads * a.group + h * a.group + gi] =
+                none ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
+    }
+}
+
+// the splits of a query row joined, in their order: a workgroup per row
+template <int D> __global__ __launch_bounds__(256) void kv_join(KvArgs a) {
+    constexpr int N = D / 16;
+    __shared__ float sums[16][D];
+    __shared__ float ms[16], lsum[16];
+    uint32_t x = blockIdx.x;
+    const uint32_t rw = x % a.row_slots; x /= a.row_slots;
+    const uint32_t h = x % a.heads, b = x / a.heads;
+    const int len = a.lens ? min(max(a.lens[b], 0), a.tokens) : a.tokens;
+    if ((int)rw >= len * a.group) return;
+    const int u = threadIdx.x & 15, part = threadIdx.x >> 4;
+    const long long at = (((long long)b * a.heads + h) * a.row_slots + rw) * a.splits;
+    float m = -1e30f, l = 0.0f, o[N];
+    for (int k = 0; k < N; k++) o[k] = 0.0f;
+    for (uint32_t s = part; s < a.splits; s += 16) {
+        const float pm = a.part_ml[2 * (at + s)], pl = a.part_ml[2 * (at + s) + 1];
+        const float nm = fmaxf(m, pm), fa = __builtin_amdgcn_exp2f(m - nm), fb = __builtin_amdgcn_exp2f(pm - nm);
+        const float* p = a.part + (at + s) * D + u * N;
+        for (int k = 0; k < N; k++) o[k] = fmaf(p[k], fb, o[k] * fa);
+        l = fmaf(pl, fb, l * fa);
+        m = nm;
+    }
+    for (int k = 0; k < N; k++) sums[part][u * N + k] = o[k];
+    if (u == 0) { ms[part] = m; lsum[part] = l; }
+    __syncthreads();
+    m = ms[0];
+    for (int k = 1; k < 16; k++) m = fmaxf(m, ms[k]);
+    l = 0.0f;
+    float f[16];
+    for (int k = 0; k < 16; k++) {
+        f[k] = __builtin_amdgcn_exp2f(ms[k] - m);
+        l = fmaf(lsum[k], f[k], l);
+    }
+    const int i = (int)div_by(rw, a.group_inv), gi = (int)rw - i * a.group;
+    int context = a.start[b];
+    context = context < 0 ? 0 : context > a.capacity ? (int)a.capacity : context;
+    const bool none = (a.causal ? context - len + 1 + i : context) <= 0;
+    const long long out = b * a.vs[0] + (long long)i * a.vs[1] + (long long)(h * a.group + gi) * a.vs[2];
+    for (int d = threadIdx.x; d < D; d += 256) {
+        float y = 0.0f;
+        for (int k = 0; k < 16; k++) y = fmaf(sums[k][d], f[k], y);
+        y = none ? 0.0f : y / l;
+        if (a.dtype == DC_BF16) ((uint16_t*)a.v)[out + d] = BF16::from(y);
+        else ((_Float16*)a.v)[out + d] = (_Float16)y;
+    }
+    if (a.lse && threadIdx.x == 0)
+        a.lse[((long long)b * a.tokens + i) * a.heads * a.group + h * a.group + gi] =
+            none ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
+}
+
+template <class E, int BITS, bool VEC> int go_rows(const KvArgs& a, bool write, hipStream_t st) {
+    const unsigned grid = (unsigned)((a.rows + 15) / 16);
+#define DC_ROWS(D) \
+    case D: \
+        if (write) kv_write<E, D, BITS, VEC><<<grid, 256, 0, st>>>(a); \
+        else kv_read<E, D, BITS, VEC><<<grid, 256, 0, st>>>(a); \
+        break
+    switch (a.dim) {
+        DC_ROWS(32); DC_ROWS(64); DC_ROWS(96); DC_ROWS(128); DC_ROWS(160); DC_ROWS(192); DC_ROWS(224); DC_ROWS(256);
+        default: return 1;
+    }
+#undef DC_ROWS
+    return hipGetLastError() != hipSuccess;
+}
+template <class E> int go_bits(const KvArgs& a, bool write, hipStream_t st) {
+    if (a.bits == 4) return a.vec ? go_rows<E, 4, true>(a, write, st) : go_rows<E, 4, false>(a, write, st);
+    return a.vec ? go_rows<E, 8, true>(a, write, st) : go_rows<E, 8, false>(a, write, st);
+}
+
+// tiles of 16 query rows that a wave takes at once where there are many: what its registers hold
+constexpr int wide_tiles(int dim) { return dim <= 64 ? 4 : dim <= 192 ? 2 : 1; }
+
+template <int D, int BITS> int go_attention(const KvArgs& a, hipStream_t st) {
+    const unsigned grid = (unsigned)((long long)a.splits * a.tiles * a.heads * a.batch);
+    constexpr int WIDE = wide_tiles(D);
+    if constexpr (WIDE > 1) {
+        if (a.cols == 16) kv_attention<D, BITS, 1><<<grid, 256, 0, st>>>(a);
+        else kv_attention<D, BITS, WIDE><<<grid, 256, 0, st>>>(a);
+    } else kv_attention<D, BITS, 1><<<grid, 256, 0, st>>>(a);
+    if (a.splits > 1) kv_join<D><<<(unsigned)((long long)a.row_slots * a.heads * a.batch), 256, 0, st>>>(a);
+    return hipGetLastError() != hipSuccess;
+}
+
+}  // namespace
+
+extern "C" int dc_launch_kv_rows(const dc::KvArgs* a, int write, dc_hip_stream st) {
+    if (a->dtype == DC_F32) return go_bits<F32>(*a, write, st);
+    if (a->dtype == DC_F16) return go_bits<F16>(*a, write, st);
+    return go_bits<BF16>(*a, write, st);
+}
+
+extern "C" int dc_kv_wide_cols(int dim) { return 16 * wide_tiles(dim); }
+
+extern "C" int dc_launch_kv_attention(const dc::KvArgs* a, dc_hip_stream st) {
+#define DC_DIM(D) case D: return a->bits == 4 ? go_attention<D, 4>(*a, st) : go_attention<D, 8>(*a, st)
+    switch (a->dim) {
+        DC_DIM(32); DC_DIM(64); DC_DIM(96); DC_DIM(128); DC_DIM(160); DC_DIM(192); DC_DIM(224); DC_DIM(256);
+        default: return 1;
+    }
+#undef DC_DIM
+}

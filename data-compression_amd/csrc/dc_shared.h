@@ -104,6 +104,42 @@ typedef struct Dec3Bufs {
                                       (zero between launches: the launch's last wave resets them) */
 } Dec3Bufs;
 
+/* key/value cache operators (dc_kv.hip): one struct for the write, the read and the attention */
+typedef struct KvArgs {
+    uint8_t* data;                 /* the cache */
+    long long pages, head_bytes;   /* bytes of one page's one head */
+    int page, heads, dim, bits;    /* tokens per page, heads, head size, 4 or 8 */
+    int batch, tokens;
+    const int* start;              /* [batch] position of the first token; attention: the sequence's length */
+    const int* lens;               /* [batch] or NULL: all `tokens` of each */
+    const int* table;              /* [batch][table_stride] pages, or NULL: page b is sequence b's */
+    long long table_stride, capacity;   /* positions a sequence can have */
+    unsigned long long page_inv, blocks_inv, heads_inv, tokens_inv, group_inv;   /* reciprocals: floor(2^64 / d) + 1, 0 for 1 */
+    const void* k;                 /* write: keys, read: keys out, attention: queries; strides (batch, token, head) in elements */
+    const void* v;                 /* write: values, read: values out, attention: the output */
+    long long ks[3], vs[3];
+    int dtype, vec;                /* vec: pointers and strides allow whole-lane accesses */
+    long long rows;                /* write / read: batch * tokens * heads * 2 */
+    unsigned* status;
+    int group, causal;             /* attention: query heads per head of the cache */
+    float scale;
+    float* lse;
+    float* part;                   /* [batch][heads][row_slots][splits][dim] unnormalised sums */
+    float* part_ml;                /* the same places: maximum, sum */
+    unsigned splits, tiles, row_slots, cols;
+} KvArgs;
+
+/* activation checkpoints (dc_act.hip) */
+typedef struct ActArgs {
+    int kind, gated, dtype, mode;  /* mode: 0 flat, 1 rows apart in whole 8s, 2 any */
+    long long n, rows, cols, groups;
+    unsigned long long cols8_inv;  /* reciprocal of cols / 8 (mode 1) */
+    const void *x, *up;            /* forward: inputs; backward: x is the output's gradient */
+    void *y, *dx, *dup;
+    long long ldx, ldup, ldy, lddx, lddup;
+    uint8_t *kept, *kept_up;
+} ActArgs;
+
 #ifdef __cplusplus
 }  /* namespace dc */
 extern "C" {
@@ -294,6 +330,10 @@ int dc_launch_flip_bits(uint8_t* s, unsigned long long nbits, long long count, u
                         dc_hip_stream st);
 int dc_launch_crc_resend(const uint32_t* crc, const uint8_t* src, uint8_t* dst, long long nbytes, int copy,
                          unsigned* count, dc_hip_stream st);
+int dc_launch_kv_rows(const DC_NS KvArgs* a, int write, dc_hip_stream st);
+int dc_launch_kv_attention(const DC_NS KvArgs* a, dc_hip_stream st);
+int dc_kv_wide_cols(int dim);
+int dc_launch_act(const DC_NS ActArgs* a, int back, dc_hip_stream st);
 int dc_launch_ham_syndrome(const uint8_t* s, long long nbytes, unsigned long long* d_syn_ones, dc_hip_stream st);
 
 #ifdef __cplusplus

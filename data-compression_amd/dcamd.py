@@ -51,6 +51,8 @@ EXT_SYMBOLS = [
     "dc_decode_status_clear", "dc_set_runs_max_bytes", "dc_last_decode_was_runs",
     "dc_last_decode_launched_runs", "dc_last_decode_used_maps", "dc_med_last_wide", "dc_set_decode3_maps", "dc_set_halo_async", "dc_med_shard_stats", "dc_med_shard_trans",
     "dc_med_shard_binades",
+    "dc_kv_page_bytes", "dc_kv_write_device", "dc_kv_read_device", "dc_kv_attention_workspace", "dc_kv_attention_device",
+    "dc_kv_status", "dc_act_bytes", "dc_act_forward_device", "dc_act_backward_device",
 ]
 
 
@@ -61,6 +63,16 @@ def build():
 
 class DCError(RuntimeError):
     pass
+
+
+class KvCacheDesc(C.Structure):     # dc_kv_cache
+    _fields_ = [("data", C.c_void_p), ("pages", C.c_longlong), ("page_size", C.c_int), ("heads", C.c_int),
+                ("head_dim", C.c_int), ("bits", C.c_int)]
+
+
+class KvBatchDesc(C.Structure):     # dc_kv_batch
+    _fields_ = [("batch", C.c_int), ("tokens", C.c_int), ("start", C.c_void_p), ("lens", C.c_void_p),
+                ("table", C.c_void_p), ("table_width", C.c_int), ("table_stride", C.c_longlong)]
 
 
 class Lib:
@@ -164,12 +176,30 @@ class Lib:
         L.dc64_last_decode_flags.restype = C.c_uint
         L.dc64_to_small_device.argtypes = [vp, ll, vp, C.POINTER(C.c_double)]
         L.dc64_med_device.argtypes = [vp, ll, C.POINTER(C.c_double), C.POINTER(C.c_int)]
+        # fixed-rate operators
+        kvc, kvb, strides = C.POINTER(KvCacheDesc), C.POINTER(KvBatchDesc), C.POINTER(ll)
+        L.dc_kv_page_bytes.argtypes = [C.c_int] * 4
+        L.dc_kv_page_bytes.restype = C.c_size_t
+        L.dc_kv_write_device.argtypes = [kvc, kvb, C.c_int, vp, strides, vp, strides, vp]
+        L.dc_kv_read_device.argtypes = [kvc, kvb, C.c_int, vp, strides, vp, strides, vp]
+        L.dc_kv_attention_workspace.argtypes = [kvc, C.c_int, C.c_int, C.c_int, ll]
+        L.dc_kv_attention_workspace.restype = C.c_size_t
+        L.dc_kv_attention_device.argtypes = [kvc, kvb, C.c_int, C.c_int, vp, strides, C.c_float, C.c_int, ll, vp, strides,
+                                             vp, vp, C.c_size_t, vp]
+        L.dc_kv_status.argtypes = [vp, C.POINTER(C.c_uint), C.c_int]
+        L.dc_act_bytes.argtypes = [ll]
+        L.dc_act_bytes.restype = C.c_size_t
+        L.dc_act_forward_device.argtypes = [C.c_int, C.c_int, ll, ll, vp, ll, vp, ll, vp, ll, vp, vp, vp]
+        L.dc_act_backward_device.argtypes = [C.c_int, C.c_int, ll, ll, vp, ll, vp, vp, vp, ll, vp, ll, vp, ll, vp]
+        self.device = None
 
     # ---- state
     def init(self, device=0):
         rc = self.L.dc_init(device)
         if rc:
             raise DCError(f"dc_init: {rc} {self.err()}")
+        if self.device is None:
+            self.device = device
 
     def err(self):
         m = self.L.dc_last_error()
@@ -1198,3 +1228,293 @@ def lib():
     if _lib is None:
         _lib = Lib()
     return _lib
+
+
+# ---- floats held in 8 or 4 bits in HBM: torch tensors on the current stream ------------------------------------------
+DC_F32, DC_F16, DC_BF16 = 0, 1, 2
+ACT_KINDS = {"none": 0, "silu": 1, "gelu": 2}
+_Strides = C.c_longlong * 3
+
+
+def _dtype_code(dtype, allowed="f32, f16 or bf16"):
+    import torch
+    code = {torch.float32: DC_F32, torch.float16: DC_F16, torch.bfloat16: DC_BF16}.get(dtype)
+    if code is None or (code == DC_F32 and "f32" not in allowed):
+        raise ValueError(f"dtype {dtype}: {allowed} is needed")
+    return code
+
+
+def _on_gpu(*tensors):
+    """The stream to launch on: all tensors lie on the library's device, which is made torch's current one by the caller
+    (`with torch.cuda.device(...)`) if it is not."""
+    import torch
+    L = lib()
+    for t in tensors:
+        if t is not None and not t.is_cuda:
+            raise ValueError("tensors must lie on the GPU")
+    if L.device is None:
+        L.init(tensors[0].device.index)
+    for t in tensors:
+        if t is not None and t.device.index != L.device:
+            raise ValueError(f"tensors must lie on the library's device (cuda:{L.device})")
+    if torch.cuda.current_device() != L.device:
+        raise ValueError(f"the current device must be the library's (cuda:{L.device})")
+    return L, torch.cuda.current_stream().cuda_stream
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+class KVCache:
+    """A decoder's key/value cache held in 4 or 8 bits (dc_kv_cache, include/dc_gpu.h): `pages` pages of page_size tokens
+    (a multiple of 16) for `heads` heads of head_dim (a multiple of 32, at most 256).  `buffer` (uint8, on the GPU) holds
+    it; without one it is allocated, zeroed.
+
+    Sequences are rows of a batch: `table` (batch, n) int32 names each one's pages (None: page b is sequence b's only one),
+    `start` / `context` and `lens` are int32 of (batch,).  Rows from lens[b] on are padding and are not touched.
+    Calls go to torch's current stream, allocate what they return (and the attention its workspace) from torch, and can be
+    captured into a graph."""
+
+    def __init__(self, pages, page_size, heads, head_dim, bits=4, buffer=None, device="cuda"):
+        page = self.page_bytes(page_size, heads, head_dim, bits)
+        if pages < 1:
+            raise ValueError("a cache has at least one page")
+        if buffer is None:
+            import torch
+            buffer = torch.zeros(pages * page, dtype=torch.uint8, device=device)
+        if str(buffer.dtype) != "torch.uint8" or not buffer.is_contiguous() or buffer.numel() < pages * page:
+            raise ValueError(f"buffer: {pages * page} contiguous bytes (uint8) are needed")
+        if buffer.data_ptr() % 16:
+            raise ValueError("buffer: 16-byte alignment is needed")
+        self.pages, self.page_size, self.heads, self.head_dim, self.bits = pages, page_size, heads, head_dim, bits
+        self.buffer = buffer
+        self._desc = KvCacheDesc(buffer.data_ptr(), pages, page_size, heads, head_dim, bits)
+
+    @staticmethod
+    def page_bytes(page_size, heads, head_dim, bits=4):
+        """Bytes of one page."""
+        n = lib().L.dc_kv_page_bytes(page_size, heads, head_dim, bits)
+        if not n:
+            raise ValueError("page_size is a multiple of 16, head_dim a multiple of 32 up to 256, bits 4 or 8")
+        return n
+
+    def _batch(self, batch, tokens, start, table, lens, what="start"):
+        for name, t in ((what, start), ("lens", lens)):
+            if t is not None and (str(t.dtype) != "torch.int32" or t.shape != (batch,) or not t.is_contiguous()):
+                raise ValueError(f"{name}: contiguous int32 of ({batch},) is needed")
+        if table is None:
+            if batch > self.pages:
+                raise ValueError("without a table each sequence has a page")
+            return KvBatchDesc(batch, tokens, start.data_ptr(), _ptr(lens), None, 0, 0)
+        if str(table.dtype) != "torch.int32" or table.dim() != 2 or table.shape[0] != batch or table.shape[1] < 1 or \
+                table.stride(1) != 1 or (batch > 1 and table.stride(0) < table.shape[1]):
+            raise ValueError(f"table: int32 of ({batch}, pages of a sequence) with consecutive entries is needed")
+        return KvBatchDesc(batch, tokens, start.data_ptr(), _ptr(lens), table.data_ptr(), table.shape[1],
+                           max(table.stride(0), table.shape[1]))
+
+    def _rows(self, x, name, heads=None):
+        if x.dim() != 4 or x.shape[3] != self.head_dim or (heads is None and x.shape[2] != self.heads):
+            raise ValueError(f"{name}: (batch, tokens, {self.heads if heads is None else 'heads'}, {self.head_dim}) is needed")
+        if x.stride(3) != 1 and x.numel():
+            raise ValueError(f"{name}: a head's values must be consecutive")
+        return _Strides(x.stride(0), x.stride(1), x.stride(2))
+
+    def write(self, k, v, start, table=None, lens=None):
+        """Quantise k, v (batch, tokens, heads, head_dim) to positions start[b] .. of each sequence."""
+        ks, vs = self._rows(k, "k"), self._rows(v, "v")
+        if k.shape != v.shape or k.dtype != v.dtype:
+            raise ValueError("k and v differ in shape or type")
+        code = _dtype_code(k.dtype)
+        at = self._batch(k.shape[0], k.shape[1], start, table, lens)
+        L, stream = _on_gpu(self.buffer, k, v, start, table, lens)
+        L.check(L.L.dc_kv_write_device(self._desc, at, code, k.data_ptr(), ks, v.data_ptr(), vs, stream), "kv_write")
+
+    def read(self, start, tokens, table=None, lens=None, dtype=None, out=None):
+        """The keys and values of positions start[b] .. start[b] + tokens as floats of `dtype` (bf16), in `out` if given
+        (rows of padding keep what they have), else in new tensors (padding is 0)."""
+        import torch
+        batch = start.shape[0] if start.dim() else 0
+        at = self._batch(batch, tokens, start, table, lens)
+        if out is None:
+            new = torch.empty if lens is None else torch.zeros
+            dtype = dtype or torch.bfloat16
+            out = [new((batch, tokens, self.heads, self.head_dim), dtype=dtype, device=self.buffer.device) for _ in range(2)]
+        k, v = out
+        ks, vs = self._rows(k, "out"), self._rows(v, "out")
+        if k.shape != v.shape or k.dtype != v.dtype or k.shape[:2] != (batch, tokens) or (dtype and k.dtype != dtype):
+            raise ValueError("out: two tensors (batch, tokens, heads, head_dim) of the type asked for are needed")
+        code = _dtype_code(k.dtype)
+        L, stream = _on_gpu(self.buffer, k, v, start, table, lens)
+        L.check(L.L.dc_kv_read_device(self._desc, at, code, k.data_ptr(), ks, v.data_ptr(), vs, stream), "kv_read")
+        return k, v
+
+    def attention(self, q, context, table=None, lens=None, scale=None, causal=True, max_context=None, out=None, lse=None):
+        """softmax(scale q k^T) v over the first context[b] positions of each sequence, q (batch, tokens, q_heads, head_dim)
+        in f16 or bf16 being its last lens[b] (None: all) tokens: causal, token i sees context[b] - lens[b] + 1 + i of
+        them.  scale: 1 / sqrt(head_dim).  max_context: the longest context expected (the table's capacity).  out: where
+        to put the output (rows of padding keep what they have; else they are 0); lse: an f32 tensor (batch, tokens,
+        q_heads) for the log of each softmax's sum."""
+        import torch
+        qs = self._rows(q, "q", heads="any")
+        code = _dtype_code(q.dtype, "f16 or bf16")
+        batch, tokens, q_heads, _ = q.shape
+        if q_heads < 1 or q_heads % self.heads:
+            raise ValueError(f"q: heads in a multiple of the cache's {self.heads} are needed")
+        at = self._batch(batch, tokens, context, table, lens, "context")
+        capacity = self.page_size * (1 if table is None else table.shape[1])
+        limit = capacity if max_context is None else min(int(max_context), capacity)
+        if limit < 0:
+            raise ValueError("max_context is not negative")
+        if out is None:
+            out = (torch.empty if lens is None else torch.zeros)(q.shape, dtype=q.dtype, device=q.device)
+        os_ = self._rows(out, "out", heads="any")
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError("out: q's shape and type are needed")
+        if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:3] or not lse.is_contiguous()):
+            raise ValueError("lse: contiguous float32 of (batch, tokens, q_heads) is needed")
+        L, stream = _on_gpu(self.buffer, q, context, table, lens, out, lse)
+        need = L.L.dc_kv_attention_workspace(self._desc, batch, tokens, q_heads, limit)
+        space = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        L.check(L.L.dc_kv_attention_device(self._desc, at, code, q_heads, q.data_ptr(), qs,
+                                           self.head_dim ** -0.5 if scale is None else float(scale), int(bool(causal)), limit,
+                                           out.data_ptr(), os_, _ptr(lse), _ptr(space), need, stream), "kv_attention")
+        return out
+
+    @staticmethod
+    def status(reset=False):
+        """The sticky status word after the work queued on the current stream (synchronous): 1, a position or page outside
+        its cache (then dropped, read as NaN or left out)."""
+        import torch
+        L, v = lib(), C.c_uint(0)
+        L.check(L.L.dc_kv_status(torch.cuda.current_stream().cuda_stream, C.byref(v), int(bool(reset))), "kv_status")
+        return int(v.value)
+
+
+def _flat(x):
+    """x as rows of its last dimension: (tensor, rows, cols, elements between rows); copied if its rows do not lie so."""
+    cols = x.shape[-1] if x.dim() else 1
+    rows = x.numel() // cols if cols else 0
+    if x.is_contiguous():
+        return x, rows, cols, cols
+    y = x.reshape(rows, cols)
+    if y.stride(1) != 1 or y.stride(0) < cols:
+        y = y.contiguous()
+    return y, rows, cols, max(y.stride(0), cols)
+
+
+class ActCheckpoint:
+    """Activations kept in 8 bits (include/dc_gpu.h): `kept` and, of a gated activation, `kept_up` (uint8, dc_act_bytes of
+    the shape each)."""
+
+    def __init__(self, shape, dtype, kept, kept_up=None):
+        self.shape, self.dtype, self.kept, self.kept_up = tuple(shape), dtype, kept, kept_up
+        n = 1
+        for s in self.shape:
+            n *= s
+        need = lib().L.dc_act_bytes(n)
+        for t in (kept, kept_up):
+            if t is not None and (str(t.dtype) != "torch.uint8" or not t.is_contiguous() or t.numel() < need):
+                raise ValueError(f"checkpoint: {need} contiguous bytes (uint8) are needed")
+        _dtype_code(dtype)
+
+    def load(self):
+        """The kept values as floats: a tuple of one tensor, or two of a gated activation."""
+        import torch
+        got = []
+        for kept in (self.kept, self.kept_up):
+            if kept is None:
+                continue
+            x = torch.empty(self.shape, dtype=self.dtype, device=kept.device)
+            _, rows, cols, ld = _flat(x)
+            L, stream = _on_gpu(kept)
+            L.check(L.L.dc_act_backward_device(0, _dtype_code(self.dtype), rows, cols, None, 0, kept.data_ptr(), None,
+                                               x.data_ptr(), ld, None, 0, None, 0, stream), "act_load")
+            got.append(x)
+        return tuple(got)
+
+
+def _act_kind(kind):
+    if kind not in ("silu", "gelu"):
+        raise ValueError(f"kind {kind!r}: 'silu' or 'gelu' is needed")
+    return ACT_KINDS[kind]
+
+
+def _new_kept(n, device):
+    import torch
+    return torch.empty(lib().L.dc_act_bytes(n), dtype=torch.uint8, device=device)
+
+
+def act_save(x):
+    """x (f32, f16, bf16) as an ActCheckpoint."""
+    code = _dtype_code(x.dtype)
+    x2, rows, cols, ld = _flat(x)
+    L, stream = _on_gpu(x)
+    kept = _new_kept(x.numel(), x.device)
+    L.check(L.L.dc_act_forward_device(0, code, rows, cols, x2.data_ptr(), ld, None, 0, None, 0, kept.data_ptr(), None, stream),
+            "act_save")
+    return ActCheckpoint(x.shape, x.dtype, kept)
+
+
+def act_forward(x, kind, up=None):
+    """y = f(x) (kind 'silu' or 'gelu', the exact one) or f(x) * up, and the ActCheckpoint of x (and up), in one pass."""
+    import torch
+    code, k = _dtype_code(x.dtype), _act_kind(kind)
+    if up is not None and (up.shape != x.shape or up.dtype != x.dtype):
+        raise ValueError("x and up differ in shape or type")
+    x2, rows, cols, ldx = _flat(x)
+    u2, _, _, ldu = _flat(up) if up is not None else (None, 0, 0, 0)
+    L, stream = _on_gpu(x, up)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    kept = _new_kept(x.numel(), x.device)
+    kept_up = _new_kept(x.numel(), x.device) if up is not None else None
+    L.check(L.L.dc_act_forward_device(k, code, rows, cols, x2.data_ptr(), ldx, _ptr(u2), ldu, y.data_ptr(), cols,
+                                      kept.data_ptr(), _ptr(kept_up), stream), "act_forward")
+    return y, ActCheckpoint(x.shape, x.dtype, kept, kept_up)
+
+
+def act_backward(dy, checkpoint, kind, recompute=False):
+    """The gradient of act_forward at the checkpoint's values: dx, or (dx, dup) of a gated activation; with recompute, a
+    tuple that ends with the activation's output at those values (for the gradient of what used it)."""
+    import torch
+    code, k = _dtype_code(dy.dtype), _act_kind(kind)
+    if tuple(dy.shape) != checkpoint.shape or dy.dtype != checkpoint.dtype:
+        raise ValueError("dy and the checkpoint differ in shape or type")
+    gated = checkpoint.kept_up is not None
+    d2, rows, cols, ldd = _flat(dy)
+    L, stream = _on_gpu(dy, checkpoint.kept, checkpoint.kept_up)
+    new = lambda on: torch.empty(dy.shape, dtype=dy.dtype, device=dy.device) if on else None  # noqa: E731
+    dx, dup, y = new(True), new(gated), new(recompute)
+    L.check(L.L.dc_act_backward_device(k, code, rows, cols, d2.data_ptr(), ldd, checkpoint.kept.data_ptr(),
+                                       _ptr(checkpoint.kept_up), dx.data_ptr(), cols, _ptr(dup), cols, _ptr(y), cols, stream),
+            "act_backward")
+    got = tuple(t for t in (dx, dup, y) if t is not None)
+    return got if len(got) > 1 else dx
+
+
+_activation = None
+
+
+def activation(x, kind, up=None):
+    """act_forward's output as a differentiable torch function: between the passes it holds the 8-bit checkpoint instead
+    of its inputs, and its gradient is that at the checkpoint's values.  Not differentiable twice."""
+    global _activation
+    import torch
+    if _activation is None:
+        class Activation(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, x, up, kind):
+                y, c = act_forward(x, kind, up)
+                ctx.kind, ctx.shape, ctx.dtype = kind, c.shape, c.dtype
+                ctx.save_for_backward(*(t for t in (c.kept, c.kept_up) if t is not None))
+                return y
+
+            @staticmethod
+            @torch.autograd.function.once_differentiable
+            def backward(ctx, dy):
+                c = ActCheckpoint(ctx.shape, ctx.dtype, *ctx.saved_tensors)
+                got = act_backward(dy, c, ctx.kind)
+                return (got[0], got[1], None) if isinstance(got, tuple) else (got, None, None)
+
+        _activation = Activation
+    return _activation.apply(x, up, kind)

@@ -276,6 +276,82 @@ unsigned dc64_last_decode_flags(void);            /* after finish: 1 = the exact
 int dc64_to_small_device(const void* d_x, long long n, void* d_out, double* min_out);   /* synchronous */
 int dc64_med_device(const void* d_x, long long n, double* mean_out, int* type_out);     /* synchronous */
 
+/* ---- floats held in 8 or 4 bits in HBM (no reference counterpart) --------------------------------------
+ * Fixed-rate codes next to the variable-rate streams above: any position can be written, read and computed from in
+ * place.  A key/value cache of a decoder (4 or 8 bits) with the attention that reads it, and 8-bit checkpoints of
+ * activations with the backward pass that uses them.  All calls are asynchronous on `stream`, a hipStream_t (NULL is
+ * HIP's default stream, dc_get_stream() the library's); they keep no state between calls but the sticky status word,
+ * read nothing back and may be recorded into a graph (call dc_init first).  Arrays lie on the library's device.
+ *
+ * Element types of arrays: */
+enum { DC_F32 = 0, DC_F16 = 1, DC_BF16 = 2 };
+
+/* A cache: `pages` pages of page_size tokens (a multiple of 16) for `heads` heads of head_dim (a multiple of 32, at most
+ * 256) in `bits` (4 or 8).  A row (one token, one head, keys or values) is held as codes with one step and one zero
+ * point: with n = 2^bits - 1,  x^ = step (zero + code),  step the smallest bfloat16 >= max(span / n, amax / 32512,
+ * 2^-100), zero = rint(min / step), codes the nearest: |x - x^| <= step / 2 (to f32's rounding of the span).  A row with a
+ * value that is not finite is NaN.  data: pages * dc_kv_page_bytes bytes, 16-byte aligned. */
+typedef struct dc_kv_cache {
+    void* data;
+    long long pages;
+    int page_size, heads, head_dim, bits;
+} dc_kv_cache;
+/* Which positions of which sequences (device arrays of 32-bit integers): sequence b has lens[b] (NULL: `tokens`) tokens
+ * in this call, the first at position start[b]; position p is in page table[b * table_stride + p / page_size] (table
+ * NULL: page b is sequence b's only one).  table_width: entries per sequence.  Rows from lens[b] on are padding: they
+ * are neither read nor written.  Attention: start[b] is the number of positions of sequence b, its lens[b] query tokens
+ * being the last of them. */
+typedef struct dc_kv_batch {
+    int batch, tokens;
+    const int *start, *lens, *table;
+    int table_width;
+    long long table_stride;
+} dc_kv_batch;
+/* Bytes of a page (0: sizes that are not supported). */
+size_t dc_kv_page_bytes(int page_size, int heads, int head_dim, int bits);
+/* Quantise keys and values [batch][tokens][heads][head_dim] (strides of batch, token and head in elements; the head's
+ * values are consecutive) into the cache.  No two tokens of one call may have the same place (that place then holds a
+ * mix).  Tokens at a position or in a page outside the cache are dropped (status bit 0). */
+int dc_kv_write_device(const dc_kv_cache* cache, const dc_kv_batch* at, int dtype, const void* d_k,
+                       const long long* k_strides, const void* d_v, const long long* v_strides, void* stream);
+/* Read them back (rounded to dtype, held at its largest finite value).  Positions and pages outside the cache read as
+ * NaN (status bit 0). */
+int dc_kv_read_device(const dc_kv_cache* cache, const dc_kv_batch* at, int dtype, void* d_k, const long long* k_strides,
+                      void* d_v, const long long* v_strides, void* stream);
+/* Attention over the cache as it is held: out = softmax(scale q k^T) v for queries [batch][tokens][q_heads][head_dim] (f16
+ * or bf16; q_heads a multiple of the cache's heads, consecutive ones share a head).  causal: query token i sees positions
+ * < start[b] - lens[b] + 1 + i, otherwise all start[b].  A query that sees nothing has output 0 and lse -inf.  Tokens in
+ * pages outside the cache are left out, and a start[b] outside it is held at its bounds (status bit 0).  d_lse (f32
+ * [batch][tokens][q_heads], may be NULL) receives the log of the softmax's sum.  max_context: no start[b] is expected above it (it
+ * sizes the split along the cache; a longer one is still computed in full).  d_workspace: dc_kv_attention_workspace
+ * bytes (16-byte aligned; NULL where that is 0), in use until the call's work is done: calls that may run at once need
+ * one each.  Outputs must not overlap the inputs. */
+size_t dc_kv_attention_workspace(const dc_kv_cache* cache, int batch, int tokens, int q_heads, long long max_context);
+int dc_kv_attention_device(const dc_kv_cache* cache, const dc_kv_batch* at, int dtype, int q_heads, const void* d_q,
+                           const long long* q_strides, float scale, int causal, long long max_context, void* d_out,
+                           const long long* out_strides, float* d_lse, void* d_workspace, size_t workspace_bytes,
+                           void* stream);
+/* The sticky status word of the cache's operators after the work queued on `stream`: bit 0, a position or page outside a
+ * cache.  reset = 1 clears it.  Synchronous (refused while the stream is being captured). */
+int dc_kv_status(void* stream, unsigned* status_out, int reset);
+
+/* Activation checkpoints: rows x cols values, groups of 32 consecutive ones (in the order of the rows) share a power of
+ * two 2^k, the smallest with amax <= 127.5 * 2^k and k >= -126; code = rint(x / 2^k) held to [-127, 127], so |x - x^| <=
+ * 2^(k-1).  A value that is not finite comes back as NaN.  Bytes of a checkpoint of n values (n < 2^35): */
+enum { DC_ACT_NONE = 0, DC_ACT_SILU = 1, DC_ACT_GELU = 2 };
+size_t dc_act_bytes(long long n);
+/* y = f(x) (d_up NULL) or f(x) up, and the checkpoints of x (and up); kind DC_ACT_NONE: the checkpoint alone (d_up and d_y
+ * NULL).  ld*: elements between the starts of rows.  Checkpoints are 16-byte aligned. */
+int dc_act_forward_device(int kind, int dtype, long long rows, long long cols, const void* d_x, long long ldx,
+                          const void* d_up, long long ldup, void* d_y, long long ldy, void* d_kept, void* d_kept_up,
+                          void* stream);
+/* The backward pass at the checkpoint's values x^: dx = dy f'(x^), gated: dx = dy up^ f'(x^) and dup = dy f(x^); d_y
+ * (may be NULL) receives f(x^) (gated: f(x^) up^) again, for the gradient of what used y.  kind DC_ACT_NONE: the
+ * values read back into d_dx (d_dy and d_y NULL), held at dtype's largest finite value. */
+int dc_act_backward_device(int kind, int dtype, long long rows, long long cols, const void* d_dy, long long lddy,
+                           const void* d_kept, const void* d_kept_up, void* d_dx, long long lddx, void* d_dup,
+                           long long lddup, void* d_y, long long ldy, void* stream);
+
 /* Decoder/encoder geometry (for tests and bench). */
 long long dc_decode_chunk_bits_value(void);                 /* chunk bits of the last decode's build */
 /* Streams of at most this capacity (bytes) decode with the 256-bit-chunk build of the decoder, larger
