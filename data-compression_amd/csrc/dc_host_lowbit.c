@@ -55,6 +55,7 @@ static int common(const dc_kv_cache* c, const dc_kv_batch* at, KvArgs* a) {
     a->start = at->start;
     a->lens = at->lens;
     a->table = at->table;
+    a->zero_padding = at->zero_padding != 0;
     a->table_stride = at->table_stride;
     a->capacity = (long long)c->page_size * (at->table ? at->table_width : 1);
     if (a->capacity > (1ll << 30)) a->capacity = 1ll << 30;      /* positions are 32-bit */
@@ -173,7 +174,9 @@ int dc_kv_attention_device(const dc_kv_cache* cache, const dc_kv_batch* at, int 
     memcpy(a.ks, q_strides, sizeof a.ks);
     memcpy(a.vs, out_strides, sizeof a.vs);
     a.dtype = dtype;
+    const unsigned piece = low_bit((unsigned)(cache->head_dim / 16 * 2));
     a.vec = fits(d_q, q_strides, 2, 16);
+    a.vec_out = fits(d_out, out_strides, 2, piece > 16 ? 16 : piece);
     a.causal = causal != 0;
     a.scale = scale;
     a.lse = d_lse;
@@ -214,7 +217,7 @@ static int act_call(ActArgs* a, int back, void* stream) {
     const int size = size_of(a->dtype);
     if (!size) REFUSE("activation: dtype is DC_F32, DC_F16 or DC_BF16");
     if (a->kind != DC_ACT_NONE && a->kind != DC_ACT_SILU && a->kind != DC_ACT_GELU) REFUSE("activation: unknown kind");
-    if (a->rows < 0 || a->cols < 0 || (a->cols && a->rows >= (1ll << 35) / a->cols)) REFUSE("activation: fewer than 2^35 values");
+    if (a->rows < 0 || a->cols < 0 || (a->cols && a->rows > ((1ll << 35) - 1) / a->cols)) REFUSE("activation: fewer than 2^35 values");
     if (a->rows == 0 || a->cols == 0) return DC_OK;
     const int works = a->kind != DC_ACT_NONE;
     if (!a->kept || (a->gated && !a->kept_up)) REFUSE("activation: a checkpoint is missing");

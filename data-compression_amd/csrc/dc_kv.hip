@@ -114,7 +114,7 @@ static __device__ __forceinline__ float rint_div(float x, float s, float inv, fl
     return up ? r + copysignf(1.0f, d) : r;
 }
 
-struct Row { long long page; int at; bool ok, bad; };
+struct Row { long long page; int at; bool ok; };
 
 // position pos of sequence b: its page and place, ok if it is inside the cache
 static __device__ __forceinline__ Row locate(const KvArgs& a, int b, long long pos) {
@@ -201,8 +201,10 @@ template <class E, int D, int BITS, bool VEC> __global__ __launch_bounds__(256) 
     const int kv = (int)(row & 1);
     const uint32_t th = (uint32_t)(row >> 1), bt = div_by(th, a.heads_inv), h = th - bt * a.heads;
     const uint32_t b = div_by(bt, a.tokens_inv), t = bt - b * a.tokens;
-    if (a.lens && (int)t >= a.lens[b]) return;
-    const Row r = locate(a, (int)b, (long long)a.start[b] + t);
+    const bool pad = a.lens && (int)t >= a.lens[b];
+    if (pad && !a.zero_padding) return;
+    Row r = {};
+    if (!pad) r = locate(a, (int)b, (long long)a.start[b] + t);
     typename E::T* dst = kv ? (typename E::T*)a.v + b * a.vs[0] + t * a.vs[1] + h * a.vs[2]
                             : (typename E::T*)a.k + b * a.ks[0] + t * a.ks[1] + h * a.ks[2];
     alignas(16) typename E::T out[N];
@@ -222,9 +224,9 @@ template <class E, int D, int BITS, bool VEC> __global__ __launch_bounds__(256) 
             out[i] = E::from(x != x ? x : fminf(fmaxf(x, -E::MOST), E::MOST));
         }
     } else {
-        if (c == 0) atomicOr(a.status, 1u);
+        if (!pad && c == 0) atomicOr(a.status, 1u);
 #pragma unroll
-        for (int i = 0; i < N; i++) out[i] = E::from(asf(0x7FC00000u));
+        for (int i = 0; i < N; i++) out[i] = E::from(pad ? 0.0f : asf(0x7FC00000u));
     }
     store_n<typename E::T, N, AL>(dst + c * N, out);
 }
@@ -300,6 +302,26 @@ template <int U> struct Stage {         // what a lane holds of 32 tokens: 2 blo
     u4 kw[2], vw[2];
 };
 
+// a query row's N values from d0 on, and (with the first of them, LSE) the log of its sum
+template <int N, bool LSE = true> static __device__ __forceinline__ void put(const KvArgs& a, uint32_t b, uint32_t h, int rw, int d0, const float* o, float lse) {
+    const int i = (int)div_by((uint32_t)rw, a.group_inv), hq = (int)h * a.group + rw - i * a.group;
+    const long long at = b * a.vs[0] + (long long)i * a.vs[1] + (long long)hq * a.vs[2] + d0;
+    if (a.dtype == DC_BF16) {
+        alignas(16) uint16_t raw[N];
+#pragma unroll
+        for (int k = 0; k < N; k++) raw[k] = BF16::from(o[k]);
+        if (a.vec_out) store_n<uint16_t, N, (2 * N & -(2 * N))>((uint16_t*)a.v + at, raw);
+        else store_n<uint16_t, N, 2>((uint16_t*)a.v + at, raw);
+    } else {
+        alignas(16) _Float16 raw[N];
+#pragma unroll
+        for (int k = 0; k < N; k++) raw[k] = (_Float16)o[k];
+        if (a.vec_out) store_n<_Float16, N, (2 * N & -(2 * N))>((_Float16*)a.v + at, raw);
+        else store_n<_Float16, N, 2>((_Float16*)a.v + at, raw);
+    }
+    if (LSE && a.lse && d0 == 0) a.lse[((long long)b * a.tokens + i) * a.heads * a.group + hq] = lse;
+}
+
 template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_attention(KvArgs a) {
     constexpr int N = D / 16, U = N * BITS / 8, ROW = 16 * U, KS = D / 32, COLS = 16 * NT;
     constexpr float BIAS = (float)(1 << (BITS - 1));
@@ -321,6 +343,14 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_att
     const int len = a.lens ? min(max(a.lens[b], 0), a.tokens) : a.tokens;
     const int rows = len * a.group;
     const int row0 = tile * COLS;
+    const int oc = threadIdx.x & 15, ou = threadIdx.x >> 4;     // a thread's output: a row, a unit
+    if (a.zero_padding && a.splits == 1) {
+        const float zero[N] = {};
+        for (int nt = 0; nt < NT; nt++) {
+            const int rw = row0 + nt * 16 + oc;
+            if (rw >= rows && rw < (int)a.row_slots) put<N, false>(a, b, h, rw, ou * N, zero, 0.0f);
+        }
+    }
     if (row0 >= rows) return;
     // what each query row of the tile sees: positions < sees
     int sees[NT], most = 0;
@@ -562,7 +592,6 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_att
         __syncthreads();
     }
     // 16 columns x 16 units: a thread writes the N values of its unit
-    const int oc = threadIdx.x & 15, ou = threadIdx.x >> 4;
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
         const int rw = row0 + nt * 16 + oc;
@@ -581,7 +610,6 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_att
             for (int v = 0; v < (ALL ? 4 : 1); v++) y += acc_lds[((v * NT + nt) * N + i) * 256 + ou * 16 + oc];
             o[i] = y;
         }
-        const int i = (int)div_by((uint32_t)rw, a.group_inv), gi = rw - i * a.group;
         if (a.splits > 1) {                                 // unnormalised, with its maximum and sum
             const long long at = ((((long long)b * a.heads + h) * a.row_slots + rw) * a.splits + split);
             float* p = a.part + at * D + ou * N;
@@ -592,19 +620,11 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_att
             }
             continue;
         }
-        const bool none = (a.causal ? context - len + 1 + i : context) <= 0;
+        const bool none = (a.causal ? context - len + 1 + (int)div_by((uint32_t)rw, a.group_inv) : context) <= 0;
         const float inv = 1.0f / l;
-        const long long at = b * a.vs[0] + (long long)i * a.vs[1] + (long long)(h * a.group + gi) * a.vs[2] + ou * N;
-        if (a.dtype == DC_BF16) {
-            uint16_t* p = (uint16_t*)a.v + at;
-            for (int k = 0; k < N; k++) p[k] = BF16::from(none ? 0.0f : o[k] * inv);
-        } else {
-            _Float16* p = (_Float16*)a.v + at;
-            for (int k = 0; k < N; k++) p[k] = (_Float16)(none ? 0.0f : o[k] * inv);
-        }
-        if (a.lse && ou == 0)
-            a.lse[((long long)b * a.tokens + i) * a.heads * a.group + h * a.group + gi] =
-                none ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
+#pragma unroll
+        for (int k = 0; k < N; k++) o[k] = none ? 0.0f : o[k] * inv;
+        put<N>(a, b, h, rw, ou * N, o, none ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f);
     }
 }
 
@@ -617,7 +637,12 @@ template <int D> __global__ __launch_bounds__(256) void kv_join(KvArgs a) {
     const uint32_t rw = x % a.row_slots; x /= a.row_slots;
     const uint32_t h = x % a.heads, b = x / a.heads;
     const int len = a.lens ? min(max(a.lens[b], 0), a.tokens) : a.tokens;
-    if ((int)rw >= len * a.group) return;
+    if ((int)rw >= len * a.group) {
+        const float zero = 0.0f;
+        if (a.zero_padding)
+            for (int d = threadIdx.x; d < D; d += 256) put<1, false>(a, b, h, (int)rw, d, &zero, 0.0f);
+        return;
+    }
     const int u = threadIdx.x & 15, part = threadIdx.x >> 4;
     const long long at = (((long long)b * a.heads + h) * a.row_slots + rw) * a.splits;
     float m = -1e30f, l = 0.0f, o[N];
@@ -641,21 +666,16 @@ template <int D> __global__ __launch_bounds__(256) void kv_join(KvArgs a) {
         f[k] = __builtin_amdgcn_exp2f(ms[k] - m);
         l = fmaf(lsum[k], f[k], l);
     }
-    const int i = (int)div_by(rw, a.group_inv), gi = (int)rw - i * a.group;
     int context = a.start[b];
     context = context < 0 ? 0 : context > a.capacity ? (int)a.capacity : context;
-    const bool none = (a.causal ? context - len + 1 + i : context) <= 0;
-    const long long out = b * a.vs[0] + (long long)i * a.vs[1] + (long long)(h * a.group + gi) * a.vs[2];
+    const bool none = (a.causal ? context - len + 1 + (int)div_by(rw, a.group_inv) : context) <= 0;
+    const float lse = none ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
     for (int d = threadIdx.x; d < D; d += 256) {
         float y = 0.0f;
         for (int k = 0; k < 16; k++) y = fmaf(sums[k][d], f[k], y);
         y = none ? 0.0f : y / l;
-        if (a.dtype == DC_BF16) ((uint16_t*)a.v)[out + d] = BF16::from(y);
-        else ((_Float16*)a.v)[out + d] = (_Float16)y;
+        put<1>(a, b, h, (int)rw, d, &y, lse);
     }
-    if (a.lse && threadIdx.x == 0)
-        a.lse[((long long)b * a.tokens + i) * a.heads * a.group + h * a.group + gi] =
-            none ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
 }
 
 template <class E, int BITS, bool VEC> int go_rows(const KvArgs& a, bool write, hipStream_t st) {

@@ -118,7 +118,8 @@ typedef struct KvArgs {
     const void* k;                 /* write: keys, read: keys out, attention: queries; strides (batch, token, head) in elements */
     const void* v;                 /* write: values, read: values out, attention: the output */
     long long ks[3], vs[3];
-    int dtype, vec;                /* vec: pointers and strides allow whole-lane accesses */
+    int zero_padding;              /* outputs behind lens[b]: 0 (1) or left as they are */
+    int dtype, vec, vec_out;       /* vec: pointers and strides allow whole-lane accesses */
     long long rows;                /* write / read: batch * tokens * heads * 2 */
     unsigned* status;
     int group, causal;             /* attention: query heads per head of the cache */

@@ -72,7 +72,7 @@ class KvCacheDesc(C.Structure):     # dc_kv_cache
 
 class KvBatchDesc(C.Structure):     # dc_kv_batch
     _fields_ = [("batch", C.c_int), ("tokens", C.c_int), ("start", C.c_void_p), ("lens", C.c_void_p),
-                ("table", C.c_void_p), ("table_width", C.c_int), ("table_stride", C.c_longlong)]
+                ("table", C.c_void_p), ("table_width", C.c_int), ("table_stride", C.c_longlong), ("zero_padding", C.c_int)]
 
 
 class Lib:
@@ -1231,39 +1231,48 @@ def lib():
 
 
 # ---- floats held in 8 or 4 bits in HBM: torch tensors on the current stream ------------------------------------------
+# (Single tokens are bound by the host's side of a call, about 3 us of which are the launch's: torch is looked up once,
+# types are compared by identity, strides and streams are asked for in one call each.)
 DC_F32, DC_F16, DC_BF16 = 0, 1, 2
-ACT_KINDS = {"none": 0, "silu": 1, "gelu": 2}
+ACT_KINDS = {"silu": 1, "gelu": 2}
 _Strides = C.c_longlong * 3
+_torch = None
+_codes = {}
 
 
-def _dtype_code(dtype, allowed="f32, f16 or bf16"):
-    import torch
-    code = {torch.float32: DC_F32, torch.float16: DC_F16, torch.bfloat16: DC_BF16}.get(dtype)
-    if code is None or (code == DC_F32 and "f32" not in allowed):
-        raise ValueError(f"dtype {dtype}: {allowed} is needed")
+def _need_torch():
+    global _torch
+    if _torch is None:
+        import torch
+        _torch = torch
+        _codes.update({torch.float32: DC_F32, torch.float16: DC_F16, torch.bfloat16: DC_BF16})
+    return _torch
+
+
+def _dtype_code(dtype):
+    _need_torch()
+    code = _codes.get(dtype)
+    if code is None:
+        raise ValueError(f"dtype {dtype}: f32, f16 or bf16 is needed")
     return code
 
 
 def _on_gpu(*tensors):
-    """The stream to launch on: all tensors lie on the library's device, which is made torch's current one by the caller
-    (`with torch.cuda.device(...)`) if it is not."""
-    import torch
-    L = lib()
-    for t in tensors:
-        if t is not None and not t.is_cuda:
-            raise ValueError("tensors must lie on the GPU")
+    """The library and torch's current stream, after checking that all tensors lie on the library's device and that it
+    is the current one (a caller with several devices says `with torch.cuda.device(...)`)."""
+    T = _need_torch()
+    L = _lib or lib()
     if L.device is None:
-        L.init(tensors[0].device.index)
+        if not tensors[0].is_cuda:
+            raise ValueError("tensors must lie on the GPU")
+        L.init(tensors[0].get_device())
+    dev = L.device
     for t in tensors:
-        if t is not None and t.device.index != L.device:
-            raise ValueError(f"tensors must lie on the library's device (cuda:{L.device})")
-    if torch.cuda.current_device() != L.device:
-        raise ValueError(f"the current device must be the library's (cuda:{L.device})")
-    return L, torch.cuda.current_stream().cuda_stream
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensors must lie on the library's device (cuda:{dev})")
+    if T._C._cuda_getDevice() != dev:
+        raise ValueError(f"the current device must be the library's (cuda:{dev})")
+    return L, T._C._cuda_getCurrentRawStream(dev)
 
 
 class KVCache:
@@ -1277,13 +1286,13 @@ class KVCache:
     captured into a graph."""
 
     def __init__(self, pages, page_size, heads, head_dim, bits=4, buffer=None, device="cuda"):
+        T = _need_torch()
         page = self.page_bytes(page_size, heads, head_dim, bits)
         if pages < 1:
             raise ValueError("a cache has at least one page")
         if buffer is None:
-            import torch
-            buffer = torch.zeros(pages * page, dtype=torch.uint8, device=device)
-        if str(buffer.dtype) != "torch.uint8" or not buffer.is_contiguous() or buffer.numel() < pages * page:
+            buffer = T.zeros(pages * page, dtype=T.uint8, device=device)
+        if buffer.dtype is not T.uint8 or not buffer.is_contiguous() or buffer.numel() < pages * page:
             raise ValueError(f"buffer: {pages * page} contiguous bytes (uint8) are needed")
         if buffer.data_ptr() % 16:
             raise ValueError("buffer: 16-byte alignment is needed")
@@ -1299,108 +1308,141 @@ class KVCache:
             raise ValueError("page_size is a multiple of 16, head_dim a multiple of 32 up to 256, bits 4 or 8")
         return n
 
-    def _batch(self, batch, tokens, start, table, lens, what="start"):
-        for name, t in ((what, start), ("lens", lens)):
-            if t is not None and (str(t.dtype) != "torch.int32" or t.shape != (batch,) or not t.is_contiguous()):
-                raise ValueError(f"{name}: contiguous int32 of ({batch},) is needed")
+    def _batch(self, batch, tokens, start, table, lens, pad, what="start"):
+        i32 = _torch.int32
+        if start.dtype is not i32 or start.shape != (batch,) or not start.is_contiguous():
+            raise ValueError(f"{what}: contiguous int32 of ({batch},) is needed")
+        n = None
+        if lens is not None:
+            if lens.dtype is not i32 or lens.shape != (batch,) or not lens.is_contiguous():
+                raise ValueError(f"lens: contiguous int32 of ({batch},) is needed")
+            n = lens.data_ptr()
         if table is None:
             if batch > self.pages:
                 raise ValueError("without a table each sequence has a page")
-            return KvBatchDesc(batch, tokens, start.data_ptr(), _ptr(lens), None, 0, 0)
-        if str(table.dtype) != "torch.int32" or table.dim() != 2 or table.shape[0] != batch or table.shape[1] < 1 or \
-                table.stride(1) != 1 or (batch > 1 and table.stride(0) < table.shape[1]):
-            raise ValueError(f"table: int32 of ({batch}, pages of a sequence) with consecutive entries is needed")
-        return KvBatchDesc(batch, tokens, start.data_ptr(), _ptr(lens), table.data_ptr(), table.shape[1],
-                           max(table.stride(0), table.shape[1]))
+            return KvBatchDesc(batch, tokens, start.data_ptr(), n, None, 0, 0, pad)
+        shape = table.shape
+        if table.dtype is i32 and len(shape) == 2 and shape[0] == batch and shape[1] >= 1:
+            stride, one = table.stride()
+            if one == 1 and (batch <= 1 or stride >= shape[1]):
+                return KvBatchDesc(batch, tokens, start.data_ptr(), n, table.data_ptr(), shape[1], max(stride, shape[1]), pad)
+        raise ValueError(f"table: int32 of ({batch}, pages of a sequence) with consecutive entries is needed")
 
-    def _rows(self, x, name, heads=None):
-        if x.dim() != 4 or x.shape[3] != self.head_dim or (heads is None and x.shape[2] != self.heads):
-            raise ValueError(f"{name}: (batch, tokens, {self.heads if heads is None else 'heads'}, {self.head_dim}) is needed")
-        if x.stride(3) != 1 and x.numel():
+    def _rows(self, x, name, heads):
+        shape = x.shape
+        if len(shape) != 4 or shape[3] != self.head_dim or (heads and shape[2] != heads):
+            raise ValueError(f"{name}: (batch, tokens, {heads or 'heads'}, {self.head_dim}) is needed")
+        a, b, c, one = x.stride()
+        if one != 1 and x.numel():
             raise ValueError(f"{name}: a head's values must be consecutive")
-        return _Strides(x.stride(0), x.stride(1), x.stride(2))
+        return _Strides(a, b, c)
 
     def write(self, k, v, start, table=None, lens=None):
         """Quantise k, v (batch, tokens, heads, head_dim) to positions start[b] .. of each sequence."""
-        ks, vs = self._rows(k, "k"), self._rows(v, "v")
-        if k.shape != v.shape or k.dtype != v.dtype:
+        ks, vs = self._rows(k, "k", self.heads), self._rows(v, "v", self.heads)
+        shape = k.shape
+        if shape != v.shape or k.dtype is not v.dtype:
             raise ValueError("k and v differ in shape or type")
         code = _dtype_code(k.dtype)
-        at = self._batch(k.shape[0], k.shape[1], start, table, lens)
+        at = self._batch(shape[0], shape[1], start, table, lens, 0)
         L, stream = _on_gpu(self.buffer, k, v, start, table, lens)
-        L.check(L.L.dc_kv_write_device(self._desc, at, code, k.data_ptr(), ks, v.data_ptr(), vs, stream), "kv_write")
+        rc = L.L.dc_kv_write_device(self._desc, at, code, k.data_ptr(), ks, v.data_ptr(), vs, stream)
+        if rc:
+            L.check(rc, "kv_write")
 
     def read(self, start, tokens, table=None, lens=None, dtype=None, out=None):
         """The keys and values of positions start[b] .. start[b] + tokens as floats of `dtype` (bf16), in `out` if given
         (rows of padding keep what they have), else in new tensors (padding is 0)."""
-        import torch
+        T = _torch
         batch = start.shape[0] if start.dim() else 0
-        at = self._batch(batch, tokens, start, table, lens)
+        at = self._batch(batch, tokens, start, table, lens, out is None)
         if out is None:
-            new = torch.empty if lens is None else torch.zeros
-            dtype = dtype or torch.bfloat16
-            out = [new((batch, tokens, self.heads, self.head_dim), dtype=dtype, device=self.buffer.device) for _ in range(2)]
-        k, v = out
-        ks, vs = self._rows(k, "out"), self._rows(v, "out")
-        if k.shape != v.shape or k.dtype != v.dtype or k.shape[:2] != (batch, tokens) or (dtype and k.dtype != dtype):
-            raise ValueError("out: two tensors (batch, tokens, heads, head_dim) of the type asked for are needed")
-        code = _dtype_code(k.dtype)
-        L, stream = _on_gpu(self.buffer, k, v, start, table, lens)
-        L.check(L.L.dc_kv_read_device(self._desc, at, code, k.data_ptr(), ks, v.data_ptr(), vs, stream), "kv_read")
+            code = _dtype_code(dtype or T.bfloat16)
+            L, stream = _on_gpu(self.buffer, start, table, lens)
+            k = T.empty((batch, tokens, self.heads, self.head_dim), dtype=dtype or T.bfloat16, device=self.buffer.device)
+            v = T.empty_like(k)
+            ks = vs = _Strides(*k.stride()[:3])
+        else:
+            k, v = out
+            ks, vs = self._rows(k, "out", self.heads), self._rows(v, "out", self.heads)
+            if k.shape != v.shape or k.dtype is not v.dtype or k.shape[:2] != (batch, tokens) or (dtype and k.dtype is not dtype):
+                raise ValueError("out: two tensors (batch, tokens, heads, head_dim) of the type asked for are needed")
+            code = _dtype_code(k.dtype)
+            L, stream = _on_gpu(self.buffer, start, table, lens, k, v)
+        rc = L.L.dc_kv_read_device(self._desc, at, code, k.data_ptr(), ks, v.data_ptr(), vs, stream)
+        if rc:
+            L.check(rc, "kv_read")
         return k, v
 
     def attention(self, q, context, table=None, lens=None, scale=None, causal=True, max_context=None, out=None, lse=None):
         """softmax(scale q k^T) v over the first context[b] positions of each sequence, q (batch, tokens, q_heads, head_dim)
         in f16 or bf16 being its last lens[b] (None: all) tokens: causal, token i sees context[b] - lens[b] + 1 + i of
         them.  scale: 1 / sqrt(head_dim).  max_context: the longest context expected (the table's capacity).  out: where
-        to put the output (rows of padding keep what they have; else they are 0); lse: an f32 tensor (batch, tokens,
-        q_heads) for the log of each softmax's sum."""
-        import torch
-        qs = self._rows(q, "q", heads="any")
-        code = _dtype_code(q.dtype, "f16 or bf16")
+        to put the output (rows of padding keep what they have; in a new tensor they are 0); lse: an f32 tensor (batch,
+        tokens, q_heads) for the log of each softmax's sum."""
+        T = _torch
+        qs = self._rows(q, "q", 0)
+        code = _dtype_code(q.dtype)
+        if code == DC_F32:
+            raise ValueError("q: f16 or bf16 is needed")
         batch, tokens, q_heads, _ = q.shape
         if q_heads < 1 or q_heads % self.heads:
             raise ValueError(f"q: heads in a multiple of the cache's {self.heads} are needed")
-        at = self._batch(batch, tokens, context, table, lens, "context")
-        capacity = self.page_size * (1 if table is None else table.shape[1])
-        limit = capacity if max_context is None else min(int(max_context), capacity)
-        if limit < 0:
-            raise ValueError("max_context is not negative")
-        if out is None:
-            out = (torch.empty if lens is None else torch.zeros)(q.shape, dtype=q.dtype, device=q.device)
-        os_ = self._rows(out, "out", heads="any")
-        if out.shape != q.shape or out.dtype != q.dtype:
-            raise ValueError("out: q's shape and type are needed")
-        if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:3] or not lse.is_contiguous()):
+        at = self._batch(batch, tokens, context, table, lens, out is None, "context")
+        limit = self.page_size * (1 if table is None else at.table_width)
+        if max_context is not None:
+            if max_context < 0:
+                raise ValueError("max_context is not negative")
+            limit = min(int(max_context), limit)
+        if lse is not None and (lse.dtype is not T.float32 or lse.shape != q.shape[:3] or not lse.is_contiguous()):
             raise ValueError("lse: contiguous float32 of (batch, tokens, q_heads) is needed")
-        L, stream = _on_gpu(self.buffer, q, context, table, lens, out, lse)
+        if out is None:
+            L, stream = _on_gpu(self.buffer, q, context, table, lens, lse)
+            out = T.empty_like(q, memory_format=T.contiguous_format)
+            os_ = _Strides(*out.stride()[:3])
+        else:
+            os_ = self._rows(out, "out", 0)
+            if out.shape != q.shape or out.dtype is not q.dtype:
+                raise ValueError("out: q's shape and type are needed")
+            L, stream = _on_gpu(self.buffer, q, context, table, lens, lse, out)
         need = L.L.dc_kv_attention_workspace(self._desc, batch, tokens, q_heads, limit)
-        space = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        L.check(L.L.dc_kv_attention_device(self._desc, at, code, q_heads, q.data_ptr(), qs,
-                                           self.head_dim ** -0.5 if scale is None else float(scale), int(bool(causal)), limit,
-                                           out.data_ptr(), os_, _ptr(lse), _ptr(space), need, stream), "kv_attention")
+        space = T.empty(need, dtype=T.uint8, device=q.device) if need else None
+        rc = L.L.dc_kv_attention_device(self._desc, at, code, q_heads, q.data_ptr(), qs,
+                                        self.head_dim ** -0.5 if scale is None else scale, bool(causal), limit, out.data_ptr(),
+                                        os_, lse.data_ptr() if lse is not None else None,
+                                        space.data_ptr() if need else None, need, stream)
+        if rc:
+            L.check(rc, "kv_attention")
         return out
 
     @staticmethod
     def status(reset=False):
         """The sticky status word after the work queued on the current stream (synchronous): 1, a position or page outside
         its cache (then dropped, read as NaN or left out)."""
-        import torch
         L, v = lib(), C.c_uint(0)
-        L.check(L.L.dc_kv_status(torch.cuda.current_stream().cuda_stream, C.byref(v), int(bool(reset))), "kv_status")
+        L.check(L.L.dc_kv_status(_need_torch().cuda.current_stream().cuda_stream, C.byref(v), int(bool(reset))), "kv_status")
         return int(v.value)
 
 
 def _flat(x):
     """x as rows of its last dimension: (tensor, rows, cols, elements between rows); copied if its rows do not lie so."""
-    cols = x.shape[-1] if x.dim() else 1
-    rows = x.numel() // cols if cols else 0
-    if x.is_contiguous():
-        return x, rows, cols, cols
-    y = x.reshape(rows, cols)
+    if x.is_contiguous():                                   # one row
+        n = x.numel()
+        return x, 1, n, n
+    cols = x.shape[-1]
+    y = x.reshape(x.numel() // cols, cols)
     if y.stride(1) != 1 or y.stride(0) < cols:
         y = y.contiguous()
-    return y, rows, cols, max(y.stride(0), cols)
+    return y, y.shape[0], cols, max(y.stride(0), cols)
+
+
+def _same_rows(a, b):
+    """Two _flat()s with one's rows and cols: an array in one row takes the other's."""
+    if a[1] == 1 and b[1] > 1:
+        return (a[0], b[1], b[2], b[2]), b
+    if b[1] == 1 and a[1] > 1:
+        return a, (b[0], a[1], a[2], a[2])
+    return a, b
 
 
 class ActCheckpoint:
@@ -1408,88 +1450,100 @@ class ActCheckpoint:
     the shape each)."""
 
     def __init__(self, shape, dtype, kept, kept_up=None):
-        self.shape, self.dtype, self.kept, self.kept_up = tuple(shape), dtype, kept, kept_up
-        n = 1
-        for s in self.shape:
-            n *= s
-        need = lib().L.dc_act_bytes(n)
+        T = _need_torch()
+        self.shape, self.dtype, self.kept, self.kept_up = T.Size(shape), dtype, kept, kept_up
+        need = lib().L.dc_act_bytes(self.shape.numel())
         for t in (kept, kept_up):
-            if t is not None and (str(t.dtype) != "torch.uint8" or not t.is_contiguous() or t.numel() < need):
+            if t is not None and (t.dtype is not T.uint8 or not t.is_contiguous() or t.numel() < need):
                 raise ValueError(f"checkpoint: {need} contiguous bytes (uint8) are needed")
         _dtype_code(dtype)
 
     def load(self):
         """The kept values as floats: a tuple of one tensor, or two of a gated activation."""
-        import torch
-        got = []
+        got, code, n = [], _dtype_code(self.dtype), self.shape.numel()
         for kept in (self.kept, self.kept_up):
             if kept is None:
                 continue
-            x = torch.empty(self.shape, dtype=self.dtype, device=kept.device)
-            _, rows, cols, ld = _flat(x)
             L, stream = _on_gpu(kept)
-            L.check(L.L.dc_act_backward_device(0, _dtype_code(self.dtype), rows, cols, None, 0, kept.data_ptr(), None,
-                                               x.data_ptr(), ld, None, 0, None, 0, stream), "act_load")
+            x = _torch.empty(self.shape, dtype=self.dtype, device=kept.device)
+            rc = L.L.dc_act_backward_device(0, code, 1, n, None, 0, kept.data_ptr(), None, x.data_ptr(), n, None, 0, None, 0,
+                                            stream)
+            if rc:
+                L.check(rc, "act_load")
             got.append(x)
         return tuple(got)
 
 
 def _act_kind(kind):
-    if kind not in ("silu", "gelu"):
+    code = ACT_KINDS.get(kind)
+    if code is None:
         raise ValueError(f"kind {kind!r}: 'silu' or 'gelu' is needed")
-    return ACT_KINDS[kind]
-
-
-def _new_kept(n, device):
-    import torch
-    return torch.empty(lib().L.dc_act_bytes(n), dtype=torch.uint8, device=device)
+    return code
 
 
 def act_save(x):
     """x (f32, f16, bf16) as an ActCheckpoint."""
     code = _dtype_code(x.dtype)
-    x2, rows, cols, ld = _flat(x)
     L, stream = _on_gpu(x)
-    kept = _new_kept(x.numel(), x.device)
-    L.check(L.L.dc_act_forward_device(0, code, rows, cols, x2.data_ptr(), ld, None, 0, None, 0, kept.data_ptr(), None, stream),
-            "act_save")
+    x2, rows, cols, ld = _flat(x)
+    T = _torch
+    kept = T.empty(L.L.dc_act_bytes(x.numel()), dtype=T.uint8, device=x.device)
+    rc = L.L.dc_act_forward_device(0, code, rows, cols, x2.data_ptr(), ld, None, 0, None, 0, kept.data_ptr(), None, stream)
+    if rc:
+        L.check(rc, "act_save")
     return ActCheckpoint(x.shape, x.dtype, kept)
 
 
 def act_forward(x, kind, up=None):
     """y = f(x) (kind 'silu' or 'gelu', the exact one) or f(x) * up, and the ActCheckpoint of x (and up), in one pass."""
-    import torch
     code, k = _dtype_code(x.dtype), _act_kind(kind)
-    if up is not None and (up.shape != x.shape or up.dtype != x.dtype):
+    T = _torch
+    if up is not None and (up.shape != x.shape or up.dtype is not x.dtype):
         raise ValueError("x and up differ in shape or type")
-    x2, rows, cols, ldx = _flat(x)
-    u2, _, _, ldu = _flat(up) if up is not None else (None, 0, 0, 0)
     L, stream = _on_gpu(x, up)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    kept = _new_kept(x.numel(), x.device)
-    kept_up = _new_kept(x.numel(), x.device) if up is not None else None
-    L.check(L.L.dc_act_forward_device(k, code, rows, cols, x2.data_ptr(), ldx, _ptr(u2), ldu, y.data_ptr(), cols,
-                                      kept.data_ptr(), _ptr(kept_up), stream), "act_forward")
+    fx = _flat(x)
+    y = T.empty_like(x, memory_format=T.contiguous_format)
+    n = L.L.dc_act_bytes(x.numel())
+    kept = T.empty(n, dtype=T.uint8, device=x.device)
+    if up is None:
+        x2, rows, cols, ldx = fx
+        rc = L.L.dc_act_forward_device(k, code, rows, cols, x2.data_ptr(), ldx, None, 0, y.data_ptr(), cols, kept.data_ptr(), None,
+                                       stream)
+        kept_up = None
+    else:
+        kept_up = T.empty_like(kept)
+        (x2, rows, cols, ldx), (u2, _, _, ldu) = _same_rows(fx, _flat(up))
+        rc = L.L.dc_act_forward_device(k, code, rows, cols, x2.data_ptr(), ldx, u2.data_ptr(), ldu, y.data_ptr(), cols,
+                                       kept.data_ptr(), kept_up.data_ptr(), stream)
+    if rc:
+        L.check(rc, "act_forward")
     return y, ActCheckpoint(x.shape, x.dtype, kept, kept_up)
 
 
 def act_backward(dy, checkpoint, kind, recompute=False):
     """The gradient of act_forward at the checkpoint's values: dx, or (dx, dup) of a gated activation; with recompute, a
     tuple that ends with the activation's output at those values (for the gradient of what used it)."""
-    import torch
     code, k = _dtype_code(dy.dtype), _act_kind(kind)
-    if tuple(dy.shape) != checkpoint.shape or dy.dtype != checkpoint.dtype:
+    T = _torch
+    if dy.shape != checkpoint.shape or dy.dtype is not checkpoint.dtype:
         raise ValueError("dy and the checkpoint differ in shape or type")
-    gated = checkpoint.kept_up is not None
+    kept, kept_up = checkpoint.kept, checkpoint.kept_up
+    L, stream = _on_gpu(dy, kept, kept_up)
     d2, rows, cols, ldd = _flat(dy)
-    L, stream = _on_gpu(dy, checkpoint.kept, checkpoint.kept_up)
-    new = lambda on: torch.empty(dy.shape, dtype=dy.dtype, device=dy.device) if on else None  # noqa: E731
-    dx, dup, y = new(True), new(gated), new(recompute)
-    L.check(L.L.dc_act_backward_device(k, code, rows, cols, d2.data_ptr(), ldd, checkpoint.kept.data_ptr(),
-                                       _ptr(checkpoint.kept_up), dx.data_ptr(), cols, _ptr(dup), cols, _ptr(y), cols, stream),
-            "act_backward")
-    got = tuple(t for t in (dx, dup, y) if t is not None)
-    return got if len(got) > 1 else dx
+    dx = T.empty_like(dy, memory_format=T.contiguous_format)
+    got, dup, y = [dx], None, None
+    if kept_up is not None:
+        got.append(T.empty_like(dx))
+        dup = got[-1].data_ptr()
+        kept_up = kept_up.data_ptr()
+    if recompute:
+        got.append(T.empty_like(dx))
+        y = got[-1].data_ptr()
+    rc = L.L.dc_act_backward_device(k, code, rows, cols, d2.data_ptr(), ldd, kept.data_ptr(), kept_up, dx.data_ptr(), cols, dup, cols,
+                                    y, cols, stream)
+    if rc:
+        L.check(rc, "act_backward")
+    return tuple(got) if len(got) > 1 else dx
 
 
 _activation = None
@@ -1499,9 +1553,10 @@ def activation(x, kind, up=None):
     """act_forward's output as a differentiable torch function: between the passes it holds the 8-bit checkpoint instead
     of its inputs, and its gradient is that at the checkpoint's values.  Not differentiable twice."""
     global _activation
-    import torch
     if _activation is None:
-        class Activation(torch.autograd.Function):
+        T = _need_torch()
+
+        class Activation(T.autograd.Function):
             @staticmethod
             def forward(ctx, x, up, kind):
                 y, c = act_forward(x, kind, up)
@@ -1510,7 +1565,7 @@ def activation(x, kind, up=None):
                 return y
 
             @staticmethod
-            @torch.autograd.function.once_differentiable
+            @T.autograd.function.once_differentiable
             def backward(ctx, dy):
                 c = ActCheckpoint(ctx.shape, ctx.dtype, *ctx.saved_tensors)
                 got = act_backward(dy, c, ctx.kind)

@@ -298,14 +298,15 @@ typedef struct dc_kv_cache {
 } dc_kv_cache;
 /* Which positions of which sequences (device arrays of 32-bit integers): sequence b has lens[b] (NULL: `tokens`) tokens
  * in this call, the first at position start[b]; position p is in page table[b * table_stride + p / page_size] (table
- * NULL: page b is sequence b's only one).  table_width: entries per sequence.  Rows from lens[b] on are padding: they
- * are neither read nor written.  Attention: start[b] is the number of positions of sequence b, its lens[b] query tokens
- * being the last of them. */
+ * NULL: page b is sequence b's only one).  table_width: entries per sequence.  Rows from lens[b] on are padding: inputs
+ * there are not read, outputs are left as they are (zero_padding 0) or set to 0 (1; the lse is left).  Attention:
+ * start[b] is the number of positions of sequence b, its lens[b] query tokens being the last of them. */
 typedef struct dc_kv_batch {
     int batch, tokens;
     const int *start, *lens, *table;
     int table_width;
     long long table_stride;
+    int zero_padding;
 } dc_kv_batch;
 /* Bytes of a page (0: sizes that are not supported). */
 size_t dc_kv_page_bytes(int page_size, int heads, int head_dim, int bits);

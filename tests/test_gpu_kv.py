@@ -403,6 +403,11 @@ def test_attention_strides_and_padding(kv):
     qv[1, 3:] = math.nan
     f.cache.attention(qv, i32(150, 90), table=f.table, lens=i32(9, 3), out=out)
     assert same(out[0], plain[0]) and same(out[1, :3], plain[1, :3])
+    far = Filled(kv, 43, 1, 3000, 1, 64, 16, 4)                        # split along the cache: padding is set to 0 too
+    for tok, n in ((3, 1), (40, 17), (5, 0)):
+        qq = torch.randn(1, tok, 2, 64, generator=gen(tok)).half()
+        y = far.cache.attention(qq.to(DEV), i32(3000), table=far.table, lens=i32(n))
+        assert bool((y[0, n:] == 0).all())
     assert bool((out[1, 3:] == -3).all()) and bool((store[..., :3] == -3).all()) and bool((store[..., 67:] == -3).all())
 
 

@@ -26,9 +26,9 @@ def desc(d, **k):
 
 
 def batch(d, **k):
-    a = dict(batch=2, tokens=3, start=P, lens=None, table=P, table_width=2, table_stride=2)
+    a = dict(batch=2, tokens=3, start=P, lens=None, table=P, table_width=2, table_stride=2, zero_padding=0)
     a.update(k)
-    return d.KvBatchDesc(*(a[n] for n in ("batch", "tokens", "start", "lens", "table", "table_width", "table_stride")))
+    return d.KvBatchDesc(*(a[n] for n in ("batch", "tokens", "start", "lens", "table", "table_width", "table_stride", "zero_padding")))
 
 
 def test_page_bytes(lib):
