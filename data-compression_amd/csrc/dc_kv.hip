@@ -232,19 +232,23 @@ template <class E, int D, int BITS, bool VEC> __global__ __launch_bounds__(256) 
 }
 
 // ---- attention ---------------------------------------------------------------------------------------------------------
-// O = softmax(scale q k^T) v^ over the positions a query sees.  With k^ = s (z + code), code' = code - 2^(BITS-1) and
-// z' = z + 2^(BITS-1):
-//     q . k^_t = ks_t (q . code'_t + kz'_t sum(q)),      O_d = sum_t (p_t vs_t) (code'_td + vz'_t):
-// the matrix instructions see the codes alone, as f16 whole numbers (exact), and a token's step and zero point enter as
-// two multiply-adds on its score and as a factor of its weight.  The queries of a group of heads that share keys are the
+// O = softmax(scale q k^T) v^ over the positions a query sees.  With k^ = s (z + code):
+//     q . k^_t = ks_t (q . code_t + kz_t sum(q)),      O_d = sum_t (p_t vs_t) (code_td + vz_t):
+// the matrix instructions see the codes alone, as whole numbers (exact), and a token's step and zero point enter as two
+// multiply-adds on its score and as a factor of its weight.  The queries of a group of heads that share keys are the
 // columns of mfma 16x16x32: A = 16 tokens' codes, B = 16 queries.  The score tile's lane layout (token = 4 (lane / 16) +
 // r, query = lane % 16) is that of the weights' operand in the second product if its 32 tokens are taken in the order
 // (block of 16, r) for each group of lanes, and the values' layout in the cache has that order: no data crosses lanes.
 //
+// A code becomes an f16 by its bits alone: in bits 4..7 they are the subnormal code * 2^-20, in bits 0..7 code * 2^-24
+// (UNIT), a power of two that is taken out of the sums.  An instruction's sum keeps 24 bits from its largest product's
+// exponent on, in which a subnormal counts as 2^-14: it is exact to 2^-18 (4 bits; 2^-14: 8 bits) of a code's unit times the
+// largest weight.  (In bits 0..3 that were 2^-14 of 15.)
+//
 // The weights w_t = p_t vs_t go into the product as f16.  A running maximum of log2(p_t) + exponent(vs_t) keeps the
 // largest of them in [1, 2^9], whatever the steps are; the sum of p_t is kept in f32 with the same reference.  f16 has 11
-// bits: each w_t is off by 2^-12 of itself at most, below half a unit of what bf16 or f16 outputs round to.  Queries are
-// scaled to 2^10..2^11 by a power of two (exact); elements 2^-24 of a row's largest lose bits.
+// bits: each w_t is off by 2^-11 of itself at most, half a unit of what f16 outputs round to and less than bf16's.
+// Queries are scaled to 2^14..2^15 by a power of two (exact); elements 2^-30 of a row's largest lose bits.
 static __device__ __forceinline__ float over_groups_max(float x) {     // over the 4 groups of 16 lanes
     auto p = __builtin_amdgcn_permlane32_swap((int)asu(x), (int)asu(x), false, false);
     x = fmaxf(asf((uint32_t)p[0]), asf((uint32_t)p[1]));
@@ -258,28 +262,20 @@ static __device__ __forceinline__ float over_groups_sum(float x) {
     return asf((uint32_t)q[0]) + asf((uint32_t)q[1]);
 }
 
-union Frag { h8 v; h2 p[4]; uint32_t u[4]; };
-union Two { h2 h; uint32_t u; };
-static __device__ __forceinline__ uint32_t h2_sub(uint32_t x, float c) {
-    Two t;
-    t.u = x;
-    t.h = t.h - (h2){(_Float16)c, (_Float16)c};
-    return t.u;
-}
+union Frag { h8 v; uint32_t u[4]; };
 
-// whole numbers as f16: 1024 + n and 64 + n are n's bits behind a constant exponent
-// 4 bits: nibbles 0..3 of both halves of x -> pairs o[0..3], less 8
-static __device__ __forceinline__ void pairs4(uint32_t x, uint32_t* o, int n) {
-    const uint32_t y = x >> 8;
-    o[0] = h2_sub((x & 0x000F000Fu) | 0x64006400u, 1032.0f);
-    if (n > 1) o[1] = h2_sub((x & 0x00F000F0u) | 0x54005400u, 72.0f);
-    if (n > 2) o[2] = h2_sub((y & 0x000F000Fu) | 0x64006400u, 1032.0f);
-    if (n > 3) o[3] = h2_sub((y & 0x00F000F0u) | 0x54005400u, 72.0f);
-}
-// 8 bits: bytes 0..1 of both halves, less 128
-static __device__ __forceinline__ void pairs8(uint32_t x, uint32_t* o) {
-    o[0] = h2_sub((x & 0x00FF00FFu) | 0x64006400u, 1152.0f);
-    o[1] = h2_sub(((x >> 8) & 0x00FF00FFu) | 0x64006400u, 1152.0f);
+// the codes in both halves of x times 1 / UNIT: 4 bits, four pairs of nibbles 0..3; 8 bits, two of bytes 0..1
+template <int BITS> constexpr float UNIT = BITS == 4 ? 1048576.0f : 16777216.0f;
+template <int BITS> static __device__ __forceinline__ void codes_of(uint32_t x, uint32_t* o) {
+    if constexpr (BITS == 4) {
+        o[0] = (x << 4) & 0x00F000F0u;
+        o[1] = x & 0x00F000F0u;
+        o[2] = (x >> 4) & 0x00F000F0u;
+        o[3] = (x >> 8) & 0x00F000F0u;
+    } else {
+        o[0] = x & 0x00FF00FFu;
+        o[1] = (x >> 8) & 0x00FF00FFu;
+    }
 }
 // the 16 bits at byte offset o of w[] (offsets are known when this is compiled); those at two offsets, one per half
 static __device__ __forceinline__ uint32_t at16(const uint32_t* w, int o) {
@@ -300,6 +296,7 @@ template <int BITS> static __device__ __forceinline__ constexpr int key_order(in
 template <int U> struct Stage {         // what a lane holds of 32 tokens: 2 blocks of 16
     uint32_t k[2][U], v[2][U + 1];      // (one word more: a 16-bit piece may end in it; never used)
     u4 kw[2], vw[2];
+    bool hole[2];                       // not in the cache
 };
 
 // a query row's N values from d0 on, and (with the first of them, LSE) the log of its sum
@@ -321,10 +318,104 @@ template <int N, bool LSE = true> static __device__ __forceinline__ void put(con
     }
     if (LSE && a.lse && d0 == 0) a.lse[((long long)b * a.tokens + i) * a.heads * a.group + hq] = lse;
 }
+// the log of a row's sum l with the reference m (in which an exponent counts one more)
+static __device__ __forceinline__ float log_sum(float m, float l) { return (m - 1.0f + log2f(l)) * 0.69314718055994530942f; }
+// 1 / l; NaN where a row is NaN (its sum is then negative or NaN) or nothing of what a query sees is in the cache
+static __device__ __forceinline__ float inverse_sum(float l) { return l > 0.0f ? 1.0f / l : asf(0x7FC00000u); }
+
+// One step of a wave: 32 tokens from t0 on against NT tiles of 16 queries.  EDGE: some of them may not be seen.
+template <int D, int BITS, int NT, bool EDGE>
+static __device__ __forceinline__ void attend(const Stage<D * BITS / 128>& c, const Frag (*q)[D / 32], const float* qsum,
+                                              const float* unit, const int* sees, int t0, int g, f4 (*acc)[D / 16], float* M,
+                                              float* L, float* Z) {
+    constexpr int N = D / 16, U = N * BITS / 8, KS = D / 32, PER = 16 / BITS;
+    f4 s[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) s[nt][0] = s[nt][1] = (f4){0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+#pragma unroll
+        for (int st = 0; st < KS; st++) {
+            Frag k;
+            codes_of<BITS>(c.k[j][st * BITS / 4], k.u);
+            if constexpr (BITS == 8) codes_of<BITS>(c.k[j][2 * st + 1], k.u + 2);
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) s[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k.v, q[nt][st].v, s[nt][j], 0, 0, 0);
+        }
+    // the tokens' words: keys' step and zero point; values' exponent + 1, significand, 2^-exponent, zero point.  (The
+    // exponent without its bias: what is added to a score costs it bits)
+    float ks[8], kz[8], ve[8], vm[8], vi[8], vz[8];
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int t = 4 * j + r;
+            const uint32_t kw = c.kw[j][r], vw = c.vw[j][r], step = vw << 16;
+            ks[t] = asf(kw << 16);
+            kz[t] = (float)(int16_t)(kw >> 16);
+            ve[t] = (float)__builtin_amdgcn_frexp_expf(asf(step));
+            vm[t] = asf((step & 0x007FFFFFu) | 0x3F800000u);
+            vi[t] = asf(0x7F000000u - (step & 0x7F800000u));    // (a NaN's: minus infinity, which stays in the sum)
+            vz[t] = (float)(int16_t)(vw >> 16);
+        }
+    Frag w[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        float ref[8], mx = -INFINITY;
+        int left[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            left[j] = c.hole[j] ? 0 : sees[nt] - (t0 + 16 * j + 4 * g);      // tokens of this lane that are seen
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int t = 4 * j + r;
+                ref[t] = fmaf(fmaf(kz[t], qsum[nt], s[nt][j][r]) * unit[nt], ks[t], ve[t]);
+                if (EDGE && r >= left[j]) ref[t] = -INFINITY;
+                mx = fmaxf(mx, ref[t]);
+            }
+        }
+        mx = over_groups_max(mx);
+        if (__any(mx > M[nt] + 8.0f)) {                     // (weights stay below 2^9)
+            const float m = fmaxf(M[nt], mx), al = __builtin_amdgcn_exp2f(M[nt] - m);
+            M[nt] = m;
+            L[nt] *= al;
+            Z[nt] *= al;
+#pragma unroll
+            for (int i = 0; i < N; i++) acc[nt][i] *= al;
+        }
+#pragma unroll
+        for (int t = 0; t < 8; t++) {
+            const float p = __builtin_amdgcn_exp2f(ref[t] - M[nt]);
+            const _Float16 wt = (_Float16)(p * vm[t]);
+            const float l = fmaf(p, vi[t], L[nt]);
+            L[nt] = EDGE && (t & 3) >= left[t >> 2] ? L[nt] : l;
+            Z[nt] = fmaf((float)wt, vz[t], Z[nt]);
+            w[nt].v[t] = wt;
+        }
+    }
+    // values: unit lane % 16, tokens 4 g .. 4 g + 3 of both blocks, 16 bits of each token at a time
+#pragma unroll
+    for (int i0 = 0; i0 < N; i0 += PER) {
+        uint32_t got[4][PER];
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int r = 0; r < 2; r++)
+                codes_of<BITS>(pair16(c.v[j], 2 * r * U + i0 * BITS / 8, (2 * r + 1) * U + i0 * BITS / 8), got[2 * j + r]);
+#pragma unroll
+        for (int i = 0; i < PER && i0 + i < N; i++) {
+            Frag f;
+#pragma unroll
+            for (int k = 0; k < 4; k++) f.u[k] = got[k][i];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+                acc[nt][i0 + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.v, w[nt].v, acc[nt][i0 + i], 0, 0, 0);
+        }
+    }
+}
 
 template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_attention(KvArgs a) {
     constexpr int N = D / 16, U = N * BITS / 8, ROW = 16 * U, KS = D / 32, COLS = 16 * NT;
-    constexpr float BIAS = (float)(1 << (BITS - 1));
     constexpr bool ALL = D * NT <= 256;                     // every wave its own sums in LDS, or one after the other
     __shared__ float acc_lds[(ALL ? 4 : 1) * N * 16 * COLS];
     __shared__ float ml[3][4][COLS];
@@ -352,17 +443,18 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_att
         }
     }
     if (row0 >= rows) return;
-    // what each query row of the tile sees: positions < sees
-    int sees[NT], most = 0;
+    // what the tile's queries see: positions below sees, from least (all of them) to most (the last one)
+    const int last_row = min(row0 + COLS, rows) - 1;
+    int least = context, most = context;
+    if (a.causal) {
+        least = max(context - len + 1 + (int)div_by((uint32_t)row0, a.group_inv), 0);
+        most = max(context - len + 1 + (int)div_by((uint32_t)last_row, a.group_inv), 0);
+    }
+    int sees[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-        const int rw = row0 + nt * 16 + col;
-        const int i = (int)div_by((uint32_t)rw, a.group_inv);
-        sees[nt] = rw < rows ? (a.causal ? max(context - len + 1 + i, 0) : context) : 0;
-    }
-    {
-        const int last = (int)div_by((uint32_t)(min(row0 + COLS, rows) - 1), a.group_inv);
-        most = a.causal ? max(context - len + 1 + last, 0) : context;
+        const int i = (int)div_by((uint32_t)min(row0 + nt * 16 + col, last_row), a.group_inv);
+        sees[nt] = a.causal ? max(context - len + 1 + i, 0) : context;
     }
     const int chunk = ((context + (int)a.splits - 1) / (int)a.splits + 127) & ~127;
     const long long lo64 = (long long)split * chunk;
@@ -373,11 +465,10 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_att
     float qsum[NT], unit[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-        const int rw = row0 + nt * 16 + col;
-        const bool on = rw < rows;
-        const int i = (int)div_by((uint32_t)(on ? rw : 0), a.group_inv), gi = (on ? rw : 0) - i * a.group;
+        const int rw = min(row0 + nt * 16 + col, last_row);     // (rows behind the last one repeat it; they are not put out)
+        const int i = (int)div_by((uint32_t)rw, a.group_inv), gi = rw - i * a.group;
         const long long at = b * a.ks[0] + (long long)i * a.ks[1] + (long long)(h * a.group + gi) * a.ks[2] + g * (D / 4);
-        float f[D / 4], big = 0.0f;
+        float f[D / 4];
         uint32_t top = 0;
         if (a.dtype == DC_BF16) {
             const uint16_t* p = (const uint16_t*)a.k + at;
@@ -385,19 +476,19 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_att
             if (a.vec) load_n<uint16_t, D / 4, 16>(p, raw);
             else load_n<uint16_t, D / 4, 2>(p, raw);
 #pragma unroll
-            for (int j = 0; j < D / 4; j++) f[j] = on ? BF16::to(raw[j]) : 0.0f;
+            for (int j = 0; j < D / 4; j++) f[j] = BF16::to(raw[j]);
         } else {
             const _Float16* p = (const _Float16*)a.k + at;
             alignas(16) _Float16 raw[D / 4];
             if (a.vec) load_n<_Float16, D / 4, 16>(p, raw);
             else load_n<_Float16, D / 4, 2>(p, raw);
 #pragma unroll
-            for (int j = 0; j < D / 4; j++) f[j] = on ? (float)raw[j] : 0.0f;
+            for (int j = 0; j < D / 4; j++) f[j] = (float)raw[j];
         }
 #pragma unroll
         for (int j = 0; j < D / 4; j++) top = max(top, asu(f[j]) & 0x7FFFFFFFu);
-        big = over_groups_max(asf(min(top, 0x7F7FFFFFu)));
-        const int e = min(264 - (int)(asu(big) >> 23), 253);            // 2^(10 - exponent of the largest)
+        const float big = over_groups_max(asf(min(top, 0x7F7FFFFFu)));
+        const int e = min(268 - (int)(asu(big) >> 23), 253);            // 2^(14 - exponent of the largest)
         const float up = asf((uint32_t)e << 23), down = asf((uint32_t)(254 - e) << 23);
         float sum = 0.0f;
 #pragma unroll
@@ -408,8 +499,8 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_att
                 q[nt][j].v[k] = v;
                 sum += (float)v;
             }
-        qsum[nt] = over_groups_sum(sum);
-        unit[nt] = a.scale * 1.44269504088896340736f * down;
+        qsum[nt] = over_groups_sum(sum) * (1.0f / UNIT<BITS>);
+        unit[nt] = a.scale * 1.44269504088896340736f * down * UNIT<BITS>;
     }
 
     f4 acc[NT][N];
@@ -418,144 +509,64 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_att
     for (int nt = 0; nt < NT; nt++) {
         M[nt] = -1e30f;
         L[nt] = Z[nt] = 0.0f;
+#pragma unroll
         for (int i = 0; i < N; i++) acc[nt][i] = (f4){0, 0, 0, 0};
     }
 
+    // the wave's tokens: 32 of each 128.  Their pages are followed from step to step: a table entry and a block of 16
+    // within its page, for the first block and for the one behind it
     const int* table = a.table ? a.table + (long long)b * a.table_stride : nullptr;
-    const uint32_t blocks = (uint32_t)a.page >> 4;
-    // the page and place of the block of 16 tokens from t on (t < hi); -1: not in the cache
-    auto page_of = [&](int t, uint32_t& in) -> long long {
-        const uint32_t blk = (uint32_t)t >> 4, slot = div_by(blk, a.blocks_inv);
-        in = blk - slot * blocks;
-        const long long p = table ? (long long)table[slot] : (long long)b;
-        return p >= 0 && p < a.pages ? p : -1;
+    const uint32_t blocks = (uint32_t)a.page >> 4, slot_step = div_by(8u, a.blocks_inv), in_step = 8u - slot_step * blocks;
+    const int first = lo + wave * 32;
+    uint32_t slot = div_by((uint32_t)first >> 4, a.blocks_inv), in = ((uint32_t)first >> 4) - slot * blocks;
+    const uint32_t lane_codes = (uint32_t)(col * ROW + g * (4 * U)), lane_words = (uint32_t)g * 16;
+    int page[2];                                            // -1: not in the cache
+    uint32_t place_in[2];
+    auto find = [&](int t) {                                // (the second block may lie past the end: then the first again)
+        const uint32_t s1 = in + 1 == blocks ? slot + 1 : slot;
+        const bool two = t + 16 < hi;
+        place_in[0] = in;
+        place_in[1] = !two ? in : in + 1 == blocks ? 0 : in + 1;
+        const int p0 = table ? table[slot] : (int)b, p1 = table ? table[two ? s1 : slot] : (int)b;
+        page[0] = p0 >= 0 && p0 < a.pages ? p0 : -1;
+        page[1] = p1 >= 0 && p1 < a.pages ? p1 : -1;
+        in += in_step;
+        slot += slot_step;
+        if (in >= blocks) { in -= blocks; slot++; }
     };
-    auto fetch = [&](Stage<U>& s, const long long* page, const uint32_t* in) {
+    auto fetch = [&](Stage<U>& s) {
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            const uint8_t* base = a.data + ((page[j] < 0 ? 0 : page[j]) * a.heads + h) * a.head_bytes;
-            const uint8_t* codes = base + (long long)in[j] * (16 * ROW) + col * ROW + g * (4 * U);
-            load_n<uint32_t, U, 4 * (U & -U)>((const uint32_t*)codes, s.k[j]);
-            load_n<uint32_t, U, 4 * (U & -U)>((const uint32_t*)(codes + (long long)a.page * ROW), s.v[j]);
-            const uint8_t* words = base + 2ll * a.page * ROW + in[j] * 64 + g * 16;
-            s.kw[j] = *(const u4*)words;
-            s.vw[j] = *(const u4*)(words + 4ll * a.page);
+            const int pg = __builtin_amdgcn_readfirstlane(page[j]);
+            const uint32_t pl = __builtin_amdgcn_readfirstlane(place_in[j]);
+            s.hole[j] = pg < 0;
+            const uint8_t* base = a.data + ((long long)max(pg, 0) * a.heads + h) * a.head_bytes;
+            const uint8_t* codes = base + (unsigned long long)pl * (16 * ROW);
+            const uint8_t* words = base + 2ll * a.page * ROW + (unsigned long long)pl * 64;
+            load_n<uint32_t, U, 4 * (U & -U)>((const uint32_t*)(codes + lane_codes), s.k[j]);
+            s.kw[j] = *(const u4*)(words + lane_words);
+            load_n<uint32_t, U, 4 * (U & -U)>((const uint32_t*)(codes + (unsigned long long)a.page * ROW + lane_codes), s.v[j]);
+            s.vw[j] = *(const u4*)(words + 4ll * a.page + lane_words);
         }
     };
     Stage<U> cur, nxt;
-    long long pg[2];
-    uint32_t in[2];
-    bool hole[2], hole_nxt[2];
-    const int first = lo + wave * 32;
-    auto find = [&](int t) {                                // the second block may lie past the end: then the first again
-        pg[0] = page_of(t, in[0]);
-        if (t + 16 < hi) pg[1] = page_of(t + 16, in[1]);
-        else { pg[1] = pg[0]; in[1] = in[0]; }
-    };
     if (first < hi) {
         find(first);
-        hole[0] = pg[0] < 0; hole[1] = pg[1] < 0;
-        fetch(cur, pg, in);
+        fetch(cur);
         if (first + 128 < hi) find(first + 128);
     }
     for (int t0 = first; t0 < hi; t0 += 128) {
         if (t0 + 128 < hi) {
-            hole_nxt[0] = pg[0] < 0; hole_nxt[1] = pg[1] < 0;
-            fetch(nxt, pg, in);
+            fetch(nxt);
             if (t0 + 256 < hi) find(t0 + 256);
         }
-        if ((hole[0] || hole[1]) && lane == 0) atomicOr(a.status, 1u);
-        // scores
-        f4 s[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) s[nt][0] = s[nt][1] = (f4){0, 0, 0, 0};
-#pragma unroll
-        for (int j = 0; j < 2; j++)
-#pragma unroll
-            for (int st = 0; st < KS; st++) {
-                Frag k;
-                if constexpr (BITS == 4) pairs4(cur.k[j][st], k.u, 4);
-                else {
-                    pairs8(cur.k[j][2 * st], k.u);
-                    pairs8(cur.k[j][2 * st + 1], k.u + 2);
-                }
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-                    s[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k.v, q[nt][st].v, s[nt][j], 0, 0, 0);
-            }
-        // the tokens' words
-        float ks[8], kz[8], ve[8], vm[8], vi[8], vz[8];
-#pragma unroll
-        for (int j = 0; j < 2; j++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int t = 4 * j + r;
-                const uint32_t kw = cur.kw[j][r], vw = cur.vw[j][r], e = (vw >> 7) & 0xFFu;
-                ks[t] = asf(kw << 16);
-                kz[t] = (float)((int)kw >> 16) + BIAS;
-                ve[t] = e == 255u ? asf(0x7FC00000u) : (float)((int)e - 127);
-                vm[t] = asf(((vw & 0x7Fu) << 16) | 0x3F800000u);
-                vi[t] = asf((254u - min(e, 254u)) << 23);
-                vz[t] = (float)((int)vw >> 16) + BIAS;
-            }
-        Frag w[NT];
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            float ref[8], mx = -INFINITY;
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const int left = hole[j] ? -1 : sees[nt] - (t0 + 16 * j + 4 * g);    // tokens of this lane that are seen
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int t = 4 * j + r;
-                    const float y = fmaf(fmaf(kz[t], qsum[nt], s[nt][j][r]) * unit[nt], ks[t], ve[t]);
-                    ref[t] = r < left ? y : -INFINITY;
-                    mx = fmaxf(mx, ref[t]);
-                }
-            }
-            mx = over_groups_max(mx);
-            if (__any(mx > M[nt] + 8.0f)) {                 // (weights stay below 2^9)
-                const float m = fmaxf(M[nt], mx), al = __builtin_amdgcn_exp2f(M[nt] - m);
-                M[nt] = m;
-                L[nt] *= al;
-                Z[nt] *= al;
-                for (int i = 0; i < N; i++) acc[nt][i] *= al;
-            }
-#pragma unroll
-            for (int t = 0; t < 8; t++) {
-                const float p = __builtin_amdgcn_exp2f(ref[t] - M[nt]);
-                const _Float16 wt = (_Float16)(p * vm[t]);
-                L[nt] = fmaf(p, vi[t], L[nt]);
-                Z[nt] = fmaf((float)wt, vz[t], Z[nt]);
-                w[nt].v[t] = wt;
-            }
-        }
-        // values: unit col, tokens 4 g .. 4 g + 3 of both blocks
-#pragma unroll
-        for (int i0 = 0; i0 < N; i0 += 16 / BITS) {         // 16 bits of each token at a time
-            constexpr int PER = 16 / BITS;
-            const int n = N - i0 < PER ? N - i0 : PER, o = i0 * BITS / 8;
-            uint32_t got[4][PER];
-#pragma unroll
-            for (int j = 0; j < 2; j++)
-#pragma unroll
-                for (int r = 0; r < 2; r++) {
-                    const uint32_t y = pair16(cur.v[j], 2 * r * U + o, (2 * r + 1) * U + o);
-                    if constexpr (BITS == 4) pairs4(y, got[2 * j + r], n);
-                    else pairs8(y, got[2 * j + r]);
-                }
-#pragma unroll
-            for (int i = 0; i < PER; i++) {
-                if (i >= n) break;
-                Frag f;
-                for (int k = 0; k < 4; k++) f.u[k] = got[k][i];
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-                    acc[nt][i0 + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.v, w[nt].v, acc[nt][i0 + i], 0, 0, 0);
-            }
+        if (t0 + 32 <= least && t0 + 32 <= hi && !cur.hole[0] && !cur.hole[1])
+            attend<D, BITS, NT, false>(cur, q, qsum, unit, sees, t0, g, acc, M, L, Z);
+        else {
+            if ((cur.hole[0] || cur.hole[1]) && lane == 0) atomicOr(a.status, 1u);
+            attend<D, BITS, NT, true>(cur, q, qsum, unit, sees, t0, g, acc, M, L, Z);
         }
         cur = nxt;
-        hole[0] = hole_nxt[0]; hole[1] = hole_nxt[1];
     }
 
     // the four waves' sums, in a fixed order
@@ -575,7 +586,7 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_att
     for (int nt = 0; nt < NT; nt++) {
         float m = ml[0][0][nt * 16 + col];
         for (int v = 1; v < 4; v++) m = fmaxf(m, ml[0][v][nt * 16 + col]);
-        f[nt] = __builtin_amdgcn_exp2f(M[nt] - m);
+        f[nt] = __builtin_amdgcn_exp2f(M[nt] - m) * UNIT<BITS>;
     }
     for (int v = 0; v < (ALL ? 1 : 4); v++) {
         if (ALL || wave == v)
@@ -621,10 +632,10 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_att
             continue;
         }
         const bool none = (a.causal ? context - len + 1 + (int)div_by((uint32_t)rw, a.group_inv) : context) <= 0;
-        const float inv = 1.0f / l;
+        const float inv = inverse_sum(l);
 #pragma unroll
         for (int k = 0; k < N; k++) o[k] = none ? 0.0f : o[k] * inv;
-        put<N>(a, b, h, rw, ou * N, o, none ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f);
+        put<N>(a, b, h, rw, ou * N, o, none ? -INFINITY : log_sum(m, l));
     }
 }
 
@@ -669,11 +680,11 @@ template <int D> __global__ __launch_bounds__(256) void kv_join(KvArgs a) {
     int context = a.start[b];
     context = context < 0 ? 0 : context > a.capacity ? (int)a.capacity : context;
     const bool none = (a.causal ? context - len + 1 + (int)div_by(rw, a.group_inv) : context) <= 0;
-    const float lse = none ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
+    const float lse = none ? -INFINITY : log_sum(m, l), inv = inverse_sum(l);
     for (int d = threadIdx.x; d < D; d += 256) {
         float y = 0.0f;
         for (int k = 0; k < 16; k++) y = fmaf(sums[k][d], f[k], y);
-        y = none ? 0.0f : y / l;
+        y = none ? 0.0f : y * inv;
         put<1>(a, b, h, (int)rw, d, &y, lse);
     }
 }

@@ -252,16 +252,18 @@ class Filled:
         self.cache.write(k.to(DEV), v.to(DEV), torch.zeros(B, dtype=torch.int32, device=DEV), table=self.table)
         self.k, self.ks, self.kz, self.kc = held(k, bits)
         self.v, self.vs, self.vz, self.vc = held(v, bits)
-        self.bias = 1 << (bits - 1)
 
 
 def formula(f, q, context, lens, scale, causal):
     """(output, log of the sum, how far the kernel's output may be off) in doubles.
 
-    With u = 2^-24: a score is a sum of D products of whole numbers with queries (at most D + 8 roundings, each u of the
-    sum of magnitudes A = ks (sum |q| |code'| + |kz'| sum |q|)), so a weight is off by (D + 8) u scale A of itself, and by
+    With u = 2^-24: a score is a sum of D products of codes with queries (at most D + 8 roundings, each u of the
+    sum of magnitudes A = ks (sum |q| code + |kz| sum |q|)), so a weight is off by (D + 8) u scale A of itself, and by
     2^-11 (to f16) + 8 u (its factors); weights below f16's range by 2^-25 of the largest, which is 1 or more.  The sum
-    over positions adds N u of magnitudes; the output's type half a unit."""
+    over positions adds N u of magnitudes; the output's type half a unit.  A matrix instruction cuts each of its 33 terms
+    at 24 bits below the largest one's exponent, in which a code counts as 2^-14: at 2^-18 (codes are n 2^-20: 4 bits) or
+    2^-14 (n 2^-24: 8 bits) of a code times the largest query element or weight; D / 32 of them make a score, a 32nd of N
+    and one for each wave and each split of the work the sums."""
     B, T, HQ, D = q.shape
     H, N = f.k.shape[2], f.k.shape[1]
     G = HQ // H
@@ -278,16 +280,19 @@ def formula(f, q, context, lens, scale, causal):
                 qq = q[b, i, h * G:(h + 1) * G].double()                                # (G, D)
                 k, v = f.k[b, :n, h], f.v[b, :n, h]                                     # (n, D)
                 s = qq @ k.t() * scale
-                A = (qq.abs() @ (f.kc[b, :n, h] - f.bias).abs().t() + qq.abs().sum(-1, keepdim=True) *
-                     (f.kz[b, :n, h] + f.bias).abs().t()) * f.ks[b, :n, h].t() * abs(scale)
+                A = (qq.abs() @ f.kc[b, :n, h].t() + qq.abs().sum(-1, keepdim=True) * f.kz[b, :n, h].abs().t()) * \
+                    f.ks[b, :n, h].t() * abs(scale)
                 p = torch.softmax(s, -1)
                 o = p @ v
-                mag = f.vs[b, :n, h] * ((f.vc[b, :n, h] - f.bias).abs() + (f.vz[b, :n, h] + f.bias).abs())
+                cut = 33 * (2.0 ** -18 if f.kc.max() < 16 else 2.0 ** -14)
+                A = A + cut / u / (D + 8) * (D / 32) * qq.abs().amax(-1, keepdim=True) * f.ks[b, :n, h].t() * abs(scale)
+                mag = f.vs[b, :n, h] * (f.vc[b, :n, h] + f.vz[b, :n, h].abs())
                 eps = torch.expm1((D + 8) * u * A) + 8 * u
                 w = p * f.vs[b, :n, h].t()
                 largest = w.amax(-1, keepdim=True)
                 err = (p * (eps + 2.0 ** -11)) @ v.abs() + (p * eps).sum(-1, keepdim=True) * o.abs()
                 err = err + ((n + 8) * u * w + 2.0 ** -25 * largest) @ (mag / f.vs[b, :n, h])
+                err = err + cut * (n / 32 + 4 * (1 + n / 256)) * largest
                 out[b, i, h * G:(h + 1) * G] = o
                 lse[b, i, h * G:(h + 1) * G, 0] = torch.logsumexp(s, -1)
                 tol[b, i, h * G:(h + 1) * G] = err * 1.01 + half * (o.abs() + err) + 2.0 ** -25
@@ -384,7 +389,7 @@ def test_attention_rows_of_zeros(kv):
     c.write(k.to(DEV), v.to(DEV), i32(0))
     q = k[:, :1].half()
     f = Filled.__new__(Filled)
-    f.cache, f.table, f.bias = c, torch.zeros(1, 1, dtype=torch.int32, device=DEV), 8
+    f.cache, f.table = c, torch.zeros(1, 1, dtype=torch.int32, device=DEV)
     f.k, f.ks, f.kz, f.kc = held(k, 4)
     f.v, f.vs, f.vz, f.vc = held(v, 4)
     check(f, q, [N])
@@ -444,7 +449,6 @@ def test_attention_outside_the_cache(kv):
     assert kv.KVCache.status(reset=True) == 1
     keep = list(range(32)) + list(range(64, 96))
     g = Filled.__new__(Filled)
-    g.bias = f.bias
     for n in ("k", "ks", "kz", "kc", "v", "vs", "vz", "vc"):
         setattr(g, n, getattr(f, n)[:, keep])
     want, _, tol = formula(g, q, [64], [1], 0.125, True)
@@ -468,7 +472,7 @@ def test_decode_loop(kv):
     whole.write(k.to(DEV), v.to(DEV), i32(0, 0), table=table)
     c.write(k[:, :first].to(DEV), v[:, :first].to(DEV), i32(0, 0), table=table)
     f = Filled.__new__(Filled)
-    f.cache, f.table, f.bias = c, table, 8
+    f.cache, f.table = c, table
     f.k, f.ks, f.kz, f.kc = held(k, bits)
     f.v, f.vs, f.vz, f.vc = held(v, bits)
     for t in range(first, first + n):
@@ -540,7 +544,7 @@ def test_far_pages(kv):
     zero = torch.zeros(1, 900, H, D, device=DEV)
     c.write(zero, zero, i32(0), table=table)
     f = Filled.__new__(Filled)
-    f.cache, f.table, f.bias = c, table, 128
+    f.cache, f.table = c, table
     z = torch.zeros(1, 900, H, D)
     f.k, f.ks, f.kz, f.kc = held(torch.cat((z, k.float()), 1), bits)
     f.v, f.vs, f.vz, f.vc = held(torch.cat((z, v.float()), 1), bits)
