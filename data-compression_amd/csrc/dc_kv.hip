@@ -262,6 +262,9 @@ static __device__ __forceinline__ float over_groups_sum(float x) {
     return asf((uint32_t)q[0]) + asf((uint32_t)q[1]);
 }
 
+// lengths and tables: the kernel writes none, so they are read by scalar loads
+typedef __attribute__((address_space(4))) int Const;
+
 union Frag { h8 v; uint32_t u[4]; };
 
 // the codes in both halves of x times 1 / UNIT: 4 bits, four pairs of nibbles 0..3; 8 bits, two of bytes 0..1
@@ -296,7 +299,12 @@ template <int BITS> static __device__ __forceinline__ constexpr int key_order(in
 template <int U> struct Stage {         // what a lane holds of 32 tokens: 2 blocks of 16
     uint32_t k[2][U], v[2][U + 1];      // (one word more: a 16-bit piece may end in it; never used)
     u4 kw[2], vw[2];
-    bool hole[2];                       // not in the cache
+};
+// where a step's two blocks lie: the first byte of their keys' codes and of their words (uniform over a wave), and
+// whether they are not in the cache
+struct Where {
+    const uint8_t *codes[2], *words[2];
+    bool hole[2];
 };
 
 // a query row's N values from d0 on, and (with the first of them, LSE) the log of its sum
@@ -323,76 +331,99 @@ static __device__ __forceinline__ float log_sum(float m, float l) { return (m - 
 // 1 / l; NaN where a row is NaN (its sum is then negative or NaN) or nothing of what a query sees is in the cache
 static __device__ __forceinline__ float inverse_sum(float l) { return l > 0.0f ? 1.0f / l : asf(0x7FC00000u); }
 
-// One step of a wave: 32 tokens from t0 on against NT tiles of 16 queries.  EDGE: some of them may not be seen.
+template <int U> static __device__ __forceinline__ void load_keys(Stage<U>& c, const Where& at, uint32_t lane_codes) {
+#pragma unroll
+    for (int j = 0; j < 2; j++) load_n<uint32_t, U, 4 * (U & -U)>((const uint32_t*)(at.codes[j] + lane_codes), c.k[j]);
+}
+template <int U> static __device__ __forceinline__ void load_values(Stage<U>& c, const Where& at, uint64_t to_values, uint32_t lane_codes) {
+#pragma unroll
+    for (int j = 0; j < 2; j++) load_n<uint32_t, U, 4 * (U & -U)>((const uint32_t*)(at.codes[j] + to_values + lane_codes), c.v[j]);
+}
+template <int U> static __device__ __forceinline__ void load_words(Stage<U>& c, const Where& at, uint32_t to_values, uint32_t lane_words) {
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        c.kw[j] = *(const u4*)(at.words[j] + lane_words);
+        c.vw[j] = *(const u4*)(at.words[j] + to_values + lane_words);
+    }
+}
+
+// One step of a wave: 32 tokens from t0 on against NT tiles of 16 queries.  EDGE: some of them may not be seen.  What the
+// registers of `c` held is replaced by the next step's as soon as it is used, so that those loads are under way during the
+// rest of this step and the beginning of the next.
 template <int D, int BITS, int NT, bool EDGE>
-static __device__ __forceinline__ void attend(const Stage<D * BITS / 128>& c, const Frag (*q)[D / 32], const float* qsum,
-                                              const float* unit, const int* sees, int t0, int g, f4 (*acc)[D / 16], float* M,
+static __device__ __forceinline__ void attend(Stage<D * BITS / 128>& c, const Frag (*q)[D / 32], const float* qsum,
+                                              const float* unit, const int* sees, int t0, int g, const bool* hole,
+                                              const Where& next, uint64_t codes_to_values, uint32_t words_to_values,
+                                              uint32_t lane_codes, uint32_t lane_words, f4 (*acc)[D / 16], float* M,
                                               float* L, float* Z) {
     constexpr int N = D / 16, U = N * BITS / 8, KS = D / 32, PER = 16 / BITS;
     f4 s[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) s[nt][0] = s[nt][1] = (f4){0, 0, 0, 0};
 #pragma unroll
-    for (int j = 0; j < 2; j++)
+    for (int st = 0; st < KS; st++)
 #pragma unroll
-        for (int st = 0; st < KS; st++) {
+        for (int j = 0; j < 2; j++) {
             Frag k;
             codes_of<BITS>(c.k[j][st * BITS / 4], k.u);
             if constexpr (BITS == 8) codes_of<BITS>(c.k[j][2 * st + 1], k.u + 2);
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) s[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k.v, q[nt][st].v, s[nt][j], 0, 0, 0);
         }
-    // the tokens' words: keys' step and zero point; values' exponent + 1, significand, 2^-exponent, zero point.  (The
+    load_keys(c, next, lane_codes);
+    // a token's words: keys' step and zero point; values' exponent + 1, significand, 2^-exponent, zero point.  (The
     // exponent without its bias: what is added to a score costs it bits)
-    float ks[8], kz[8], ve[8], vm[8], vi[8], vz[8];
+    float ref[NT][8], mx[NT];
+    int left[NT][2];
 #pragma unroll
-    for (int j = 0; j < 2; j++)
+    for (int nt = 0; nt < NT; nt++) mx[nt] = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) left[nt][j] = hole[j] ? 0 : sees[nt] - (t0 + 16 * j + 4 * g);   // tokens of this lane that are seen
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-            const int t = 4 * j + r;
-            const uint32_t kw = c.kw[j][r], vw = c.vw[j][r], step = vw << 16;
-            ks[t] = asf(kw << 16);
-            kz[t] = (float)(int16_t)(kw >> 16);
-            ve[t] = (float)__builtin_amdgcn_frexp_expf(asf(step));
-            vm[t] = asf((step & 0x007FFFFFu) | 0x3F800000u);
-            vi[t] = asf(0x7F000000u - (step & 0x7F800000u));    // (a NaN's: minus infinity, which stays in the sum)
-            vz[t] = (float)(int16_t)(vw >> 16);
-        }
-    Frag w[NT];
+            const uint32_t kw = c.kw[j][r], vw = c.vw[j][r];
+            const float ks = asf(kw << 16), kz = (float)(int16_t)(kw >> 16);
+            const float ve = (float)__builtin_amdgcn_frexp_expf(asf(vw << 16));
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        float ref[8], mx = -INFINITY;
-        int left[2];
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-            left[j] = c.hole[j] ? 0 : sees[nt] - (t0 + 16 * j + 4 * g);      // tokens of this lane that are seen
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int t = 4 * j + r;
-                ref[t] = fmaf(fmaf(kz[t], qsum[nt], s[nt][j][r]) * unit[nt], ks[t], ve[t]);
-                if (EDGE && r >= left[j]) ref[t] = -INFINITY;
-                mx = fmaxf(mx, ref[t]);
+            for (int nt = 0; nt < NT; nt++) {
+                float y = fmaf(fmaf(kz, qsum[nt], s[nt][j][r]) * unit[nt], ks, ve);
+                if (EDGE && r >= left[nt][j]) y = -INFINITY;
+                ref[nt][4 * j + r] = y;
+                mx[nt] = fmaxf(mx[nt], y);
             }
         }
-        mx = over_groups_max(mx);
-        if (__any(mx > M[nt] + 8.0f)) {                     // (weights stay below 2^9)
-            const float m = fmaxf(M[nt], mx), al = __builtin_amdgcn_exp2f(M[nt] - m);
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        const float top = over_groups_max(mx[nt]);
+        if (__any(top > M[nt] + 8.0f)) {                    // (weights stay below 2^9)
+            const float m = fmaxf(M[nt], top), al = __builtin_amdgcn_exp2f(M[nt] - m);
             M[nt] = m;
             L[nt] *= al;
             Z[nt] *= al;
 #pragma unroll
             for (int i = 0; i < N; i++) acc[nt][i] *= al;
         }
+    }
+    Frag w[NT];
 #pragma unroll
-        for (int t = 0; t < 8; t++) {
-            const float p = __builtin_amdgcn_exp2f(ref[t] - M[nt]);
-            const _Float16 wt = (_Float16)(p * vm[t]);
-            const float l = fmaf(p, vi[t], L[nt]);
-            L[nt] = EDGE && (t & 3) >= left[t >> 2] ? L[nt] : l;
-            Z[nt] = fmaf((float)wt, vz[t], Z[nt]);
+    for (int t = 0; t < 8; t++) {
+        const uint32_t vw = c.vw[t >> 2][t & 3], step = vw << 16;
+        const float vm = asf((step & 0x007FFFFFu) | 0x3F800000u), vz = (float)(int16_t)(vw >> 16);
+        const float vi = asf(0x7F000000u - (step & 0x7F800000u));       // (a NaN's: minus infinity, which stays in the sum)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const float p = __builtin_amdgcn_exp2f(ref[nt][t] - M[nt]);
+            const _Float16 wt = (_Float16)(p * vm);
+            const float l = fmaf(p, vi, L[nt]);
+            L[nt] = EDGE && (t & 3) >= left[nt][t >> 2] ? L[nt] : l;
+            Z[nt] = fmaf((float)wt, vz, Z[nt]);
             w[nt].v[t] = wt;
         }
     }
+    load_words(c, next, words_to_values, lane_words);
     // values: unit lane % 16, tokens 4 g .. 4 g + 3 of both blocks, 16 bits of each token at a time
 #pragma unroll
     for (int i0 = 0; i0 < N; i0 += PER) {
@@ -412,6 +443,7 @@ static __device__ __forceinline__ void attend(const Stage<D * BITS / 128>& c, co
                 acc[nt][i0 + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.v, w[nt].v, acc[nt][i0 + i], 0, 0, 0);
         }
     }
+    load_values(c, next, codes_to_values, lane_codes);
 }
 
 template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_attention(KvArgs a) {
@@ -426,12 +458,12 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_att
     const uint32_t split = x % a.splits; x /= a.splits;
     const uint32_t tile = x % a.tiles; x /= a.tiles;
     const uint32_t h = x % a.heads, b = x / a.heads;
-    int context = a.start[b];
+    int context = ((const Const*)a.start)[b];
     if (context < 0 || context > a.capacity) {
         if (threadIdx.x == 0) atomicOr(a.status, 1u);
         context = context < 0 ? 0 : (int)a.capacity;
     }
-    const int len = a.lens ? min(max(a.lens[b], 0), a.tokens) : a.tokens;
+    const int len = a.lens ? min(max(((const Const*)a.lens)[b], 0), a.tokens) : a.tokens;
     const int rows = len * a.group;
     const int row0 = tile * COLS;
     const int oc = threadIdx.x & 15, ou = threadIdx.x >> 4;     // a thread's output: a row, a unit
@@ -515,58 +547,69 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_att
 
     // the wave's tokens: 32 of each 128.  Their pages are followed from step to step: a table entry and a block of 16
     // within its page, for the first block and for the one behind it
-    const int* table = a.table ? a.table + (long long)b * a.table_stride : nullptr;
+    const Const* table = a.table ? (const Const*)a.table + (long long)b * a.table_stride : nullptr;
     const uint32_t blocks = (uint32_t)a.page >> 4, slot_step = div_by(8u, a.blocks_inv), in_step = 8u - slot_step * blocks;
     const int first = lo + wave * 32;
     uint32_t slot = div_by((uint32_t)first >> 4, a.blocks_inv), in = ((uint32_t)first >> 4) - slot * blocks;
     const uint32_t lane_codes = (uint32_t)(col * ROW + g * (4 * U)), lane_words = (uint32_t)g * 16;
-    int page[2];                                            // -1: not in the cache
-    uint32_t place_in[2];
+    const uint64_t codes_to_values = (uint64_t)a.page * ROW;
+    const uint32_t words_to_values = 4u * (uint32_t)a.page;
+    int page[2];
+    uint32_t place[2];
     auto find = [&](int t) {                                // (the second block may lie past the end: then the first again)
         const uint32_t s1 = in + 1 == blocks ? slot + 1 : slot;
         const bool two = t + 16 < hi;
-        place_in[0] = in;
-        place_in[1] = !two ? in : in + 1 == blocks ? 0 : in + 1;
-        const int p0 = table ? table[slot] : (int)b, p1 = table ? table[two ? s1 : slot] : (int)b;
-        page[0] = p0 >= 0 && p0 < a.pages ? p0 : -1;
-        page[1] = p1 >= 0 && p1 < a.pages ? p1 : -1;
+        place[0] = in;
+        place[1] = !two ? in : in + 1 == blocks ? 0 : in + 1;
+        page[0] = table ? table[slot] : (int)b;
+        page[1] = table ? table[two ? s1 : slot] : (int)b;
         in += in_step;
         slot += slot_step;
         if (in >= blocks) { in -= blocks; slot++; }
     };
-    auto fetch = [&](Stage<U>& s) {
+    auto where = [&](Where& w) {
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            const int pg = __builtin_amdgcn_readfirstlane(page[j]);
-            const uint32_t pl = __builtin_amdgcn_readfirstlane(place_in[j]);
-            s.hole[j] = pg < 0;
-            const uint8_t* base = a.data + ((long long)max(pg, 0) * a.heads + h) * a.head_bytes;
-            const uint8_t* codes = base + (unsigned long long)pl * (16 * ROW);
-            const uint8_t* words = base + 2ll * a.page * ROW + (unsigned long long)pl * 64;
-            load_n<uint32_t, U, 4 * (U & -U)>((const uint32_t*)(codes + lane_codes), s.k[j]);
-            s.kw[j] = *(const u4*)(words + lane_words);
-            load_n<uint32_t, U, 4 * (U & -U)>((const uint32_t*)(codes + (unsigned long long)a.page * ROW + lane_codes), s.v[j]);
-            s.vw[j] = *(const u4*)(words + 4ll * a.page + lane_words);
+            w.hole[j] = page[j] < 0 || page[j] >= a.pages;
+            const uint8_t* base = a.data + ((long long)(w.hole[j] ? 0 : page[j]) * a.heads + h) * a.head_bytes;
+            w.codes[j] = base + (uint64_t)place[j] * (16 * ROW);
+            w.words[j] = base + 2 * codes_to_values + (uint64_t)place[j] * 64;
         }
     };
-    Stage<U> cur, nxt;
+    Stage<U> c;
+    Where now, next;
     if (first < hi) {
         find(first);
-        fetch(cur);
+        where(now);
+        load_keys(c, now, lane_codes);
+        load_words(c, now, words_to_values, lane_words);
+        load_values(c, now, codes_to_values, lane_codes);
         if (first + 128 < hi) find(first + 128);
     }
-    for (int t0 = first; t0 < hi; t0 += 128) {
+    int t0 = first;
+    auto advance = [&] {                                    // (behind the last step its own tokens are loaded once more)
         if (t0 + 128 < hi) {
-            fetch(nxt);
+            where(next);
             if (t0 + 256 < hi) find(t0 + 256);
         }
-        if (t0 + 32 <= least && t0 + 32 <= hi && !cur.hole[0] && !cur.hole[1])
-            attend<D, BITS, NT, false>(cur, q, qsum, unit, sees, t0, g, acc, M, L, Z);
-        else {
-            if ((cur.hole[0] || cur.hole[1]) && lane == 0) atomicOr(a.status, 1u);
-            attend<D, BITS, NT, true>(cur, q, qsum, unit, sees, t0, g, acc, M, L, Z);
-        }
-        cur = nxt;
+    };
+    // steps whose tokens are all seen, then the others
+    while (t0 < hi && t0 + 32 <= least && t0 + 32 <= hi && !now.hole[0] && !now.hole[1]) {
+        next = now;
+        advance();
+        attend<D, BITS, NT, false>(c, q, qsum, unit, sees, t0, g, now.hole, next, codes_to_values, words_to_values, lane_codes,
+                                   lane_words, acc, M, L, Z);
+        now = next;
+        t0 += 128;
+    }
+    while (t0 < hi) {
+        if ((now.hole[0] || now.hole[1]) && lane == 0) atomicOr(a.status, 1u);
+        next = now;
+        advance();
+        attend<D, BITS, NT, true>(c, q, qsum, unit, sees, t0, g, now.hole, next, codes_to_values, words_to_values, lane_codes,
+                                  lane_words, acc, M, L, Z);
+        now = next;
+        t0 += 128;
     }
 
     // the four waves' sums, in a fixed order
