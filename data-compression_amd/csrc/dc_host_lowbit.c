@@ -8,6 +8,7 @@
 #include <hip/hip_runtime_api.h>
 #include <stdint.h>
 #include <string.h>
+#include <stdlib.h>
 
 #include "dc_shared.h"
 #include "../../include/dc_gpu.h"
@@ -125,10 +126,14 @@ static int plan(const dc_kv_cache* c, int batch, int tokens, int q_heads, long l
     a->row_slots = (unsigned)rows;
     const long long base = (long long)batch * c->heads * a->tiles;
     if (base > (1ll << 30)) return 1;
-    long long splits = base > 0 ? (1024 + base - 1) / base : 1, most = (max_context + 255) / 256;
+    long long T = 1024, SH = 640, MX=2; const char* e_ = getenv("DC_T"); if (e_) T = atoll(e_); e_ = getenv("DC_SH"); if (e_) SH = atoll(e_); e_ = getenv("DC_MX"); if (e_) MX = atoll(e_);
+    long long splits = base > 0 && max_context > SH ? MX * ((T + base - 1) / base) : 1;
+    const long long most = (max_context + 255) / 256;
+    if (base >= T) splits = 1;
     if (splits > most) splits = most;
     if (splits > 256) splits = 256;
     a->splits = splits < 1 ? 1u : (unsigned)splits;
+    a->target = (unsigned)(T > base ? T - base / 2 : T);
     return 0;
 }
 
@@ -164,7 +169,7 @@ int dc_kv_attention_device(const dc_kv_cache* cache, const dc_kv_batch* at, int 
         REFUSE("attention: queries, output and lse are aligned to their types");
     if (plan(cache, at->batch, at->tokens, q_heads, max_context, &a)) REFUSE("attention: too many query rows in one call");
     if ((long long)a.splits * a.tiles * a.heads * a.batch > (1ll << 31) - 1 ||
-        (a.splits > 1 && (long long)a.row_slots * a.heads * a.batch > (1ll << 31) - 1))
+        (a.splits > 1 && (long long)a.row_slots * a.heads * a.batch * 8 > (1ll << 31) - 1))
         REFUSE("attention: too many query rows in one call");
     const size_t need = workspace_of(&a, at->batch);
     if (need && (!d_workspace || workspace_bytes < need || ((uintptr_t)d_workspace & 15u)))

@@ -15,6 +15,7 @@
 // reads a block of 16 tokens of either as one contiguous piece.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <utility>
 #include "dc_shared.h"
 #include "../../include/dc_gpu.h"
 
@@ -245,10 +246,15 @@ template <class E, int D, int BITS, bool VEC> __global__ __launch_bounds__(256) 
 // exponent on, in which a subnormal counts as 2^-14: it is exact to 2^-18 (4 bits; 2^-14: 8 bits) of a code's unit times the
 // largest weight.  (In bits 0..3 that were 2^-14 of 15.)
 //
-// The weights w_t = p_t vs_t go into the product as f16.  A running maximum of log2(p_t) + exponent(vs_t) keeps the
-// largest of them in [1, 2^9], whatever the steps are; the sum of p_t is kept in f32 with the same reference.  f16 has 11
-// bits: each w_t is off by 2^-11 of itself at most, half a unit of what f16 outputs round to and less than bf16's.
+// The weights w_t = p_t vs_t go into the product as f16, vs_t in units of the power of two 2^(R - 7) above the largest
+// step that the wave has met: p_t <= 2^8 (the running maximum of the scores is raised only when a score passes it by 8),
+// so w_t < 2^15, and 11 bits are kept down to 2^-21 of that step's full weight, fewer below: a weight is off by 2^-11 of
+// itself, half a unit of what f16 outputs round to, or by 2^-32 of the largest step.  The sum of p_t is kept in f32.
 // Queries are scaled to 2^14..2^15 by a power of two (exact); elements 2^-30 of a row's largest lose bits.
+//
+// A token's words are wanted by the 16 lanes that share its 4 tokens of a block: lane % 8 decodes one of the group's 8
+// tokens, and the others take the factors from it by DPP (row_newbcast), mostly within the instruction that uses them.
+// (Decoded by every lane for itself that was 80 of a step's 300 vector instructions, which bound it at short heads.)
 static __device__ __forceinline__ float over_groups_max(float x) {     // over the 4 groups of 16 lanes
     auto p = __builtin_amdgcn_permlane32_swap((int)asu(x), (int)asu(x), false, false);
     x = fmaxf(asf((uint32_t)p[0]), asf((uint32_t)p[1]));
@@ -296,9 +302,17 @@ template <int BITS> static __device__ __forceinline__ constexpr int key_order(in
     else return (e & 4) + ((e >> 1) & 1) + 2 * (e & 1);
 }
 
+// lane T of the row's 16
+template <int T> static __device__ __forceinline__ float row_lane(float x) {
+    return asf((uint32_t)__builtin_amdgcn_update_dpp(0, (int)asu(x), 0x150 + T, 0xF, 0xF, true));
+}
+template <int... I, class F> static __device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F f) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+
 template <int U> struct Stage {         // what a lane holds of 32 tokens: 2 blocks of 16
     uint32_t k[2][U], v[2][U + 1];      // (one word more: a 16-bit piece may end in it; never used)
-    u4 kw[2], vw[2];
+    uint32_t kw, vw;                    // of token 16 j + 4 g + r, j and r the bits of lane % 8
 };
 // where a step's two blocks lie: the first byte of their keys' codes and of their words (uniform over a wave), and
 // whether they are not in the cache
@@ -326,9 +340,9 @@ template <int N, bool LSE = true> static __device__ __forceinline__ void put(con
     }
     if (LSE && a.lse && d0 == 0) a.lse[((long long)b * a.tokens + i) * a.heads * a.group + hq] = lse;
 }
-// the log of a row's sum l with the reference m (in which an exponent counts one more)
-static __device__ __forceinline__ float log_sum(float m, float l) { return (m - 1.0f + log2f(l)) * 0.69314718055994530942f; }
-// 1 / l; NaN where a row is NaN (its sum is then negative or NaN) or nothing of what a query sees is in the cache
+// the log of a row's sum l with the reference m
+static __device__ __forceinline__ float log_sum(float m, float l) { return (m + log2f(l)) * 0.69314718055994530942f; }
+// 1 / l; NaN where it is NaN, or nothing of what a query sees is in the cache
 static __device__ __forceinline__ float inverse_sum(float l) { return l > 0.0f ? 1.0f / l : asf(0x7FC00000u); }
 
 template <int U> static __device__ __forceinline__ void load_keys(Stage<U>& c, const Where& at, uint32_t lane_codes) {
@@ -339,12 +353,10 @@ template <int U> static __device__ __forceinline__ void load_values(Stage<U>& c,
 #pragma unroll
     for (int j = 0; j < 2; j++) load_n<uint32_t, U, 4 * (U & -U)>((const uint32_t*)(at.codes[j] + to_values + lane_codes), c.v[j]);
 }
-template <int U> static __device__ __forceinline__ void load_words(Stage<U>& c, const Where& at, uint32_t to_values, uint32_t lane_words) {
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-        c.kw[j] = *(const u4*)(at.words[j] + lane_words);
-        c.vw[j] = *(const u4*)(at.words[j] + to_values + lane_words);
-    }
+template <int U> static __device__ __forceinline__ void load_words(Stage<U>& c, const Where& at, uint32_t to_values, bool second, uint32_t lane_words) {
+    const uint8_t* p = (second ? at.words[1] : at.words[0]) + lane_words;
+    c.kw = *(const uint32_t*)p;
+    c.vw = *(const uint32_t*)(p + to_values);
 }
 
 // One step of a wave: 32 tokens from t0 on against NT tiles of 16 queries.  EDGE: some of them may not be seen.  What the
@@ -352,10 +364,10 @@ template <int U> static __device__ __forceinline__ void load_words(Stage<U>& c, 
 // rest of this step and the beginning of the next.
 template <int D, int BITS, int NT, bool EDGE>
 static __device__ __forceinline__ void attend(Stage<D * BITS / 128>& c, const Frag (*q)[D / 32], const float* qsum,
-                                              const float* unit, const int* sees, int t0, int g, const bool* hole,
-                                              const Where& next, uint64_t codes_to_values, uint32_t words_to_values,
-                                              uint32_t lane_codes, uint32_t lane_words, f4 (*acc)[D / 16], float* M,
-                                              float* L, float* Z) {
+                                              const float* unit, const int* sees, int t0, int most, int g,
+                                              const bool* hole, const Where& next, uint64_t codes_to_values,
+                                              uint32_t words_to_values, uint32_t lane_codes, bool second, uint32_t lane_words,
+                                              f4 (*acc)[D / 16], float* M, float* L, float* Z, float& R) {
     constexpr int N = D / 16, U = N * BITS / 8, KS = D / 32, PER = 16 / BITS;
     f4 s[NT][2];
 #pragma unroll
@@ -371,59 +383,69 @@ static __device__ __forceinline__ void attend(Stage<D * BITS / 128>& c, const Fr
             for (int nt = 0; nt < NT; nt++) s[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k.v, q[nt][st].v, s[nt][j], 0, 0, 0);
         }
     load_keys(c, next, lane_codes);
-    // a token's words: keys' step and zero point; values' exponent + 1, significand, 2^-exponent, zero point.  (The
-    // exponent without its bias: what is added to a score costs it bits)
+    // the lane's token's words.  (Behind the last position that is seen there may be anything)
+    if (EDGE) {
+        const int at = t0 + (second ? 16 : 0) + (int)(lane_words >> 2);
+        if (at >= most || hole[second]) c.kw = c.vw = 0;
+    }
+    const float ks = asf(c.kw << 16), kz = (float)(int16_t)(c.kw >> 16), vs = asf(c.vw << 16), vz = (float)(int16_t)(c.vw >> 16);
     float ref[NT][8], mx[NT];
     int left[NT][2];
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) mx[nt] = -INFINITY;
+    for (int nt = 0; nt < NT; nt++) {
+        mx[nt] = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) left[nt][j] = hole[j] ? 0 : sees[nt] - (t0 + 16 * j + 4 * g);   // tokens of this lane that are seen
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const uint32_t kw = c.kw[j][r], vw = c.vw[j][r];
-            const float ks = asf(kw << 16), kz = (float)(int16_t)(kw >> 16);
-            const float ve = (float)__builtin_amdgcn_frexp_expf(asf(vw << 16));
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                float y = fmaf(fmaf(kz, qsum[nt], s[nt][j][r]) * unit[nt], ks, ve);
-                if (EDGE && r >= left[nt][j]) y = -INFINITY;
-                ref[nt][4 * j + r] = y;
-                mx[nt] = fmaxf(mx[nt], y);
-            }
-        }
+        for (int j = 0; j < 2; j++) left[nt][j] = hole[j] ? 0 : sees[nt] - (t0 + 16 * j + 4 * g);   // tokens of this lane that are seen
     }
+    each_of(std::make_integer_sequence<int, 8>{}, [&](auto I) {
+        constexpr int t = I.value;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            float y = fmaf(s[nt][t >> 2][t & 3], unit[nt], row_lane<t>(kz) * qsum[nt]) * row_lane<t>(ks);
+            if (EDGE && (t & 3) >= left[nt][t >> 2]) y = -INFINITY;
+            ref[nt][t] = y;
+            mx[nt] = fmaxf(mx[nt], y);
+        }
+    });
+    // a score that passes its maximum by 8, or a step as large as the unit (not a NaN): new references
+    bool raise = vs >= R;
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-        const float top = over_groups_max(mx[nt]);
-        if (__any(top > M[nt] + 8.0f)) {                    // (weights stay below 2^9)
-            const float m = fmaxf(M[nt], top), al = __builtin_amdgcn_exp2f(M[nt] - m);
+        mx[nt] = over_groups_max(mx[nt]);
+        raise |= mx[nt] > M[nt] + 8.0f;
+    }
+    if (__any(raise)) {
+        float top = vs >= R ? vs : 0.0f;
+        for (int k = 32; k; k >>= 1) top = fmaxf(top, __shfl_xor(top, k));
+        const float r = fmaxf(R, asf((asu(top) & 0x7F800000u) + 0x00800000u));
+        const float down = asf((uint32_t)max((int)(0x3F800000u + asu(R) - asu(r)), 0));     // R / r, powers of two
+        R = r;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const float m = mx[nt] > M[nt] + 8.0f ? mx[nt] : M[nt], al = __builtin_amdgcn_exp2f(M[nt] - m);
             M[nt] = m;
             L[nt] *= al;
-            Z[nt] *= al;
+            Z[nt] *= al * down;
 #pragma unroll
-            for (int i = 0; i < N; i++) acc[nt][i] *= al;
+            for (int i = 0; i < N; i++) acc[nt][i] *= al * down;
         }
     }
+    const float vr = vs * asf(0x7F000000u - asu(R)) * 128.0f;       // 2^7 / R
     Frag w[NT];
-#pragma unroll
-    for (int t = 0; t < 8; t++) {
-        const uint32_t vw = c.vw[t >> 2][t & 3], step = vw << 16;
-        const float vm = asf((step & 0x007FFFFFu) | 0x3F800000u), vz = (float)(int16_t)(vw >> 16);
-        const float vi = asf(0x7F000000u - (step & 0x7F800000u));       // (a NaN's: minus infinity, which stays in the sum)
+    each_of(std::make_integer_sequence<int, 8>{}, [&](auto I) {
+        constexpr int t = I.value;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
             const float p = __builtin_amdgcn_exp2f(ref[nt][t] - M[nt]);
-            const _Float16 wt = (_Float16)(p * vm);
-            const float l = fmaf(p, vi, L[nt]);
-            L[nt] = EDGE && (t & 3) >= left[nt][t >> 2] ? L[nt] : l;
-            Z[nt] = fmaf((float)wt, vz, Z[nt]);
+            float x = p * row_lane<t>(vr);
+            if (EDGE && (t & 3) >= left[nt][t >> 2]) x = 0.0f;      // (0 times a NaN)
+            const _Float16 wt = (_Float16)x;
+            L[nt] += p;
+            Z[nt] = fmaf((float)wt, row_lane<t>(vz), Z[nt]);
             w[nt].v[t] = wt;
         }
-    }
-    load_words(c, next, words_to_values, lane_words);
+    });
+    load_words(c, next, words_to_values, second, lane_words);
     // values: unit lane % 16, tokens 4 g .. 4 g + 3 of both blocks, 16 bits of each token at a time
 #pragma unroll
     for (int i0 = 0; i0 < N; i0 += PER) {
@@ -446,28 +468,52 @@ static __device__ __forceinline__ void attend(Stage<D * BITS / 128>& c, const Fr
     load_values(c, next, codes_to_values, lane_codes);
 }
 
-template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_attention(KvArgs a) {
+static __device__ __forceinline__ int context_of(const KvArgs& a, uint32_t b) {
+    return (int)min((long long)max(((const Const*)a.start)[b], 0), a.capacity);
+}
+// Into how many pieces (at most a.splits) sequence b's positions are cut, and how long they are: all workgroups of a call
+// get about the same number of positions, whatever the sequences' lengths, and there are about a.target of them.  (A cut
+// by the same number for all takes as long as the longest sequence's piece.)  Called by all lanes of a wave.
+static __device__ __forceinline__ int cut(const KvArgs& a, int context, int& pieces) {
+    pieces = 1;
+    if (a.splits > 1) {
+        float total = (float)context;
+        if (a.batch > 1) {
+            total = 0.0f;
+            for (int i = threadIdx.x & 63; i < a.batch; i += 64) total += (float)min((long long)max(a.start[i], 0), a.capacity);
+            for (int m = 32; m; m >>= 1) total += __shfl_xor(total, m);
+            total = asf(__builtin_amdgcn_readfirstlane(asu(total)));
+        }
+        const int even = max((int)min(total * (float)a.heads * (float)a.tiles / (float)a.target, 1e9f), 255) + 1;
+        pieces = max(min((context + even - 1) / even, (int)a.splits), 1);
+    }
+    return ((context + pieces - 1) / pieces + 127) & ~127;
+}
+
+#ifndef KW
+#define KW 1
+#endif
+template <int D, int BITS, int NT> __global__ __launch_bounds__(256, (NT == 1 && D <= 128 && BITS == 4) ? KW : 1) void kv_attention(KvArgs a) {
     constexpr int N = D / 16, U = N * BITS / 8, ROW = 16 * U, KS = D / 32, COLS = 16 * NT;
     constexpr bool ALL = D * NT <= 256;                     // every wave its own sums in LDS, or one after the other
     __shared__ float acc_lds[(ALL ? 4 : 1) * N * 16 * COLS];
     __shared__ float ml[3][4][COLS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
-    // block -> (split, tile of query rows, head, sequence)
+    // Workgroup -> (piece, sequence, head, tile of query rows), the tile fastest: workgroups go round the 8 XCDs one by
+    // one, and pieces that a short sequence does not have lie together at the end.  (With the piece as the fastest index
+    // whole XCDs idle; a head's tiles kept on one XCD are slower where there are few heads, of unequal lengths.)
     uint32_t x = blockIdx.x;
-    const uint32_t split = x % a.splits; x /= a.splits;
     const uint32_t tile = x % a.tiles; x /= a.tiles;
-    const uint32_t h = x % a.heads, b = x / a.heads;
-    int context = ((const Const*)a.start)[b];
-    if (context < 0 || context > a.capacity) {
-        if (threadIdx.x == 0) atomicOr(a.status, 1u);
-        context = context < 0 ? 0 : (int)a.capacity;
-    }
+    const uint32_t h = x % a.heads; x /= a.heads;
+    const uint32_t b = x % a.batch, split = x / a.batch;
+    const int context = context_of(a, b);
+    if (context != a.start[b] && threadIdx.x == 0) atomicOr(a.status, 1u);
     const int len = a.lens ? min(max(((const Const*)a.lens)[b], 0), a.tokens) : a.tokens;
     const int rows = len * a.group;
     const int row0 = tile * COLS;
     const int oc = threadIdx.x & 15, ou = threadIdx.x >> 4;     // a thread's output: a row, a unit
-    if (a.zero_padding && a.splits == 1) {
+    if (a.zero_padding && split == 0) {
         const float zero[N] = {};
         for (int nt = 0; nt < NT; nt++) {
             const int rw = row0 + nt * 16 + oc;
@@ -475,6 +521,9 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_att
         }
     }
     if (row0 >= rows) return;
+    int pieces;
+    const int chunk = cut(a, context, pieces);
+    if ((int)split >= pieces) return;
     // what the tile's queries see: positions below sees, from least (all of them) to most (the last one)
     const int last_row = min(row0 + COLS, rows) - 1;
     int least = context, most = context;
@@ -488,11 +537,10 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_att
         const int i = (int)div_by((uint32_t)min(row0 + nt * 16 + col, last_row), a.group_inv);
         sees[nt] = a.causal ? max(context - len + 1 + i, 0) : context;
     }
-    const int chunk = ((context + (int)a.splits - 1) / (int)a.splits + 127) & ~127;
     const long long lo64 = (long long)split * chunk;
     const int lo = lo64 < most ? (int)lo64 : most, hi = (int)min((long long)most, lo64 + chunk);
 
-    // queries, as f16 in the keys' order; their sum; the factor that takes a score to log2 units
+    // queries, as f16 in the keys' order; their sum and the factor that takes a score to log2 units
     Frag q[NT][KS];
     float qsum[NT], unit[NT];
 #pragma unroll
@@ -531,12 +579,13 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_att
                 q[nt][j].v[k] = v;
                 sum += (float)v;
             }
-        qsum[nt] = over_groups_sum(sum) * (1.0f / UNIT<BITS>);
-        unit[nt] = a.scale * 1.44269504088896340736f * down * UNIT<BITS>;
+        const float u = a.scale * 1.44269504088896340736f * down;
+        qsum[nt] = over_groups_sum(sum) * u;
+        unit[nt] = u * UNIT<BITS>;
     }
 
     f4 acc[NT][N];
-    float M[NT], L[NT], Z[NT];
+    float M[NT], L[NT], Z[NT], R = 1.17549435e-38f;         // (2^-126: below every step)
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
         M[nt] = -1e30f;
@@ -551,7 +600,8 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_att
     const uint32_t blocks = (uint32_t)a.page >> 4, slot_step = div_by(8u, a.blocks_inv), in_step = 8u - slot_step * blocks;
     const int first = lo + wave * 32;
     uint32_t slot = div_by((uint32_t)first >> 4, a.blocks_inv), in = ((uint32_t)first >> 4) - slot * blocks;
-    const uint32_t lane_codes = (uint32_t)(col * ROW + g * (4 * U)), lane_words = (uint32_t)g * 16;
+    const uint32_t lane_codes = (uint32_t)(col * ROW + g * (4 * U)), lane_words = (uint32_t)(g * 4 + (lane & 3)) * 4;
+    const bool second = lane & 4;
     const uint64_t codes_to_values = (uint64_t)a.page * ROW;
     const uint32_t words_to_values = 4u * (uint32_t)a.page;
     int page[2];
@@ -582,7 +632,7 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_att
         find(first);
         where(now);
         load_keys(c, now, lane_codes);
-        load_words(c, now, words_to_values, lane_words);
+        load_words(c, now, words_to_values, second, lane_words);
         load_values(c, now, codes_to_values, lane_codes);
         if (first + 128 < hi) find(first + 128);
     }
@@ -597,8 +647,8 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_att
     while (t0 < hi && t0 + 32 <= least && t0 + 32 <= hi && !now.hole[0] && !now.hole[1]) {
         next = now;
         advance();
-        attend<D, BITS, NT, false>(c, q, qsum, unit, sees, t0, g, now.hole, next, codes_to_values, words_to_values, lane_codes,
-                                   lane_words, acc, M, L, Z);
+        attend<D, BITS, NT, false>(c, q, qsum, unit, sees, t0, most, g, now.hole, next, codes_to_values, words_to_values,
+                                   lane_codes, second, lane_words, acc, M, L, Z, R);
         now = next;
         t0 += 128;
     }
@@ -606,8 +656,8 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_att
         if ((now.hole[0] || now.hole[1]) && lane == 0) atomicOr(a.status, 1u);
         next = now;
         advance();
-        attend<D, BITS, NT, true>(c, q, qsum, unit, sees, t0, g, now.hole, next, codes_to_values, words_to_values, lane_codes,
-                                  lane_words, acc, M, L, Z);
+        attend<D, BITS, NT, true>(c, q, qsum, unit, sees, t0, most, g, now.hole, next, codes_to_values, words_to_values,
+                                  lane_codes, second, lane_words, acc, M, L, Z, R);
         now = next;
         t0 += 128;
     }
@@ -620,7 +670,7 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_att
         if (g == 0) {
             ml[0][wave][nt * 16 + col] = M[nt];
             ml[1][wave][nt * 16 + col] = L[nt];
-            ml[2][wave][nt * 16 + col] = Z[nt];
+            ml[2][wave][nt * 16 + col] = Z[nt] * (R * 0.0078125f);
         }
     }
     __syncthreads();
@@ -629,7 +679,7 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_att
     for (int nt = 0; nt < NT; nt++) {
         float m = ml[0][0][nt * 16 + col];
         for (int v = 1; v < 4; v++) m = fmaxf(m, ml[0][v][nt * 16 + col]);
-        f[nt] = __builtin_amdgcn_exp2f(M[nt] - m) * UNIT<BITS>;
+        f[nt] = __builtin_amdgcn_exp2f(M[nt] - m) * (R * 0.0078125f) * UNIT<BITS>;
     }
     for (int v = 0; v < (ALL ? 1 : 4); v++) {
         if (ALL || wave == v)
@@ -664,7 +714,7 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_att
             for (int v = 0; v < (ALL ? 4 : 1); v++) y += acc_lds[((v * NT + nt) * N + i) * 256 + ou * 16 + oc];
             o[i] = y;
         }
-        if (a.splits > 1) {                                 // unnormalised, with its maximum and sum
+        if (pieces > 1) {                                   // unnormalised, with its maximum and sum
             const long long at = ((((long long)b * a.heads + h) * a.row_slots + rw) * a.splits + split);
             float* p = a.part + at * D + ou * N;
             for (int k = 0; k < N; k++) p[k] = o[k];
@@ -682,53 +732,82 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256) void kv_att
     }
 }
 
-// the splits of a query row joined, in their order: a workgroup per row
-template <int D> __global__ __launch_bounds__(256) void kv_join(KvArgs a) {
-    constexpr int N = D / 16;
-    __shared__ float sums[16][D];
-    __shared__ float ms[16], lsum[16];
+// The pieces of a query row joined, in a fixed order.  Few pieces: 32 or 64 lanes for a row, four values each, one piece
+// after the other.
+template <int D> __global__ __launch_bounds__(256) void kv_join_few(KvArgs a) {
+    constexpr int LANES = D <= 128 ? 32 : 64, ROWS = 256 / LANES;
     uint32_t x = blockIdx.x;
+    const uint32_t row_blocks = (a.row_slots + ROWS - 1) / ROWS;
+    const int rw = (int)(x % row_blocks) * ROWS + (int)threadIdx.x / LANES; x /= row_blocks;
+    const uint32_t h = x % a.heads, b = x / a.heads;
+    const int context = context_of(a, b), len = a.lens ? min(max(((const Const*)a.lens)[b], 0), a.tokens) : a.tokens;
+    int pieces;
+    cut(a, context, pieces);
+    const int d0 = (int)threadIdx.x % LANES * 4;
+    if (rw >= len * a.group || pieces == 1 || d0 >= D) return;
+    const long long at = (((long long)b * a.heads + h) * a.row_slots + rw) * a.splits;
+    float m = -1e30f, l = 0.0f;
+    for (int s = 0; s < pieces; s++) m = fmaxf(m, a.part_ml[2 * (at + s)]);
+    f4 o = {0, 0, 0, 0};
+#pragma unroll 4
+    for (int s = 0; s < pieces; s++) {
+        const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * (at + s)] - m);
+        l = fmaf(a.part_ml[2 * (at + s) + 1], f, l);
+        o += *(const f4*)(a.part + (at + s) * D + d0) * f;
+    }
+    const bool none = (a.causal ? context - len + 1 + (int)div_by((uint32_t)rw, a.group_inv) : context) <= 0;
+    const float inv = none ? 0.0f : inverse_sum(l);
+    float y[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) y[k] = none ? 0.0f : o[k] * inv;
+    put<4>(a, b, h, rw, d0, y, none ? -INFINITY : log_sum(m, l));
+}
+
+// Many pieces: a workgroup for 32 values of a row.  The pieces' references and sums first, a thread each (at most 256),
+// then 8 x 32 threads, four values of every 32nd piece each.
+template <int D> __global__ __launch_bounds__(256) void kv_join(KvArgs a) {
+    __shared__ float f[256], red[2][4];
+    __shared__ f4 sums[32][8];
+    uint32_t x = blockIdx.x;
+    const uint32_t d0 = x % (D / 32) * 32; x /= D / 32;
     const uint32_t rw = x % a.row_slots; x /= a.row_slots;
     const uint32_t h = x % a.heads, b = x / a.heads;
-    const int len = a.lens ? min(max(a.lens[b], 0), a.tokens) : a.tokens;
-    if ((int)rw >= len * a.group) {
-        const float zero = 0.0f;
-        if (a.zero_padding)
-            for (int d = threadIdx.x; d < D; d += 256) put<1, false>(a, b, h, (int)rw, d, &zero, 0.0f);
-        return;
-    }
-    const int u = threadIdx.x & 15, part = threadIdx.x >> 4;
+    const int context = context_of(a, b), len = a.lens ? min(max(((const Const*)a.lens)[b], 0), a.tokens) : a.tokens;
+    int pieces;
+    cut(a, context, pieces);
+    if ((int)rw >= len * a.group || pieces == 1) return;
+    const int tid = threadIdx.x;
     const long long at = (((long long)b * a.heads + h) * a.row_slots + rw) * a.splits;
-    float m = -1e30f, l = 0.0f, o[N];
-    for (int k = 0; k < N; k++) o[k] = 0.0f;
-    for (uint32_t s = part; s < a.splits; s += 16) {
-        const float pm = a.part_ml[2 * (at + s)], pl = a.part_ml[2 * (at + s) + 1];
-        const float nm = fmaxf(m, pm), fa = __builtin_amdgcn_exp2f(m - nm), fb = __builtin_amdgcn_exp2f(pm - nm);
-        const float* p = a.part + (at + s) * D + u * N;
-        for (int k = 0; k < N; k++) o[k] = fmaf(p[k], fb, o[k] * fa);
-        l = fmaf(pl, fb, l * fa);
-        m = nm;
+    float m = -1e30f, l = 0.0f;
+    if (tid < pieces) {
+        m = a.part_ml[2 * (at + tid)];
+        l = a.part_ml[2 * (at + tid) + 1];
     }
-    for (int k = 0; k < N; k++) sums[part][u * N + k] = o[k];
-    if (u == 0) { ms[part] = m; lsum[part] = l; }
+    float top = m;
+    for (int k = 32; k; k >>= 1) top = fmaxf(top, __shfl_xor(top, k));
+    if ((tid & 63) == 0) red[0][tid >> 6] = top;
     __syncthreads();
-    m = ms[0];
-    for (int k = 1; k < 16; k++) m = fmaxf(m, ms[k]);
-    l = 0.0f;
-    float f[16];
-    for (int k = 0; k < 16; k++) {
-        f[k] = __builtin_amdgcn_exp2f(ms[k] - m);
-        l = fmaf(lsum[k], f[k], l);
-    }
-    int context = a.start[b];
-    context = context < 0 ? 0 : context > a.capacity ? (int)a.capacity : context;
-    const bool none = (a.causal ? context - len + 1 + (int)div_by(rw, a.group_inv) : context) <= 0;
-    const float lse = none ? -INFINITY : log_sum(m, l), inv = inverse_sum(l);
-    for (int d = threadIdx.x; d < D; d += 256) {
+    top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    const float scale = __builtin_amdgcn_exp2f(m - top);
+    f[tid] = scale;
+    l *= scale;
+    for (int k = 32; k; k >>= 1) l += __shfl_xor(l, k);
+    if ((tid & 63) == 0) red[1][tid >> 6] = l;
+    __syncthreads();
+    l = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+    const int dl = tid & 7, sl = tid >> 3;
+    f4 o = {0, 0, 0, 0};
+    const float* p = a.part + at * D + d0 + dl * 4;
+#pragma unroll 4
+    for (int s = sl; s < pieces; s += 32) o += *(const f4*)(p + (long long)s * D) * f[s];
+    sums[sl][dl] = o;
+    __syncthreads();
+    if (tid < 32) {
         float y = 0.0f;
-        for (int k = 0; k < 16; k++) y = fmaf(sums[k][d], f[k], y);
-        y = none ? 0.0f : y * inv;
-        put<1>(a, b, h, (int)rw, d, &y, lse);
+        for (int k = 0; k < 32; k++) y += ((const float*)&sums[k][0])[tid];
+        const bool none = (a.causal ? context - len + 1 + (int)div_by(rw, a.group_inv) : context) <= 0;
+        y = none ? 0.0f : y * inverse_sum(l);
+        put<1>(a, b, h, (int)rw, (int)d0 + tid, &y, none ? -INFINITY : log_sum(top, l));
     }
 }
 
@@ -761,7 +840,10 @@ template <int D, int BITS> int go_attention(const KvArgs& a, hipStream_t st) {
         if (a.cols == 16) kv_attention<D, BITS, 1><<<grid, 256, 0, st>>>(a);
         else kv_attention<D, BITS, WIDE><<<grid, 256, 0, st>>>(a);
     } else kv_attention<D, BITS, 1><<<grid, 256, 0, st>>>(a);
-    if (a.splits > 1) kv_join<D><<<(unsigned)((long long)a.row_slots * a.heads * a.batch), 256, 0, st>>>(a);
+    constexpr int ROWS = D <= 128 ? 8 : 4;                  // (kv_join_few)
+    if (a.splits > 16) kv_join<D><<<(unsigned)((long long)a.row_slots * a.heads * a.batch * (D / 32)), 256, 0, st>>>(a);
+    else if (a.splits > 1)
+        kv_join_few<D><<<(unsigned)((long long)((a.row_slots + ROWS - 1) / ROWS) * a.heads * a.batch), 256, 0, st>>>(a);
     return hipGetLastError() != hipSuccess;
 }
 

@@ -127,7 +127,7 @@ typedef struct KvArgs {
     float* lse;
     float* part;                   /* [batch][heads][row_slots][splits][dim] unnormalised sums */
     float* part_ml;                /* the same places: maximum, sum */
-    unsigned splits, tiles, row_slots, cols;
+    unsigned splits, target, tiles, row_slots, cols;   /* pieces of a sequence at most; workgroups aimed at */
 } KvArgs;
 
 /* activation checkpoints (dc_act.hip) */

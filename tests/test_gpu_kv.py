@@ -259,7 +259,8 @@ def formula(f, q, context, lens, scale, causal):
 
     With u = 2^-24: a score is a sum of D products of codes with queries (at most D + 8 roundings, each u of the
     sum of magnitudes A = ks (sum |q| code + |kz| sum |q|)), so a weight is off by (D + 8) u scale A of itself, and by
-    2^-11 (to f16) + 8 u (its factors); weights below f16's range by 2^-25 of the largest, which is 1 or more.  The sum
+    2^-11 (to f16) + 8 u (its factors); weights below f16's normal range by 2^-25 of units of which the largest step is
+    64 or more.  The sum
     over positions adds N u of magnitudes; the output's type half a unit.  A matrix instruction cuts each of its 33 terms
     at 24 bits below the largest one's exponent, in which a code counts as 2^-14: at 2^-18 (codes are n 2^-20: 4 bits) or
     2^-14 (n 2^-24: 8 bits) of a code times the largest query element or weight; D / 32 of them make a score, a 32nd of N
@@ -291,7 +292,8 @@ def formula(f, q, context, lens, scale, causal):
                 w = p * f.vs[b, :n, h].t()
                 largest = w.amax(-1, keepdim=True)
                 err = (p * (eps + 2.0 ** -11)) @ v.abs() + (p * eps).sum(-1, keepdim=True) * o.abs()
-                err = err + ((n + 8) * u * w + 2.0 ** -25 * largest) @ (mag / f.vs[b, :n, h])
+                tiny = 2.0 ** -31 * f.vs[b, :n, h].max()
+                err = err + ((n + 8) * u * w + tiny) @ (mag / f.vs[b, :n, h])
                 err = err + cut * (n / 32 + 4 * (1 + n / 256)) * largest
                 out[b, i, h * G:(h + 1) * G] = o
                 lse[b, i, h * G:(h + 1) * G, 0] = torch.logsumexp(s, -1)
