@@ -8,7 +8,6 @@
 #include <hip/hip_runtime_api.h>
 #include <stdint.h>
 #include <string.h>
-#include <stdlib.h>
 
 #include "dc_shared.h"
 #include "../../include/dc_gpu.h"
@@ -112,9 +111,13 @@ int dc_kv_read_device(const dc_kv_cache* cache, const dc_kv_batch* at, int dtype
     return rows_call(cache, at, dtype, d_k, k_strides, d_v, v_strides, stream, 0);
 }
 
-/* How the attention is cut: query rows (tokens x the group that shares a head) in tiles of 16, or of as many as a wave's
- * registers hold where there are more; the cache's positions in `splits` where that alone would leave compute units
- * without work.  A split is a whole number of 128 tokens (the four waves' 32 each). */
+/* How the attention is cut.  Query rows (tokens x the group that shares a head) in tiles of 16, or of as many as a wave's
+ * registers hold where there are more.  The cache's positions in up to `splits` pieces a sequence, so that there are
+ * about 768 workgroups, 3 per compute unit (48 sequences of up to 8192 positions, 8 heads: 512 88 us, 768 79, 1024 84;
+ * one of 262143, 2 heads: 256 25 us, 512 and more 22), or half of that where a compute unit holds two of them, wide tiles
+ * and long rows (16 sequences of 8192, heads of 256: 256 37 us, 384 32, 768 38; 8 queries each, heads of 64: 256 31,
+ * 384 27, 768 33); up to twice the even number of pieces, for sequences longer than the others.  None up to 640 positions: there a second kernel, which joins the pieces, costs what they save (8 heads, 517
+ * positions: 10.2 us in one piece, 7.0 + 2.8 in three). */
 static int plan(const dc_kv_cache* c, int batch, int tokens, int q_heads, long long max_context, KvArgs* a) {
     if (q_heads < 1 || q_heads % c->heads) return 1;
     const long long group = q_heads / c->heads, rows = (long long)tokens * group;
@@ -126,14 +129,17 @@ static int plan(const dc_kv_cache* c, int batch, int tokens, int q_heads, long l
     a->row_slots = (unsigned)rows;
     const long long base = (long long)batch * c->heads * a->tiles;
     if (base > (1ll << 30)) return 1;
-    long long T = 1024, SH = 640, MX=2; const char* e_ = getenv("DC_T"); if (e_) T = atoll(e_); e_ = getenv("DC_SH"); if (e_) SH = atoll(e_); e_ = getenv("DC_MX"); if (e_) MX = atoll(e_);
-    long long splits = base > 0 && max_context > SH ? MX * ((T + base - 1) / base) : 1;
-    const long long most = (max_context + 255) / 256;
-    if (base >= T) splits = 1;
-    if (splits > most) splits = most;
-    if (splits > 256) splits = 256;
-    a->splits = splits < 1 ? 1u : (unsigned)splits;
-    a->target = (unsigned)(T > base ? T - base / 2 : T);
+    const int AIM = a->cols == 16 && c->head_dim <= 128 ? 768 : 384;
+    enum { SHORT = 640, LEAST = 256, MOST = 256 };
+    long long splits = 1;
+    if (base > 0 && base < AIM && max_context > SHORT) {
+        const long long most = (max_context + LEAST - 1) / LEAST;
+        splits = 2 * ((AIM + base - 1) / base);
+        if (splits > most) splits = most;
+        if (splits > MOST) splits = MOST;
+    }
+    a->splits = (unsigned)splits;
+    a->target = base < AIM ? (unsigned)(AIM - base / 2) : 1u;
     return 0;
 }
 

@@ -234,7 +234,7 @@ template <class E, int D, int BITS, bool VEC> __global__ __launch_bounds__(256) 
 
 // ---- attention ---------------------------------------------------------------------------------------------------------
 // O = softmax(scale q k^T) v^ over the positions a query sees.  With k^ = s (z + code):
-//     q . k^_t = ks_t (q . code_t + kz_t sum(q)),      O_d = sum_t (p_t vs_t) (code_td + vz_t):
+//     q . k^_t = ks_t q . code_t + ks_t kz_t sum(q),      O_d = sum_t (p_t vs_t) (code_td + vz_t):
 // the matrix instructions see the codes alone, as whole numbers (exact), and a token's step and zero point enter as two
 // multiply-adds on its score and as a factor of its weight.  The queries of a group of heads that share keys are the
 // columns of mfma 16x16x32: A = 16 tokens' codes, B = 16 queries.  The score tile's lane layout (token = 4 (lane / 16) +
@@ -388,7 +388,7 @@ static __device__ __forceinline__ void attend(Stage<D * BITS / 128>& c, const Fr
         const int at = t0 + (second ? 16 : 0) + (int)(lane_words >> 2);
         if (at >= most || hole[second]) c.kw = c.vw = 0;
     }
-    const float ks = asf(c.kw << 16), kz = (float)(int16_t)(c.kw >> 16), vs = asf(c.vw << 16), vz = (float)(int16_t)(c.vw >> 16);
+    const float ks = asf(c.kw << 16), kz = ks * (float)(int16_t)(c.kw >> 16), vs = asf(c.vw << 16), vz = (float)(int16_t)(c.vw >> 16);
     float ref[NT][8], mx[NT];
     int left[NT][2];
 #pragma unroll
@@ -401,7 +401,7 @@ static __device__ __forceinline__ void attend(Stage<D * BITS / 128>& c, const Fr
         constexpr int t = I.value;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            float y = fmaf(s[nt][t >> 2][t & 3], unit[nt], row_lane<t>(kz) * qsum[nt]) * row_lane<t>(ks);
+            float y = fmaf(s[nt][t >> 2][t & 3], row_lane<t>(ks) * unit[nt], row_lane<t>(kz) * qsum[nt]);
             if (EDGE && (t & 3) >= left[nt][t >> 2]) y = -INFINITY;
             ref[nt][t] = y;
             mx[nt] = fmaxf(mx[nt], y);
@@ -490,10 +490,8 @@ static __device__ __forceinline__ int cut(const KvArgs& a, int context, int& pie
     return ((context + pieces - 1) / pieces + 127) & ~127;
 }
 
-#ifndef KW
-#define KW 1
-#endif
-template <int D, int BITS, int NT> __global__ __launch_bounds__(256, (NT == 1 && D <= 128 && BITS == 4) ? KW : 1) void kv_attention(KvArgs a) {
+// (codes of up to 64 bytes a row: four waves per SIMD, 88 us against 92 with three at 48 x 8192 positions)
+template <int D, int BITS, int NT> __global__ __launch_bounds__(256, NT == 1 && D * BITS <= 512 ? 4 : 1) void kv_attention(KvArgs a) {
     constexpr int N = D / 16, U = N * BITS / 8, ROW = 16 * U, KS = D / 32, COLS = 16 * NT;
     constexpr bool ALL = D * NT <= 256;                     // every wave its own sums in LDS, or one after the other
     __shared__ float acc_lds[(ALL ? 4 : 1) * N * 16 * COLS];
@@ -830,8 +828,10 @@ template <class E> int go_bits(const KvArgs& a, bool write, hipStream_t st) {
     return a.vec ? go_rows<E, 8, true>(a, write, st) : go_rows<E, 8, false>(a, write, st);
 }
 
-// tiles of 16 query rows that a wave takes at once where there are many: what its registers hold
-constexpr int wide_tiles(int dim) { return dim <= 64 ? 4 : dim <= 192 ? 2 : 1; }
+// Tiles of 16 query rows that a wave takes at once where there are more than 16 of them: what leaves two waves per SIMD.
+// (509 queries x 4 heads x 8192 positions, 64 values in 8 bits: four tiles, one wave per SIMD more seldom hidden, 102 us,
+// two 88.)
+constexpr int wide_tiles(int dim) { return dim <= 192 ? 2 : 1; }
 
 template <int D, int BITS> int go_attention(const KvArgs& a, hipStream_t st) {
     const unsigned grid = (unsigned)((long long)a.splits * a.tiles * a.heads * a.batch);
