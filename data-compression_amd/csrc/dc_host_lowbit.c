@@ -62,7 +62,6 @@ static int common(const dc_kv_cache* c, const dc_kv_batch* at, KvArgs* a) {
     a->page_inv = inverse((unsigned long long)c->page_size);
     a->blocks_inv = inverse((unsigned long long)c->page_size / 16);
     a->heads_inv = inverse((unsigned long long)c->heads);
-    a->tokens_inv = inverse((unsigned long long)at->tokens);
     return DC_OK;
 }
 
@@ -87,8 +86,10 @@ static int rows_call(const dc_kv_cache* c, const dc_kv_batch* at, int dtype, con
     if (at->batch == 0 || at->tokens == 0) return DC_OK;
     if (!k || !v || !ks || !vs) REFUSE("cache: keys, values and their strides are needed");
     if (((uintptr_t)k | (uintptr_t)v) & (uintptr_t)(size - 1)) REFUSE("cache: keys and values are aligned to their type");
-    if ((long long)at->batch * at->tokens > (1ll << 31) / c->heads) REFUSE("cache: too many rows in one call");
-    a.rows = (long long)at->batch * at->tokens * c->heads * 2;
+    if ((long long)at->batch * at->tokens > (1ll << 30) / c->heads) REFUSE("cache: too many rows in one call");
+    a.blocks = (int)(((long long)at->tokens + 30) / 16);        /* at any place within the first block */
+    a.tokens_inv = inverse((unsigned long long)a.blocks);
+    a.rows = (long long)at->batch * a.blocks * c->heads * (write ? 2 : 1);
     a.k = k;
     a.v = v;
     memcpy(a.ks, ks, sizeof a.ks);

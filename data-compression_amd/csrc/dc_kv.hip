@@ -58,28 +58,38 @@ struct BF16 {
 template <class T, int N, int A> static __device__ __forceinline__ void load_n(const T* p, T* x) {
     constexpr int BYTES = N * (int)sizeof(T);
     if constexpr (A >= 16 && BYTES % 16 == 0) {
+#pragma unroll
         for (int i = 0; i < BYTES / 16; i++) ((uint4*)x)[i] = ((const uint4*)p)[i];
     } else if constexpr (A >= 8 && BYTES % 8 == 0) {
+#pragma unroll
         for (int i = 0; i < BYTES / 8; i++) ((uint2*)x)[i] = ((const uint2*)p)[i];
     } else if constexpr (A >= 4 && BYTES % 4 == 0) {
+#pragma unroll
         for (int i = 0; i < BYTES / 4; i++) ((uint32_t*)x)[i] = ((const uint32_t*)p)[i];
     } else if constexpr (A >= 2 && BYTES % 2 == 0) {
+#pragma unroll
         for (int i = 0; i < BYTES / 2; i++) ((uint16_t*)x)[i] = ((const uint16_t*)p)[i];
     } else {
+#pragma unroll
         for (int i = 0; i < BYTES; i++) ((uint8_t*)x)[i] = ((const uint8_t*)p)[i];
     }
 }
 template <class T, int N, int A> static __device__ __forceinline__ void store_n(T* p, const T* x) {
     constexpr int BYTES = N * (int)sizeof(T);
     if constexpr (A >= 16 && BYTES % 16 == 0) {
+#pragma unroll
         for (int i = 0; i < BYTES / 16; i++) ((uint4*)p)[i] = ((const uint4*)x)[i];
     } else if constexpr (A >= 8 && BYTES % 8 == 0) {
+#pragma unroll
         for (int i = 0; i < BYTES / 8; i++) ((uint2*)p)[i] = ((const uint2*)x)[i];
     } else if constexpr (A >= 4 && BYTES % 4 == 0) {
+#pragma unroll
         for (int i = 0; i < BYTES / 4; i++) ((uint32_t*)p)[i] = ((const uint32_t*)x)[i];
     } else if constexpr (A >= 2 && BYTES % 2 == 0) {
+#pragma unroll
         for (int i = 0; i < BYTES / 2; i++) ((uint16_t*)p)[i] = ((const uint16_t*)x)[i];
     } else {
+#pragma unroll
         for (int i = 0; i < BYTES; i++) ((uint8_t*)p)[i] = ((const uint8_t*)x)[i];
     }
 }
@@ -93,143 +103,201 @@ static __device__ __forceinline__ uint32_t div_by(uint32_t n, unsigned long long
 template <int N> static __device__ __forceinline__ float ror16(float x) {
     return asf((uint32_t)__builtin_amdgcn_update_dpp(0, (int)asu(x), 0x120 + N, 0xF, 0xF, false));
 }
+// (these minima and maxima are NaN if a value is)
+static __device__ __forceinline__ float least(float a, float b) { return __builtin_elementwise_minimum(a, b); }
+static __device__ __forceinline__ float most(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 static __device__ __forceinline__ float min16(float x) {
-    x = fminf(x, ror16<8>(x)); x = fminf(x, ror16<4>(x)); x = fminf(x, ror16<2>(x)); return fminf(x, ror16<1>(x));
+    x = least(x, ror16<8>(x)); x = least(x, ror16<4>(x)); x = least(x, ror16<2>(x)); return least(x, ror16<1>(x));
 }
 static __device__ __forceinline__ float max16(float x) {
-    x = fmaxf(x, ror16<8>(x)); x = fmaxf(x, ror16<4>(x)); x = fmaxf(x, ror16<2>(x)); return fmaxf(x, ror16<1>(x));
+    x = most(x, ror16<8>(x)); x = most(x, ror16<4>(x)); x = most(x, ror16<2>(x)); return most(x, ror16<1>(x));
 }
 
-// the smallest bfloat16 c with c * n >= v, from an estimate of v / n that is not above it (c n is exact: 8 + 8 bits)
-static __device__ __forceinline__ float step_up(float v, float inv_n, float n) {
-    float c = asf(asu(v * inv_n * 0.9999990f) & 0xFFFF0000u);
-    for (int i = 0; i < 2; i++) c = c * n < v ? asf(asu(c) + 0x10000u) : c;
+// the smallest bfloat16 c >= 2^-100 with c * n >= v and c * m >= w, from estimates of v / n and w / m that are not above
+// them and at most two bfloat16s below (the products are exact: 8 + 8 bits)
+static __device__ __forceinline__ float step_up(float v, float inv_n, float n, float w, float inv_m, float m) {
+    float c = asf(asu(fmaxf(fmaxf(v * inv_n, w * inv_m) * 0.9999990f, 7.888609052210118e-31f)) & 0xFFFF0000u);
+#pragma unroll
+    for (int i = 0; i < 2; i++) c = (c * n < v || c * m < w) ? asf(asu(c) + 0x10000u) : c;
     return c;
 }
 
-// rint(x / s) of the exact quotient: an estimate within one, put right by the remainder (exact, as r s has 24 bits)
+// rint(x / s) of the exact quotient: an estimate within one, put right by the remainder, which is exact (r s has 24 bits).
+// It is right to move where the remainder is above half a step, or half a step and r odd: above the float before it.
+// (1.5 * 2^23 added to the estimate rounds it, and leaves it as a whole number in the low bits.)
 static __device__ __forceinline__ float rint_div(float x, float s, float inv, float half) {
-    float r = rintf(x * inv);
-    const float d = fmaf(-r, s, x), a = fabsf(d);
-    const bool up = a > half || (a == half && ((int)r & 1));
-    return up ? r + copysignf(1.0f, d) : r;
+    const float y = fmaf(x, inv, 12582912.0f), r = y - 12582912.0f, d = fmaf(-r, s, x);
+    const float far = asf(asu(half) - (asu(y) & 1u));
+    return r + (fabsf(d) > far ? copysignf(1.0f, d) : 0.0f);
 }
 
-struct Row { long long page; int at; bool ok; };
+// ---- write and read ----------------------------------------------------------------------------------------------------
+// A wave takes the up to 16 tokens of one block of the cache, for a head: their keys or their values to write them (its
+// arithmetic bounds the write: more, shorter waves), both to read them (the loads' latency bounds the read).  Lane (u, g) =
+// (lane % 16, lane / 16) has the unit u (D/16 values) of the tokens 4 g .. 4 g + 3.  A token's values are then 16 lanes'
+// consecutive pieces, its smallest and largest value are found within a DPP row, and four tokens' codes of a unit are
+// consecutive bytes of the values' layout.  All loads of a wave are on their way before the first is used.
+struct Block {
+    uint32_t b, h;
+    int t0, n;                          // t0: the call's token at the block's first place (may be negative)
+    int kv;                             // write: keys or values
+    const uint8_t* base;                // the head's bytes in the page; null: not in the cache
+    uint32_t at;                        // the block's first place in the page
+};
+typedef __attribute__((address_space(4))) int Const;    // lengths, tables: no kernel writes them, so scalar loads will do
 
-// position pos of sequence b: its page and place, ok if it is inside the cache
-static __device__ __forceinline__ Row locate(const KvArgs& a, int b, long long pos) {
-    Row r;
-    const bool in = pos >= 0 && pos < a.capacity;
-    const uint32_t p = in ? (uint32_t)pos : 0u, slot = div_by(p, a.page_inv);
-    r.at = (int)(p - slot * (uint32_t)a.page);
-    r.page = a.table ? (long long)a.table[(long long)b * a.table_stride + slot] : (long long)b;
-    r.ok = in && r.page >= 0 && r.page < a.pages;
-    return r;
+template <bool WRITE> static __device__ __forceinline__ bool block_of(const KvArgs& a, Block& k) {
+    long long w = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (w >= a.rows) return false;
+    k.kv = WRITE ? (int)(w & 1) : 0;
+    if (WRITE) w >>= 1;
+    const uint32_t x = (uint32_t)w, y = div_by(x, a.heads_inv);
+    k.h = x - y * a.heads;
+    k.b = div_by(y, a.tokens_inv);                          // (the inverse of the blocks per sequence)
+    const int blk = (int)(y - k.b * a.blocks), first = ((const Const*)a.start)[k.b];
+    k.n = a.lens ? min(max(((const Const*)a.lens)[k.b], 0), a.tokens) : a.tokens;
+    const long long p0 = (long long)(first & ~15) + 16ll * blk;
+    k.t0 = 16 * blk - (first & 15);
+    k.base = nullptr;
+    k.at = 0;
+    if (p0 >= 0 && p0 < a.capacity) {
+        const uint32_t slot = div_by((uint32_t)p0, a.page_inv);
+        k.at = (uint32_t)p0 - slot * a.page;
+        const int page = a.table ? ((const Const*)a.table)[(long long)k.b * a.table_stride + slot] : (int)k.b;
+        if (page >= 0 && page < a.pages) k.base = a.data + ((long long)page * a.heads + k.h) * a.head_bytes;
+    }
+    return true;
 }
 
-// ---- write -----------------------------------------------------------------------------------------------------------
-// 16 lanes per row, each with the D/16 consecutive values whose codes are one unit of the layout; min and max over the
-// row's lanes, then the codes.  One read of the input, one write of the codes: HBM bound for long inputs, launch bound
-// for single tokens.
 template <class E, int D, int BITS, bool VEC> __global__ __launch_bounds__(256) void kv_write(KvArgs a) {
     constexpr int N = D / 16, U = N * BITS / 8, ROW = 16 * U;
     constexpr int BYTES = N * (int)sizeof(typename E::T);
     constexpr int AL = VEC ? (BYTES & -BYTES) : (int)sizeof(typename E::T);
-    const long long row = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
-    const int c = threadIdx.x & 15;
-    if (row >= a.rows) return;                              // (a whole row's lanes leave together)
-    const int kv = (int)(row & 1);
-    const uint32_t th = (uint32_t)(row >> 1), bt = div_by(th, a.heads_inv), h = th - bt * a.heads;
-    const uint32_t b = div_by(bt, a.tokens_inv), t = bt - b * a.tokens;
-    if (a.lens && (int)t >= a.lens[b]) return;
-    const Row r = locate(a, (int)b, (long long)a.start[b] + t);
-    if (!r.ok) {
-        if (c == 0) atomicOr(a.status, 1u);
+    constexpr int CODES = (1 << BITS) - 1;
+    Block k;
+    if (!block_of<true>(a, k)) return;
+    const int u = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3, t = k.t0 + 4 * g;
+    bool on[4], all = true, any = false;
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        on[r] = t + r >= 0 && t + r < k.n;
+        all &= on[r];
+        any |= on[r];
+    }
+    if (!k.base) {
+        if (any && u == 0) atomicOr(a.status, 1u);
         return;
     }
-    const typename E::T* src = kv ? (const typename E::T*)a.v + b * a.vs[0] + t * a.vs[1] + h * a.vs[2]
-                                  : (const typename E::T*)a.k + b * a.ks[0] + t * a.ks[1] + h * a.ks[2];
-    alignas(16) typename E::T raw[N];
-    load_n<typename E::T, N, AL>(src + c * N, raw);
-    float x[N], lo, hi;
-    uint32_t top = 0;
+    const typename E::T* src = (k.kv ? (const typename E::T*)a.v + k.b * a.vs[0] + k.h * a.vs[2]
+                                     : (const typename E::T*)a.k + k.b * a.ks[0] + k.h * a.ks[2]) + u * N;
+    const long long stride = k.kv ? a.vs[1] : a.ks[1];
+    alignas(16) typename E::T raw[4][N];
+    if (!all) {
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        x[i] = E::to(raw[i]);
-        lo = i ? fminf(lo, x[i]) : x[i];
-        hi = i ? fmaxf(hi, x[i]) : x[i];
-        top = max(top, asu(x[i]) & 0x7FFFFFFFu);
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int i = 0; i < N; i++) raw[r][i] = E::from(0.0f);
     }
-    const unsigned long long odd = __ballot(top >= 0x7F800000u);
-    const bool bad = (odd >> (threadIdx.x & 48)) & 0xFFFFull;
-    lo = min16(lo);
-    hi = max16(hi);
-    constexpr float CODES = (float)((1 << BITS) - 1);
-    const float half_span = 0.5f * hi - 0.5f * lo;
-    float s = fmaxf(step_up(half_span, 2.0f / CODES, 0.5f * CODES), step_up(fmaxf(hi, -lo), 1.0f / 32512.0f, 32512.0f));
-    s = fmaxf(s, 7.888609052210118e-31f);                   // 2^-100
-    const float inv = __builtin_amdgcn_rcpf(s), half = 0.5f * s;
-    const float z = rint_div(lo, s, inv, half);
-    alignas(16) uint8_t out[U];
 #pragma unroll
-    for (int i = 0; i < N; i += 8 / BITS) {
-        uint32_t q = 0;
-        for (int j = 0; j < 8 / BITS; j++) {
-            const float f = fminf(fmaxf(rint_div(x[i + j], s, inv, half) - z, 0.0f), CODES);
-            q |= (uint32_t)(int)f << (j * BITS);
+    for (int r = 0; r < 4; r++)
+        if (on[r]) load_n<typename E::T, N, AL>(src + (t + r) * stride, raw[r]);
+    const int kv = k.kv;
+    alignas(16) uint8_t out[4][U];
+    alignas(16) uint32_t word[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        if (!__any(on[r])) continue;                    // (single tokens: one of the four)
+        float x[N], lo, hi;
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] = E::to(raw[r][i]);
+        lo = hi = x[0];
+#pragma unroll
+        for (int i = 1; i < N; i++) {
+            lo = least(lo, x[i]);
+            hi = most(hi, x[i]);
         }
-        out[i * BITS / 8] = bad ? (uint8_t)0 : (uint8_t)q;
+        lo = min16(lo);
+        hi = max16(hi);
+        const bool bad = !(most(fabsf(lo), fabsf(hi)) < INFINITY);
+        const float half_span = 0.5f * hi - 0.5f * lo;
+        const float s = step_up(half_span, 2.0f / (float)CODES, 0.5f * (float)CODES, fmaxf(hi, -lo), 1.0f / 32512.0f, 32512.0f);
+        const float inv = __builtin_amdgcn_rcpf(s), half = 0.5f * s;
+        const float z = rint_div(lo, s, inv, half);
+#pragma unroll
+        for (int i = 0; i < N; i += 8 / BITS) {
+            uint32_t q = 0;
+#pragma unroll
+            for (int j = 0; j < 8 / BITS; j++)
+                q |= (uint32_t)__builtin_amdgcn_fmed3f(rint_div(x[i + j], s, inv, half) - z, 0.0f, (float)CODES) << (j * BITS);
+            out[r][i * BITS / 8] = bad ? (uint8_t)0 : (uint8_t)q;
+        }
+        word[r] = bad ? 0x7FC0u : (asu(s) >> 16) | ((uint32_t)(int)z << 16);
     }
-    uint8_t* base = a.data + (r.page * a.heads + h) * a.head_bytes;
-    uint8_t* dst = kv ? base + (long long)a.page * ROW + (r.at >> 4) * (16 * ROW) + c * (16 * U) + (r.at & 15) * U
-                      : base + (long long)r.at * ROW + c * U;
-    store_n<uint8_t, U, (U & -U)>(dst, out);
-    if (c == 0) {
-        const uint32_t w = bad ? 0x7FC0u : (asu(s) >> 16) | ((uint32_t)(int)z << 16);
-        *(uint32_t*)(base + 2ll * a.page * ROW + (kv ? 4ll * a.page : 0) + 4ll * r.at) = w;
-    }
+    uint8_t* codes = (uint8_t*)k.base + (kv ? (long long)a.page * ROW : 0) + (long long)k.at * ROW;
+    uint32_t* words = (uint32_t*)((uint8_t*)k.base + 2ll * a.page * ROW + (kv ? 4ll * a.page : 0)) + k.at + 4 * g;
+    if (all) {
+        if (kv) store_n<uint8_t, 4 * U, (4 * U & -(4 * U))>(codes + u * (16 * U) + g * (4 * U), out[0]);
+        else
+#pragma unroll
+            for (int r = 0; r < 4; r++) store_n<uint8_t, U, (U & -U)>(codes + (4 * g + r) * ROW + u * U, out[r]);
+        if (u == 0) *(uint4*)words = *(const uint4*)word;
+    } else
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            if (on[r]) {
+                store_n<uint8_t, U, (U & -U)>(codes + (kv ? u * (16 * U) + (4 * g + r) * U : (4 * g + r) * ROW + u * U), out[r]);
+                if (u == 0) words[r] = word[r];
+            }
 }
 
-// ---- read ------------------------------------------------------------------------------------------------------------
 template <class E, int D, int BITS, bool VEC> __global__ __launch_bounds__(256) void kv_read(KvArgs a) {
     constexpr int N = D / 16, U = N * BITS / 8, ROW = 16 * U;
     constexpr int BYTES = N * (int)sizeof(typename E::T);
     constexpr int AL = VEC ? (BYTES & -BYTES) : (int)sizeof(typename E::T);
-    const long long row = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
-    const int c = threadIdx.x & 15;
-    if (row >= a.rows) return;
-    const int kv = (int)(row & 1);
-    const uint32_t th = (uint32_t)(row >> 1), bt = div_by(th, a.heads_inv), h = th - bt * a.heads;
-    const uint32_t b = div_by(bt, a.tokens_inv), t = bt - b * a.tokens;
-    const bool pad = a.lens && (int)t >= a.lens[b];
-    if (pad && !a.zero_padding) return;
-    Row r = {};
-    if (!pad) r = locate(a, (int)b, (long long)a.start[b] + t);
-    typename E::T* dst = kv ? (typename E::T*)a.v + b * a.vs[0] + t * a.vs[1] + h * a.vs[2]
-                            : (typename E::T*)a.k + b * a.ks[0] + t * a.ks[1] + h * a.ks[2];
-    alignas(16) typename E::T out[N];
-    if (r.ok) {
-        const uint8_t* base = a.data + (r.page * a.heads + h) * a.head_bytes;
-        const uint8_t* src = kv ? base + (long long)a.page * ROW + (r.at >> 4) * (16 * ROW) + c * (16 * U) + (r.at & 15) * U
-                                : base + (long long)r.at * ROW + c * U;
-        alignas(16) uint8_t in[U];
-        load_n<uint8_t, U, (U & -U)>(src, in);
-        const uint32_t w = *(const uint32_t*)(base + 2ll * a.page * ROW + (kv ? 4ll * a.page : 0) + 4ll * r.at);
-        const float s = asf(w << 16);
-        const int z = (int)w >> 16;
+    Block k;
+    if (!block_of<false>(a, k)) return;
+    const int u = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3, t = k.t0 + 4 * g, end = a.zero_padding ? a.tokens : k.n;
+    if (k.t0 >= end) return;
+    typename E::T* dst[2] = {(typename E::T*)a.k + k.b * a.ks[0] + k.h * a.ks[2] + u * N,
+                             (typename E::T*)a.v + k.b * a.vs[0] + k.h * a.vs[2] + u * N};
+    alignas(16) uint8_t in[2][4][U];
+    alignas(16) uint32_t word[2][4];
+    if (k.base) {
+        const uint8_t* codes = k.base + (long long)k.at * ROW;
+        const uint8_t* words = k.base + 2ll * a.page * ROW + 4ll * (k.at + 4 * g);
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            const int code = BITS == 8 ? in[i] : (in[i / 2] >> ((i & 1) * 4)) & 15;
-            const float x = s * (float)(z + code);
-            out[i] = E::from(x != x ? x : fminf(fmaxf(x, -E::MOST), E::MOST));
-        }
+        for (int r = 0; r < 4; r++) load_n<uint8_t, U, (U & -U)>(codes + (4 * g + r) * ROW + u * U, in[0][r]);
+        load_n<uint8_t, 4 * U, (4 * U & -(4 * U))>(codes + (long long)a.page * ROW + u * (16 * U) + g * (4 * U), in[1][0]);
+        *(uint4*)word[0] = *(const uint4*)words;
+        *(uint4*)word[1] = *(const uint4*)(words + 4ll * a.page);
     } else {
-        if (!pad && c == 0) atomicOr(a.status, 1u);
+        if (t + 3 >= 0 && t < k.n && u == 0) atomicOr(a.status, 1u);
 #pragma unroll
-        for (int i = 0; i < N; i++) out[i] = E::from(pad ? 0.0f : asf(0x7FC00000u));
+        for (int i = 0; i < 8; i++) {
+            word[i >> 2][i & 3] = 0x7FC0u;                  // NaN
+            for (int j = 0; j < U; j++) in[i >> 2][i & 3][j] = 0;
+        }
     }
-    store_n<typename E::T, N, AL>(dst + c * N, out);
+#pragma unroll
+    for (int kv = 0; kv < 2; kv++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            if (t + r < 0 || t + r >= end) continue;
+            const bool pad = t + r >= k.n;
+            const float s = pad ? 0.0f : asf(word[kv][r] << 16), z = pad ? 0.0f : (float)((int)word[kv][r] >> 16), zs = s * z;
+            const float most = s != s ? s : E::MOST;        // (the median of three NaNs is NaN)
+            const bool far = fabsf(zs) > 1e38f;             // s z alone may pass the largest number: in halves
+            const float s1 = far ? 0.5f * s : s, zs1 = far ? 0.5f * s * z : zs, twice = far ? 2.0f : 1.0f;
+            alignas(16) typename E::T out[N];
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const uint32_t byte = in[kv][r][i * BITS / 8], code = BITS == 8 ? byte : (i & 1) ? byte >> 4 : byte & 15;
+                float x = fmaf((float)code, s1, zs1);       // (s z and s code are exact, and so is their sum)
+                x *= twice;
+                out[i] = E::from(__builtin_amdgcn_fmed3f(x, -most, most));
+            }
+            store_n<typename E::T, N, AL>(dst[kv] + (t + r) * (kv ? a.vs[1] : a.ks[1]), out);
+        }
 }
 
 // ---- attention ---------------------------------------------------------------------------------------------------------
@@ -267,9 +335,6 @@ static __device__ __forceinline__ float over_groups_sum(float x) {
     auto q = __builtin_amdgcn_permlane16_swap((int)asu(x), (int)asu(x), false, false);
     return asf((uint32_t)q[0]) + asf((uint32_t)q[1]);
 }
-
-// lengths and tables: the kernel writes none, so they are read by scalar loads
-typedef __attribute__((address_space(4))) int Const;
 
 union Frag { h8 v; uint32_t u[4]; };
 
@@ -810,7 +875,7 @@ template <int D> __global__ __launch_bounds__(256) void kv_join(KvArgs a) {
 }
 
 template <class E, int BITS, bool VEC> int go_rows(const KvArgs& a, bool write, hipStream_t st) {
-    const unsigned grid = (unsigned)((a.rows + 15) / 16);
+    const unsigned grid = (unsigned)((a.rows + 3) / 4);
 #define DC_ROWS(D) \
     case D: \
         if (write) kv_write<E, D, BITS, VEC><<<grid, 256, 0, st>>>(a); \

@@ -120,7 +120,8 @@ typedef struct KvArgs {
     long long ks[3], vs[3];
     int zero_padding;              /* outputs behind lens[b]: 0 (1) or left as they are */
     int dtype, vec, vec_out;       /* vec: pointers and strides allow whole-lane accesses */
-    long long rows;                /* write / read: batch * tokens * heads * 2 */
+    int blocks;                    /* write / read: blocks of 16 places that a sequence's tokens can touch */
+    long long rows;                /* waves: batch * blocks * heads, write: twice (keys, values) */
     unsigned* status;
     int group, causal;             /* attention: query heads per head of the cache */
     float scale;
