@@ -31,37 +31,50 @@ template <> struct Elem<DC_F32> { typedef float T; typedef f8 V; static constexp
 template <> struct Elem<DC_F16> { typedef _Float16 T; typedef h8 V; static constexpr float MOST = 65504.0f; };
 template <> struct Elem<DC_BF16> { typedef __bf16 T; typedef b8 V; static constexpr float MOST = 3.38953139e38f; };
 
-// e^x for x <= 0 (or any x whose result is not large): 2^(x log2 e); WIDE: with the product's low part, for f32 results
-template <bool WIDE> static __device__ __forceinline__ float exp_of(float x) {
-    const float hi = x * 1.44269504088896340736f;
-    if constexpr (!WIDE) return __builtin_amdgcn_exp2f(hi);
-    const float lo = fmaf(x, 1.44269504088896340736f, -hi) + x * 1.925963033500e-8f;
-    const float e = __builtin_amdgcn_exp2f(hi);
-    return fabsf(lo) < 1.0f ? fmaf(e, lo * 0.69314718055994530942f, e) : e;      // (x infinite: lo is NaN)
-}
+// 1 / x and e^x by the hardware's instructions; WIDE (f32 results): with the rounding error of the exponent's argument
 static __device__ __forceinline__ float over(float x) { return __builtin_amdgcn_rcpf(x); }
+template <bool WIDE> static __device__ __forceinline__ float exp_of(float x) {                  // e^x
+    const float hi = x * 1.44269504088896340736f, e = __builtin_amdgcn_exp2f(hi);
+    if constexpr (!WIDE) return e;
+    const float lo = fmaf(x, 1.44269504088896340736f, -hi) + x * 1.925963033500e-8f;
+    return fabsf(lo) < 1.0f ? fmaf(e, lo * 0.69314718055994530942f, e) : e;                     // (x infinite: lo is NaN)
+}
 
 // silu: f = x sigma, f' = sigma (1 + x (1 - sigma))
-// gelu: f = x Phi(x), f' = Phi(x) + x phi(x).  With t = 1 / (1 + |x| / sqrt 8) the upper tail is
-// Phi(-|x|) = e^(-x^2/2) t p(t), p of degree 8 fitted to it (relative error below 5e-8 for every x).
+// gelu: f = x Phi(x), f' = Phi(x) + x phi(x).  With t = 1 / (1 + c |x|) the upper tail is Phi(-|x|) = e^(-x^2/2) t p(t), p a
+// polynomial fitted to it, for f32 of degree 8 (relative error below 5e-8 for every x), for 16 bits of degree 5 (8e-6: the
+// forward pass is bound by its arithmetic, not by HBM, with the longer one).
 template <int KIND, bool WIDE> static __device__ __forceinline__ void value_slope(float x, float& f, float& df) {
     if constexpr (KIND == DC_ACT_SILU) {
         const float e = exp_of<WIDE>(-x), s = over(1.0f + e);
         f = x * s;
         df = fmaf(f, 1.0f - s, s);                          // (x sigma (1 - sigma): finite wherever f is)
     } else {
-        const float a = fabsf(x), t = over(fmaf(a, 0.35355339059327376f, 1.0f));
-        float p = -0.02969324142f;
-        p = fmaf(p, t, 0.1430620308f);
-        p = fmaf(p, t, -0.2452032745f);
-        p = fmaf(p, t, 0.1408667302f);
-        p = fmaf(p, t, -0.01457431771f);
-        p = fmaf(p, t, 0.1018762813f);
-        p = fmaf(p, t, 0.1214175596f);
-        p = fmaf(p, t, 0.1412060496f);
-        p = fmaf(p, t, 0.1410421657f);
-        const float e = exp_of<WIDE>(-0.5f * x * x), q = p * t * e;
-        const float phi = x < 0.0f ? q : 1.0f - q;
+        const float a = fabsf(x);
+        float t, p, e;
+        if constexpr (WIDE) {
+            t = over(fmaf(a, 0.35355339059327376f, 1.0f));
+            p = -0.02969324142f;
+            p = fmaf(p, t, 0.1430620308f);
+            p = fmaf(p, t, -0.2452032745f);
+            p = fmaf(p, t, 0.1408667302f);
+            p = fmaf(p, t, -0.01457431771f);
+            p = fmaf(p, t, 0.1018762813f);
+            p = fmaf(p, t, 0.1214175596f);
+            p = fmaf(p, t, 0.1412060496f);
+            p = fmaf(p, t, 0.1410421657f);
+            e = exp_of<true>(-0.5f * x * x);
+        } else {
+            t = over(fmaf(a, 0.30935921676911454f, 1.0f));
+            p = -0.0724743027f;
+            p = fmaf(p, t, 0.177926669f);
+            p = fmaf(p, t, 0.0188289209f);
+            p = fmaf(p, t, 0.131555132f);
+            p = fmaf(p, t, 0.120597981f);
+            p = fmaf(p, t, 0.123569132f);
+            e = __builtin_amdgcn_exp2f(x * (x * -0.72134752044448170368f));
+        }
+        const float q = p * t * e, phi = x < 0.0f ? q : 1.0f - q;
         f = x * phi;
         df = fmaf(x, e * 0.39894228040143267794f, phi);
     }
@@ -120,34 +133,33 @@ template <int CTRL> static __device__ __forceinline__ uint32_t quad(uint32_t x) 
 }
 // the lane's 8 codes and, from the quad's first lane, the group's step (lanes behind the last value take part with zeros)
 static __device__ __forceinline__ void keep8(const ActArgs& a, long long i, f8 x, uint8_t* kept) {
-    uint32_t big = 0, top = 0;
+    float top = 0.0f;                                       // (NaN if a value is)
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const uint32_t u = asu(x[j]) & 0x7FFFFFFFu;
-        top = max(top, u);
-    }
-    const bool odd = top >= 0x7F800000u;
+    for (int j = 0; j < 8; j++) top = __builtin_elementwise_maximum(top, fabsf(x[j]));
+    const bool odd = !(top < INFINITY);
     if (odd) {
-        for (int j = 0; j < 8; j++) {
-            const uint32_t u = asu(x[j]) & 0x7FFFFFFFu;
-            if (u < 0x7F800000u) big = max(big, u);
-        }
-    } else big = top;
+        top = 0.0f;
+        for (int j = 0; j < 8; j++) top = fabsf(x[j]) < INFINITY ? fmaxf(top, fabsf(x[j])) : top;
+    }
+    uint32_t big = asu(top);
     big = max(big, quad<0xB1>(big));
     big = max(big, quad<0x4E>(big));
     // 127.5 = 255/256 * 2^7: k = exponent - 6, one more where the significand is above 255/128
     int k = (int)(big >> 23) - 127 - 6 + ((big & 0x7FFFFFu) > 0x7F0000u ? 1 : 0);
     k = max(k, -126);
     const float down = asf((uint32_t)(127 - k) << 23);
-    uint32_t w[2] = {0, 0};
+    uint32_t w[2];
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const float r = __builtin_amdgcn_fmed3f(rintf(x[j] * down), -127.0f, 127.0f);
-        w[j >> 2] |= ((uint32_t)(int)r & 0xFFu) << (8 * (j & 3));
+    for (int h = 0; h < 2; h++) {
+        uint32_t c[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++)                         // 1.5 * 2^23 added: rounded, and the code in the low byte
+            c[j] = asu(__builtin_amdgcn_fmed3f(fmaf(x[4 * h + j], down, 12582912.0f), 12582912.0f - 127.0f, 12582912.0f + 127.0f));
+        w[h] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(c[3], c[2], 0x00000400u), __builtin_amdgcn_perm(c[1], c[0], 0x00000400u), 0x05040100u);
     }
     if (odd) {
         for (int j = 0; j < 8; j++)
-            if ((asu(x[j]) & 0x7FFFFFFFu) >= 0x7F800000u) w[j >> 2] = (w[j >> 2] & ~(0xFFu << (8 * (j & 3)))) | 0x80u << (8 * (j & 3));
+            if (!(fabsf(x[j]) < INFINITY)) w[j >> 2] = (w[j >> 2] & ~(0xFFu << (8 * (j & 3)))) | 0x80u << (8 * (j & 3));
     }
     if (i < a.groups * 32) {
         *(uint2*)(kept + i) = make_uint2(w[0], w[1]);

@@ -51,10 +51,12 @@ def f_df(x, kind):
 
 
 def near(got, want, dt, scale):
-    """Half a unit of the type, and 24 units of f32 (the functions' arithmetic: a dozen roundings, an exponential and a
-    reciprocal of one unit each, a fit of 5e-8) of `scale`, the magnitude of the terms that are added."""
+    """Half a unit of the type, and of `scale`, the magnitude of the terms that are added, 24 units of f32 (the functions'
+    arithmetic: a dozen roundings, an exponential and a reciprocal of one unit each, a fit of 5e-8), for 16-bit types 2^-15
+    (a fit of 8e-6, an exponent's argument rounded at up to 2^-24 of 100)."""
     got, want = got.cpu().double(), want
-    tol = torch.finfo(dt).eps / 2 * want.abs() * (1 + 2.0 ** -10) + 24 * 2.0 ** -24 * scale + torch.finfo(dt).smallest_normal * torch.finfo(dt).eps
+    arith = 24 * 2.0 ** -24 if dt == torch.float32 else 2.0 ** -15
+    tol = torch.finfo(dt).eps / 2 * want.abs() * (1 + 2.0 ** -10) + arith * scale + torch.finfo(dt).smallest_normal * torch.finfo(dt).eps
     ok = (got - want).abs() <= tol
     return bool(ok.all()), float(((got - want).abs() / tol).max())
 
