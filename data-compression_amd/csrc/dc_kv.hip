@@ -99,7 +99,15 @@ static __device__ __forceinline__ uint32_t div_by(uint32_t n, unsigned long long
     return m ? (uint32_t)__umul64hi((unsigned long long)n, m) : n;
 }
 
-// the row's lanes are 16 neighbours: rotations within a DPP row
+// lane T of the row's 16
+template <int T> static __device__ __forceinline__ float row_lane(float x) {
+    return asf((uint32_t)__builtin_amdgcn_update_dpp(0, (int)asu(x), 0x150 + T, 0xF, 0xF, true));
+}
+template <int... I, class F> static __device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F f) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+
+// rotations within a DPP row
 template <int N> static __device__ __forceinline__ float ror16(float x) {
     return asf((uint32_t)__builtin_amdgcn_update_dpp(0, (int)asu(x), 0x120 + N, 0xF, 0xF, false));
 }
@@ -201,53 +209,58 @@ template <class E, int D, int BITS, bool VEC> __global__ __launch_bounds__(256) 
 #pragma unroll
     for (int r = 0; r < 4; r++)
         if (on[r]) load_n<typename E::T, N, AL>(src + (t + r) * stride, raw[r]);
-    const int kv = k.kv;
-    alignas(16) uint8_t out[4][U];
-    alignas(16) uint32_t word[4];
+    // the four rows' smallest and largest values; then their steps and zero points, row u % 4 by lane u for all
+    float x[4][N], lo[4], hi[4];
 #pragma unroll
     for (int r = 0; r < 4; r++) {
-        if (!__any(on[r])) continue;                    // (single tokens: one of the four)
-        float x[N], lo, hi;
+        lo[r] = hi[r] = 0.0f;
+        if (!__any(on[r])) continue;                        // (single tokens: one of the four)
 #pragma unroll
-        for (int i = 0; i < N; i++) x[i] = E::to(raw[r][i]);
-        lo = hi = x[0];
+        for (int i = 0; i < N; i++) x[r][i] = E::to(raw[r][i]);
+        lo[r] = hi[r] = x[r][0];
 #pragma unroll
         for (int i = 1; i < N; i++) {
-            lo = least(lo, x[i]);
-            hi = most(hi, x[i]);
+            lo[r] = least(lo[r], x[r][i]);
+            hi[r] = most(hi[r], x[r][i]);
         }
-        lo = min16(lo);
-        hi = max16(hi);
-        const bool bad = !(most(fabsf(lo), fabsf(hi)) < INFINITY);
-        const float half_span = 0.5f * hi - 0.5f * lo;
-        const float s = step_up(half_span, 2.0f / (float)CODES, 0.5f * (float)CODES, fmaxf(hi, -lo), 1.0f / 32512.0f, 32512.0f);
-        const float inv = __builtin_amdgcn_rcpf(s), half = 0.5f * s;
-        const float z = rint_div(lo, s, inv, half);
+        lo[r] = min16(lo[r]);
+        hi[r] = max16(hi[r]);
+    }
+    const int own = u & 3;
+    const float l = own & 2 ? (own & 1 ? lo[3] : lo[2]) : own & 1 ? lo[1] : lo[0];
+    const float h = own & 2 ? (own & 1 ? hi[3] : hi[2]) : own & 1 ? hi[1] : hi[0];
+    const float s = step_up(0.5f * h - 0.5f * l, 2.0f / (float)CODES, 0.5f * (float)CODES, fmaxf(h, -l), 1.0f / 32512.0f, 32512.0f);
+    float inv = __builtin_amdgcn_rcpf(s), z = rint_div(l, s, inv, 0.5f * s);
+    uint32_t word = (asu(s) >> 16) | ((uint32_t)(int)z << 16);
+    if (!(most(fabsf(l), fabsf(h)) < INFINITY)) {           // a value that is not finite: a step of NaN, codes of 0
+        inv = z = 0.0f;
+        word = 0x7FC0u;
+    }
+    uint8_t* codes = (uint8_t*)k.base + (k.kv ? (long long)a.page * ROW : 0) + (long long)k.at * ROW;
+    uint32_t* words = (uint32_t*)((uint8_t*)k.base + 2ll * a.page * ROW + (k.kv ? 4ll * a.page : 0)) + k.at + 4 * g;
+    if (u < 4 && t + u >= 0 && t + u < k.n) words[u] = word;
+    alignas(16) uint8_t out[4][U];
+    each_of(std::make_integer_sequence<int, 4>{}, [&](auto I) {
+        constexpr int r = I.value;
+        if (!__any(on[r])) return;
+        const float sr = row_lane<r>(s), ir = row_lane<r>(inv), zr = row_lane<r>(z), half = 0.5f * sr;
 #pragma unroll
         for (int i = 0; i < N; i += 8 / BITS) {
             uint32_t q = 0;
 #pragma unroll
             for (int j = 0; j < 8 / BITS; j++)
-                q |= (uint32_t)__builtin_amdgcn_fmed3f(rint_div(x[i + j], s, inv, half) - z, 0.0f, (float)CODES) << (j * BITS);
-            out[r][i * BITS / 8] = bad ? (uint8_t)0 : (uint8_t)q;
+                q |= (uint32_t)__builtin_amdgcn_fmed3f(rint_div(x[r][i + j], sr, ir, half) - zr, 0.0f, (float)CODES) << (j * BITS);
+            out[r][i * BITS / 8] = (uint8_t)q;
         }
-        word[r] = bad ? 0x7FC0u : (asu(s) >> 16) | ((uint32_t)(int)z << 16);
-    }
-    uint8_t* codes = (uint8_t*)k.base + (kv ? (long long)a.page * ROW : 0) + (long long)k.at * ROW;
-    uint32_t* words = (uint32_t*)((uint8_t*)k.base + 2ll * a.page * ROW + (kv ? 4ll * a.page : 0)) + k.at + 4 * g;
+        if (!all && on[r])
+            store_n<uint8_t, U, (U & -U)>(codes + (k.kv ? u * (16 * U) + (4 * g + r) * U : (4 * g + r) * ROW + u * U), out[r]);
+    });
     if (all) {
-        if (kv) store_n<uint8_t, 4 * U, (4 * U & -(4 * U))>(codes + u * (16 * U) + g * (4 * U), out[0]);
+        if (k.kv) store_n<uint8_t, 4 * U, (4 * U & -(4 * U))>(codes + u * (16 * U) + g * (4 * U), out[0]);
         else
 #pragma unroll
             for (int r = 0; r < 4; r++) store_n<uint8_t, U, (U & -U)>(codes + (4 * g + r) * ROW + u * U, out[r]);
-        if (u == 0) *(uint4*)words = *(const uint4*)word;
-    } else
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-            if (on[r]) {
-                store_n<uint8_t, U, (U & -U)>(codes + (kv ? u * (16 * U) + (4 * g + r) * U : (4 * g + r) * ROW + u * U), out[r]);
-                if (u == 0) words[r] = word[r];
-            }
+    }
 }
 
 template <class E, int D, int BITS, bool VEC> __global__ __launch_bounds__(256) void kv_read(KvArgs a) {
@@ -365,14 +378,6 @@ static __device__ __forceinline__ uint32_t pair16(const uint32_t* w, int oa, int
 template <int BITS> static __device__ __forceinline__ constexpr int key_order(int e) {
     if constexpr (BITS == 4) return (e >> 1) + 4 * (e & 1);
     else return (e & 4) + ((e >> 1) & 1) + 2 * (e & 1);
-}
-
-// lane T of the row's 16
-template <int T> static __device__ __forceinline__ float row_lane(float x) {
-    return asf((uint32_t)__builtin_amdgcn_update_dpp(0, (int)asu(x), 0x150 + T, 0xF, 0xF, true));
-}
-template <int... I, class F> static __device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F f) {
-    (f(std::integral_constant<int, I>{}), ...);
 }
 
 template <int U> struct Stage {         // what a lane holds of 32 tokens: 2 blocks of 16
