@@ -94,6 +94,13 @@ template <class T, int N, int A> static __device__ __forceinline__ void store_n(
     }
 }
 
+// the same past the caches, 16 bytes at a time
+template <class T, int N> static __device__ __forceinline__ void store_past(T* p, const T* x) {
+    static_assert(N * (int)sizeof(T) % 16 == 0, "whole pieces");
+#pragma unroll
+    for (int i = 0; i < N * (int)sizeof(T) / 16; i++) __builtin_nontemporal_store(((const u4*)x)[i], (u4*)p + i);
+}
+
 // n / d by the host's reciprocal m = floor(2^64 / d) + 1 (d = 1: m = 0): exact for n d < 2^64
 static __device__ __forceinline__ uint32_t div_by(uint32_t n, unsigned long long m) {
     return m ? (uint32_t)__umul64hi((unsigned long long)n, m) : n;
@@ -263,7 +270,8 @@ template <class E, int D, int BITS, bool VEC> __global__ __launch_bounds__(256) 
     }
 }
 
-template <class E, int D, int BITS, bool VEC> __global__ __launch_bounds__(256) void kv_read(KvArgs a) {
+// PAST: the output passes the caches
+template <class E, int D, int BITS, bool VEC, bool PAST> __global__ __launch_bounds__(256) void kv_read(KvArgs a) {
     constexpr int N = D / 16, U = N * BITS / 8, ROW = 16 * U;
     constexpr int BYTES = N * (int)sizeof(typename E::T);
     constexpr int AL = VEC ? (BYTES & -BYTES) : (int)sizeof(typename E::T);
@@ -309,7 +317,9 @@ template <class E, int D, int BITS, bool VEC> __global__ __launch_bounds__(256) 
                 x *= twice;
                 out[i] = E::from(__builtin_amdgcn_fmed3f(x, -most, most));
             }
-            store_n<typename E::T, N, AL>(dst[kv] + (t + r) * (kv ? a.vs[1] : a.ks[1]), out);
+            typename E::T* to = dst[kv] + (t + r) * (kv ? a.vs[1] : a.ks[1]);
+            if constexpr (PAST && VEC && BYTES % 16 == 0) store_past<typename E::T, N>(to, out);
+            else store_n<typename E::T, N, AL>(to, out);
         }
 }
 
@@ -884,7 +894,8 @@ template <class E, int BITS, bool VEC> int go_rows(const KvArgs& a, bool write, 
 #define DC_ROWS(D) \
     case D: \
         if (write) kv_write<E, D, BITS, VEC><<<grid, 256, 0, st>>>(a); \
-        else kv_read<E, D, BITS, VEC><<<grid, 256, 0, st>>>(a); \
+        else if (VEC && a.past) kv_read<E, D, BITS, VEC, VEC><<<grid, 256, 0, st>>>(a); \
+        else kv_read<E, D, BITS, VEC, false><<<grid, 256, 0, st>>>(a); \
         break
     switch (a.dim) {
         DC_ROWS(32); DC_ROWS(64); DC_ROWS(96); DC_ROWS(128); DC_ROWS(160); DC_ROWS(192); DC_ROWS(224); DC_ROWS(256);

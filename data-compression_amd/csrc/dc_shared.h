@@ -118,6 +118,7 @@ typedef struct KvArgs {
     const void* k;                 /* write: keys, read: keys out, attention: queries; strides (batch, token, head) in elements */
     const void* v;                 /* write: values, read: values out, attention: the output */
     long long ks[3], vs[3];
+    int past;                      /* read: the output passes the caches */
     int zero_padding;              /* outputs behind lens[b]: 0 (1) or left as they are */
     int dtype, vec, vec_out;       /* vec: pointers and strides allow whole-lane accesses */
     int blocks;                    /* write / read: blocks of 16 places that a sequence's tokens can touch */
@@ -134,6 +135,7 @@ typedef struct KvArgs {
 /* activation checkpoints (dc_act.hip) */
 typedef struct ActArgs {
     int kind, gated, dtype, mode;  /* mode: 0 flat, 1 rows apart in whole 8s, 2 any */
+    int past;                      /* the outputs pass the caches */
     long long n, rows, cols, groups;
     unsigned long long cols8_inv;  /* reciprocal of cols / 8 (mode 1) */
     const void *x, *up;            /* forward: inputs; backward: x is the output's gradient */
