@@ -197,6 +197,7 @@ int dc_abi_status(void) { return G.abi_rc; }
 void dc_abi_set_status(int rc) { G.abi_rc = rc; }      /* the double ABI (dc_host64.c) reports through it too */
 int dc_set_error(int code, const char* msg) { return seterr(code, "%s", msg); }
 unsigned* dc_kv_status_word(void) { return G.d_kv_status; }   /* (dc_host_lowbit.c) */
+int dc_get_device(void) { return G.inited ? G.device : -1; }
 void* dc_get_stream(void) { return (void*)G.st; }
 void dc_set_abs_error_bound(double bound) { absErrBound = bound; absErrorBound_binary = -100; }
 double dc_get_abs_error_bound(void) { return absErrBound; }

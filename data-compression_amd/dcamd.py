@@ -52,7 +52,7 @@ EXT_SYMBOLS = [
     "dc_last_decode_launched_runs", "dc_last_decode_used_maps", "dc_med_last_wide", "dc_set_decode3_maps", "dc_set_halo_async", "dc_med_shard_stats", "dc_med_shard_trans",
     "dc_med_shard_binades",
     "dc_kv_page_bytes", "dc_kv_write_device", "dc_kv_read_device", "dc_kv_attention_workspace", "dc_kv_attention_device",
-    "dc_kv_status", "dc_act_bytes", "dc_act_forward_device", "dc_act_backward_device",
+    "dc_kv_status", "dc_get_device", "dc_act_bytes", "dc_act_forward_device", "dc_act_backward_device",
 ]
 
 
@@ -198,8 +198,7 @@ class Lib:
         rc = self.L.dc_init(device)
         if rc:
             raise DCError(f"dc_init: {rc} {self.err()}")
-        if self.device is None:
-            self.device = device
+        self.device = self.L.dc_get_device()       # (the first call's, whatever this one asks for)
 
     def err(self):
         m = self.L.dc_last_error()
@@ -1328,13 +1327,15 @@ class KVCache:
                 return KvBatchDesc(batch, tokens, start.data_ptr(), n, table.data_ptr(), shape[1], max(stride, shape[1]), pad)
         raise ValueError(f"table: int32 of ({batch}, pages of a sequence) with consecutive entries is needed")
 
-    def _rows(self, x, name, heads):
+    def _rows(self, x, name, heads, out=False):
         shape = x.shape
         if len(shape) != 4 or shape[3] != self.head_dim or (heads and shape[2] != heads):
             raise ValueError(f"{name}: (batch, tokens, {heads or 'heads'}, {self.head_dim}) is needed")
         a, b, c, one = x.stride()
         if one != 1 and x.numel():
             raise ValueError(f"{name}: a head's values must be consecutive")
+        if out and not (a and b and c) and x.numel() > x.shape[3]:
+            raise ValueError(f"{name}: rows must not lie on one another")
         return _Strides(a, b, c)
 
     def write(self, k, v, start, table=None, lens=None):
@@ -1364,7 +1365,7 @@ class KVCache:
             ks = vs = _Strides(*k.stride()[:3])
         else:
             k, v = out
-            ks, vs = self._rows(k, "out", self.heads), self._rows(v, "out", self.heads)
+            ks, vs = self._rows(k, "out", self.heads, True), self._rows(v, "out", self.heads, True)
             if k.shape != v.shape or k.dtype is not v.dtype or k.shape[:2] != (batch, tokens) or (dtype and k.dtype is not dtype):
                 raise ValueError("out: two tensors (batch, tokens, heads, head_dim) of the type asked for are needed")
             code = _dtype_code(k.dtype)
@@ -1401,7 +1402,7 @@ class KVCache:
             out = T.empty_like(q, memory_format=T.contiguous_format)
             os_ = _Strides(*out.stride()[:3])
         else:
-            os_ = self._rows(out, "out", 0)
+            os_ = self._rows(out, "out", 0, True)
             if out.shape != q.shape or out.dtype is not q.dtype:
                 raise ValueError("out: q's shape and type are needed")
             L, stream = _on_gpu(self.buffer, q, context, table, lens, lse, out)

@@ -29,6 +29,7 @@ enum {
 /* ---- library state ---------------------------------------------------------------------- */
 int dc_init(int device);                       /* optional; first call of any entry point inits dev 0 */
 const char* dc_last_error(void);
+int dc_get_device(void);                       /* the device the library runs on; -1 before the first call */
 void* dc_get_stream(void);                     /* hipStream_t all library work is ordered on */
 int dc_synchronize(void);
 /* Encoder launches of dc_encode_device go to this hipStream_t (NULL: dc_get_stream()); each such encode
@@ -298,7 +299,8 @@ typedef struct dc_kv_cache {
 } dc_kv_cache;
 /* Which positions of which sequences (device arrays of 32-bit integers): sequence b has lens[b] (NULL: `tokens`) tokens
  * in this call, the first at position start[b]; position p is in page table[b * table_stride + p / page_size] (table
- * NULL: page b is sequence b's only one).  table_width: entries per sequence.  Rows from lens[b] on are padding: inputs
+ * NULL: page b is sequence b's only one).  table_width: entries per sequence.  Rows from lens[b] (held to 0 .. tokens) on
+ * are padding: inputs
  * there are not read, outputs are left as they are (zero_padding 0) or set to 0 (1; the lse is left).  Attention:
  * start[b] is the number of positions of sequence b, its lens[b] query tokens being the last of them. */
 typedef struct dc_kv_batch {
@@ -326,7 +328,7 @@ int dc_kv_read_device(const dc_kv_cache* cache, const dc_kv_batch* at, int dtype
  * [batch][tokens][q_heads], may be NULL) receives the log of the softmax's sum.  max_context: no start[b] is expected above it (it
  * sizes the split along the cache; a longer one is still computed in full).  d_workspace: dc_kv_attention_workspace
  * bytes (16-byte aligned; NULL where that is 0), in use until the call's work is done: calls that may run at once need
- * one each.  Outputs must not overlap the inputs. */
+ * one each.  Outputs must not overlap the inputs.  Scores are formed in f32 from queries and steps below 2^100. */
 size_t dc_kv_attention_workspace(const dc_kv_cache* cache, int batch, int tokens, int q_heads, long long max_context);
 int dc_kv_attention_device(const dc_kv_cache* cache, const dc_kv_batch* at, int dtype, int q_heads, const void* d_q,
                            const long long* q_strides, float scale, int causal, long long max_context, void* d_out,

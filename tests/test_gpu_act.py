@@ -192,6 +192,23 @@ def test_rows_through_the_c_api(act):
         assert same(dx[:, :cols], act.act_backward(x, c, "silu")) and bool((dx[:, cols:] == -5).all())
 
 
+@pytest.mark.parametrize("halves", [False, True])
+def test_large(act, halves):
+    """Outputs that are written past the caches (over 128 MB) as the same in parts."""
+    rows, cols = 9001, 8000
+    h = torch.randn(rows, 2 * cols, device=DEV).bfloat16()
+    x, up = (h[:, :cols], h[:, cols:]) if halves else (h[:, :cols].contiguous(), h[:, cols:].contiguous())
+    y, c = act.act_forward(x, "gelu", up=up)
+    parts = [act.act_forward(x[i:i + 1000], "gelu", up=up[i:i + 1000]) for i in range(0, rows, 1000)]
+    assert same(y, torch.cat([p[0] for p in parts]))
+    g = act.act_backward(y, c, "gelu", recompute=True)
+    for k, i in enumerate(range(0, rows, 1000)):
+        for a, b in zip(g, act.act_backward(y[i:i + 1000], parts[k][1], "gelu", recompute=True)):
+            assert same(a[i:i + 1000], b)
+    for a, b in zip(c.load(), zip(*[p[1].load() for p in parts])):
+        assert same(a, torch.cat(b))
+
+
 def test_empty(act):
     for shape in ((0,), (0, 8), (8, 0)):
         x = torch.empty(shape, device=DEV)

@@ -367,6 +367,19 @@ def test_attention_split(kv, dtype):
     check(f, q, [9000], lens=[4])
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dim", [32, 96, 128, 160, 224, 256])
+def test_attention_split_ragged(kv, bits, dim):
+    """One long sequence among short and empty ones: pieces by the whole batch's length, joined; some have one piece."""
+    f = Filled(kv, 7 + dim, 4, 3000, 2, dim, 16, bits)
+    q = torch.randn(4, 1, 6, dim, generator=gen(dim)).half()
+    check(f, q, [3000, 3, 0, 700])
+    check(f, q, [1, 2999, 2500, 2400])
+    q = torch.randn(4, 7, 6, dim, generator=gen(dim)).bfloat16()          # several tiles of rows, padded
+    got = check(f, q, [3000, 3, 1200, 900], lens=[7, 7, 0, 2])
+    assert bool((got[1, :4] == 0).all()) and bool((got[2] == 0).all())
+
+
 def test_attention_steps_of_all_sizes(kv):
     """Values whose steps lie far apart: the largest weight times step sets the scale, not the largest weight."""
     f = Filled(kv, 11, 1, 400, 1, 64, 16, 4, kind=("plain", "wide"), dtype=torch.float32)
@@ -530,6 +543,21 @@ def test_repeatable(kv):
     q = torch.randn(1, 1, 16, 128, device=DEV).bfloat16()
     a = f.cache.attention(q, i32(5000), table=f.table)
     assert all(same(f.cache.attention(q, i32(5000), table=f.table), a) for _ in range(5))
+
+
+def test_large_read(kv):
+    """An output that is written past the caches (over 128 MB) as the same in parts."""
+    H, D, P, n = 16, 128, 64, 18000
+    c = make(kv, -(-n // P), P, H, D, 8)
+    table = torch.arange(-(-n // P), dtype=torch.int32, device=DEV).flip(0)[None]
+    k, v = (torch.randn(1, n, H, D, device=DEV) for _ in range(2))
+    c.write(k, v, i32(0), table=table)
+    a = c.read(i32(0), n, table=table, dtype=torch.float32)
+    for first in (0, 7000, 14001):
+        m = min(7000, n - first)
+        b = c.read(i32(first), m, table=table, dtype=torch.float32)
+        assert same(a[0][:, first:first + m], b[0]) and same(a[1][:, first:first + m], b[1])
+    assert same(a[0][:, :50], held(k[:, :50].cpu(), 8)[0].float())
 
 
 def test_far_pages(kv):

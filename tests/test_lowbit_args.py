@@ -102,6 +102,11 @@ def test_activation_calls(lib):
     assert forward(rows=0) == 0 and backward(cols=0) == 0
 
 
+def test_device(lib):
+    import torch as t
+    assert lib.L.dc_get_device() == -1 or t.cuda.is_available()
+
+
 def test_status_needs_a_place(lib):
     assert lib.L.dc_kv_status(None, None, 0) == ARG
 
@@ -131,10 +136,12 @@ def test_tensor_calls(d):
                      ((k.transpose(1, 3).contiguous().transpose(1, 3), k, s), {}), ((k, k, s), {})):      # (the last: not on the GPU)
         with pytest.raises(ValueError):
             c.write(*args, **kw)
-    for kw in (dict(out=(k, k[:, :2])), dict(out=(k, k.half())), dict(out=(k, k), dtype=torch.float16), dict(dtype=torch.int8)):
+    flat = torch.zeros(2, 3, 1, 64).expand(2, 3, 2, 64)
+    for kw in (dict(out=(k, k[:, :2])), dict(out=(k, k.half())), dict(out=(k, flat)), dict(out=(k, k), dtype=torch.float16), dict(dtype=torch.int8)):
         with pytest.raises(ValueError):
             c.read(s, 3, **kw)
     for args, kw in (((q[:, :, :3], s), {}), ((q.float(), s), {}), ((q, s), dict(out=q[:1])), ((q, s), dict(out=q.bfloat16())),
+                     ((q, s), dict(out=flat.half().repeat(1, 1, 2, 1)[:, :1].expand(2, 3, 4, 64))),
                      ((q, s), dict(lse=torch.zeros(2, 3, 3))), ((q, s), dict(lse=torch.zeros(2, 3, 4).half())), ((q, s), dict(max_context=-1)),
                      ((q, s), {})):
         with pytest.raises(ValueError):
