@@ -70,7 +70,7 @@ class KvCacheDesc(C.Structure):     # dc_kv_cache
                 ("head_dim", C.c_int), ("bits", C.c_int)]
 
 
-class KvBatchDesc(C.Structure):     # dc_kv_batch
+class KvBatchDesc(C.Structure):     # dc_kv_batch (for callers of the C entry points)
     _fields_ = [("batch", C.c_int), ("tokens", C.c_int), ("start", C.c_void_p), ("lens", C.c_void_p),
                 ("table", C.c_void_p), ("table_width", C.c_int), ("table_stride", C.c_longlong), ("zero_padding", C.c_int)]
 
@@ -1230,48 +1230,37 @@ def lib():
 
 
 # ---- floats held in 8 or 4 bits in HBM: torch tensors on the current stream ------------------------------------------
-# (Single tokens are bound by the host's side of a call, about 3 us of which are the launch's: torch is looked up once,
-# types are compared by identity, strides and streams are asked for in one call each.)
-DC_F32, DC_F16, DC_BF16 = 0, 1, 2
+# (the checks and launches are in csrc/dc_torch.cpp)
 ACT_KINDS = {"silu": 1, "gelu": 2}
-_Strides = C.c_longlong * 3
+_native = None
 _torch = None
 _codes = {}
 
 
-def _need_torch():
-    global _torch
-    if _torch is None:
+def native():
+    """The extension that takes torch tensors (lib/dcamd_torch.so)."""
+    global _native, _torch
+    if _native is None:
+        import importlib.machinery
+        import importlib.util
         import torch
-        _torch = torch
-        _codes.update({torch.float32: DC_F32, torch.float16: DC_F16, torch.bfloat16: DC_BF16})
-    return _torch
+        lib()                                               # (the extension uses the library that is loaded)
+        path = os.path.join(HERE, "lib", "dcamd_torch.so")
+        if not os.path.exists(path):
+            raise ImportError(f"dcamd_torch.so not built ({path}); run `make -C data-compression_amd torch`")
+        loader = importlib.machinery.ExtensionFileLoader("dcamd_torch", path)
+        m = importlib.util.module_from_spec(importlib.util.spec_from_file_location("dcamd_torch", path, loader=loader))
+        m.set_error(DCError)
+        _codes.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+        _torch, _native = torch, m
+    return _native
 
 
 def _dtype_code(dtype):
-    _need_torch()
     code = _codes.get(dtype)
     if code is None:
         raise ValueError(f"dtype {dtype}: f32, f16 or bf16 is needed")
     return code
-
-
-def _on_gpu(*tensors):
-    """The library and torch's current stream, after checking that all tensors lie on the library's device and that it
-    is the current one (a caller with several devices says `with torch.cuda.device(...)`)."""
-    T = _need_torch()
-    L = _lib or lib()
-    if L.device is None:
-        if not tensors[0].is_cuda:
-            raise ValueError("tensors must lie on the GPU")
-        L.init(tensors[0].get_device())
-    dev = L.device
-    for t in tensors:
-        if t is not None and t.get_device() != dev:
-            raise ValueError(f"tensors must lie on the library's device (cuda:{dev})")
-    if T._C._cuda_getDevice() != dev:
-        raise ValueError(f"the current device must be the library's (cuda:{dev})")
-    return L, T._C._cuda_getCurrentRawStream(dev)
 
 
 class KVCache:
@@ -1285,19 +1274,20 @@ class KVCache:
     captured into a graph."""
 
     def __init__(self, pages, page_size, heads, head_dim, bits=4, buffer=None, device="cuda"):
-        T = _need_torch()
+        self._native = native()
         page = self.page_bytes(page_size, heads, head_dim, bits)
         if pages < 1:
             raise ValueError("a cache has at least one page")
         if buffer is None:
-            buffer = T.zeros(pages * page, dtype=T.uint8, device=device)
-        if buffer.dtype is not T.uint8 or not buffer.is_contiguous() or buffer.numel() < pages * page:
+            buffer = _torch.zeros(pages * page, dtype=_torch.uint8, device=device)
+        if buffer.dtype is not _torch.uint8 or not buffer.is_contiguous() or buffer.numel() < pages * page:
             raise ValueError(f"buffer: {pages * page} contiguous bytes (uint8) are needed")
         if buffer.data_ptr() % 16:
             raise ValueError("buffer: 16-byte alignment is needed")
         self.pages, self.page_size, self.heads, self.head_dim, self.bits = pages, page_size, heads, head_dim, bits
         self.buffer = buffer
         self._desc = KvCacheDesc(buffer.data_ptr(), pages, page_size, heads, head_dim, bits)
+        self._at = C.addressof(self._desc)
 
     @staticmethod
     def page_bytes(page_size, heads, head_dim, bits=4):
@@ -1307,73 +1297,17 @@ class KVCache:
             raise ValueError("page_size is a multiple of 16, head_dim a multiple of 32 up to 256, bits 4 or 8")
         return n
 
-    def _batch(self, batch, tokens, start, table, lens, pad, what="start"):
-        i32 = _torch.int32
-        if start.dtype is not i32 or start.shape != (batch,) or not start.is_contiguous():
-            raise ValueError(f"{what}: contiguous int32 of ({batch},) is needed")
-        n = None
-        if lens is not None:
-            if lens.dtype is not i32 or lens.shape != (batch,) or not lens.is_contiguous():
-                raise ValueError(f"lens: contiguous int32 of ({batch},) is needed")
-            n = lens.data_ptr()
-        if table is None:
-            if batch > self.pages:
-                raise ValueError("without a table each sequence has a page")
-            return KvBatchDesc(batch, tokens, start.data_ptr(), n, None, 0, 0, pad)
-        shape = table.shape
-        if table.dtype is i32 and len(shape) == 2 and shape[0] == batch and shape[1] >= 1:
-            stride, one = table.stride()
-            if one == 1 and (batch <= 1 or stride >= shape[1]):
-                return KvBatchDesc(batch, tokens, start.data_ptr(), n, table.data_ptr(), shape[1], max(stride, shape[1]), pad)
-        raise ValueError(f"table: int32 of ({batch}, pages of a sequence) with consecutive entries is needed")
-
-    def _rows(self, x, name, heads, out=False):
-        shape = x.shape
-        if len(shape) != 4 or shape[3] != self.head_dim or (heads and shape[2] != heads):
-            raise ValueError(f"{name}: (batch, tokens, {heads or 'heads'}, {self.head_dim}) is needed")
-        a, b, c, one = x.stride()
-        if one != 1 and x.numel():
-            raise ValueError(f"{name}: a head's values must be consecutive")
-        if out and not (a and b and c) and x.numel() > x.shape[3]:
-            raise ValueError(f"{name}: rows must not lie on one another")
-        return _Strides(a, b, c)
-
     def write(self, k, v, start, table=None, lens=None):
         """Quantise k, v (batch, tokens, heads, head_dim) to positions start[b] .. of each sequence."""
-        ks, vs = self._rows(k, "k", self.heads), self._rows(v, "v", self.heads)
-        shape = k.shape
-        if shape != v.shape or k.dtype is not v.dtype:
-            raise ValueError("k and v differ in shape or type")
-        code = _dtype_code(k.dtype)
-        at = self._batch(shape[0], shape[1], start, table, lens, 0)
-        L, stream = _on_gpu(self.buffer, k, v, start, table, lens)
-        rc = L.L.dc_kv_write_device(self._desc, at, code, k.data_ptr(), ks, v.data_ptr(), vs, stream)
-        if rc:
-            L.check(rc, "kv_write")
+        self._native.kv_write(self._at, self.buffer, k, v, start, table, lens)
 
     def read(self, start, tokens, table=None, lens=None, dtype=None, out=None):
         """The keys and values of positions start[b] .. start[b] + tokens as floats of `dtype` (bf16), in `out` if given
         (rows of padding keep what they have), else in new tensors (padding is 0)."""
-        T = _torch
-        batch = start.shape[0] if start.dim() else 0
-        at = self._batch(batch, tokens, start, table, lens, out is None)
         if out is None:
-            code = _dtype_code(dtype or T.bfloat16)
-            L, stream = _on_gpu(self.buffer, start, table, lens)
-            k = T.empty((batch, tokens, self.heads, self.head_dim), dtype=dtype or T.bfloat16, device=self.buffer.device)
-            v = T.empty_like(k)
-            ks = vs = _Strides(*k.stride()[:3])
-        else:
-            k, v = out
-            ks, vs = self._rows(k, "out", self.heads, True), self._rows(v, "out", self.heads, True)
-            if k.shape != v.shape or k.dtype is not v.dtype or k.shape[:2] != (batch, tokens) or (dtype and k.dtype is not dtype):
-                raise ValueError("out: two tensors (batch, tokens, heads, head_dim) of the type asked for are needed")
-            code = _dtype_code(k.dtype)
-            L, stream = _on_gpu(self.buffer, start, table, lens, k, v)
-        rc = L.L.dc_kv_read_device(self._desc, at, code, k.data_ptr(), ks, v.data_ptr(), vs, stream)
-        if rc:
-            L.check(rc, "kv_read")
-        return k, v
+            return self._native.kv_read(self._at, self.buffer, start, tokens, table, lens, 2 if dtype is None else _dtype_code(dtype),
+                                        None, None)
+        return self._native.kv_read(self._at, self.buffer, start, tokens, table, lens, -1 if dtype is None else _dtype_code(dtype), *out)
 
     def attention(self, q, context, table=None, lens=None, scale=None, causal=True, max_context=None, out=None, lse=None):
         """softmax(scale q k^T) v over the first context[b] positions of each sequence, q (batch, tokens, q_heads, head_dim)
@@ -1381,69 +1315,18 @@ class KVCache:
         them.  scale: 1 / sqrt(head_dim).  max_context: the longest context expected (the table's capacity).  out: where
         to put the output (rows of padding keep what they have; in a new tensor they are 0); lse: an f32 tensor (batch,
         tokens, q_heads) for the log of each softmax's sum."""
-        T = _torch
-        qs = self._rows(q, "q", 0)
-        code = _dtype_code(q.dtype)
-        if code == DC_F32:
-            raise ValueError("q: f16 or bf16 is needed")
-        batch, tokens, q_heads, _ = q.shape
-        if q_heads < 1 or q_heads % self.heads:
-            raise ValueError(f"q: heads in a multiple of the cache's {self.heads} are needed")
-        at = self._batch(batch, tokens, context, table, lens, out is None, "context")
-        limit = self.page_size * (1 if table is None else at.table_width)
-        if max_context is not None:
-            if max_context < 0:
-                raise ValueError("max_context is not negative")
-            limit = min(int(max_context), limit)
-        if lse is not None and (lse.dtype is not T.float32 or lse.shape != q.shape[:3] or not lse.is_contiguous()):
-            raise ValueError("lse: contiguous float32 of (batch, tokens, q_heads) is needed")
-        if out is None:
-            L, stream = _on_gpu(self.buffer, q, context, table, lens, lse)
-            out = T.empty_like(q, memory_format=T.contiguous_format)
-            os_ = _Strides(*out.stride()[:3])
-        else:
-            os_ = self._rows(out, "out", 0, True)
-            if out.shape != q.shape or out.dtype is not q.dtype:
-                raise ValueError("out: q's shape and type are needed")
-            L, stream = _on_gpu(self.buffer, q, context, table, lens, lse, out)
-        need = L.L.dc_kv_attention_workspace(self._desc, batch, tokens, q_heads, limit)
-        space = T.empty(need, dtype=T.uint8, device=q.device) if need else None
-        rc = L.L.dc_kv_attention_device(self._desc, at, code, q_heads, q.data_ptr(), qs,
-                                        self.head_dim ** -0.5 if scale is None else scale, bool(causal), limit, out.data_ptr(),
-                                        os_, lse.data_ptr() if lse is not None else None,
-                                        space.data_ptr() if need else None, need, stream)
-        if rc:
-            L.check(rc, "kv_attention")
-        return out
+        if max_context is None:
+            max_context = -1
+        elif max_context < 0:
+            raise ValueError("max_context is not negative")
+        return self._native.kv_attention(self._at, self.buffer, q, context, table, lens, self.head_dim ** -0.5 if scale is None else scale,
+                                         causal, max_context, out, lse)
 
     @staticmethod
     def status(reset=False):
         """The sticky status word after the work queued on the current stream (synchronous): 1, a position or page outside
         its cache (then dropped, read as NaN or left out)."""
-        L, v = lib(), C.c_uint(0)
-        L.check(L.L.dc_kv_status(_need_torch().cuda.current_stream().cuda_stream, C.byref(v), int(bool(reset))), "kv_status")
-        return int(v.value)
-
-
-def _flat(x):
-    """x as rows of its last dimension: (tensor, rows, cols, elements between rows); copied if its rows do not lie so."""
-    if x.is_contiguous():                                   # one row
-        n = x.numel()
-        return x, 1, n, n
-    cols = x.shape[-1]
-    y = x.reshape(x.numel() // cols, cols)
-    if y.stride(1) != 1 or y.stride(0) < cols:
-        y = y.contiguous()
-    return y, y.shape[0], cols, max(y.stride(0), cols)
-
-
-def _same_rows(a, b):
-    """Two _flat()s with one's rows and cols: an array in one row takes the other's."""
-    if a[1] == 1 and b[1] > 1:
-        return (a[0], b[1], b[2], b[2]), b
-    if b[1] == 1 and a[1] > 1:
-        return a, (b[0], a[1], a[2], a[2])
-    return a, b
+        return native().kv_status(reset)
 
 
 class ActCheckpoint:
@@ -1451,28 +1334,18 @@ class ActCheckpoint:
     the shape each)."""
 
     def __init__(self, shape, dtype, kept, kept_up=None):
-        T = _need_torch()
-        self.shape, self.dtype, self.kept, self.kept_up = T.Size(shape), dtype, kept, kept_up
-        need = lib().L.dc_act_bytes(self.shape.numel())
-        for t in (kept, kept_up):
-            if t is not None and (t.dtype is not T.uint8 or not t.is_contiguous() or t.numel() < need):
-                raise ValueError(f"checkpoint: {need} contiguous bytes (uint8) are needed")
+        native()
+        self.shape, self.dtype, self.kept, self.kept_up = _torch.Size(shape), dtype, kept, kept_up
         _dtype_code(dtype)
+        need = (self.shape.numel() + 31) // 32 * 33
+        for t in (kept, kept_up):
+            if t is not None and (t.dtype is not _torch.uint8 or not t.is_contiguous() or t.numel() < need):
+                raise ValueError(f"checkpoint: {need} contiguous bytes (uint8) are needed")
 
     def load(self):
         """The kept values as floats: a tuple of one tensor, or two of a gated activation."""
-        got, code, n = [], _dtype_code(self.dtype), self.shape.numel()
-        for kept in (self.kept, self.kept_up):
-            if kept is None:
-                continue
-            L, stream = _on_gpu(kept)
-            x = _torch.empty(self.shape, dtype=self.dtype, device=kept.device)
-            rc = L.L.dc_act_backward_device(0, code, 1, n, None, 0, kept.data_ptr(), None, x.data_ptr(), n, None, 0, None, 0,
-                                            stream)
-            if rc:
-                L.check(rc, "act_load")
-            got.append(x)
-        return tuple(got)
+        code = _dtype_code(self.dtype)
+        return tuple(_native.act_load(t, code, *self.shape) for t in (self.kept, self.kept_up) if t is not None)
 
 
 def _act_kind(kind):
@@ -1484,67 +1357,22 @@ def _act_kind(kind):
 
 def act_save(x):
     """x (f32, f16, bf16) as an ActCheckpoint."""
-    code = _dtype_code(x.dtype)
-    L, stream = _on_gpu(x)
-    x2, rows, cols, ld = _flat(x)
-    T = _torch
-    kept = T.empty(L.L.dc_act_bytes(x.numel()), dtype=T.uint8, device=x.device)
-    rc = L.L.dc_act_forward_device(0, code, rows, cols, x2.data_ptr(), ld, None, 0, None, 0, kept.data_ptr(), None, stream)
-    if rc:
-        L.check(rc, "act_save")
-    return ActCheckpoint(x.shape, x.dtype, kept)
+    return ActCheckpoint(x.shape, x.dtype, native().act_forward(x, 0, None)[1])
 
 
 def act_forward(x, kind, up=None):
     """y = f(x) (kind 'silu' or 'gelu', the exact one) or f(x) * up, and the ActCheckpoint of x (and up), in one pass."""
-    code, k = _dtype_code(x.dtype), _act_kind(kind)
-    T = _torch
-    if up is not None and (up.shape != x.shape or up.dtype is not x.dtype):
-        raise ValueError("x and up differ in shape or type")
-    L, stream = _on_gpu(x, up)
-    fx = _flat(x)
-    y = T.empty_like(x, memory_format=T.contiguous_format)
-    n = L.L.dc_act_bytes(x.numel())
-    kept = T.empty(n, dtype=T.uint8, device=x.device)
-    if up is None:
-        x2, rows, cols, ldx = fx
-        rc = L.L.dc_act_forward_device(k, code, rows, cols, x2.data_ptr(), ldx, None, 0, y.data_ptr(), cols, kept.data_ptr(), None,
-                                       stream)
-        kept_up = None
-    else:
-        kept_up = T.empty_like(kept)
-        (x2, rows, cols, ldx), (u2, _, _, ldu) = _same_rows(fx, _flat(up))
-        rc = L.L.dc_act_forward_device(k, code, rows, cols, x2.data_ptr(), ldx, u2.data_ptr(), ldu, y.data_ptr(), cols,
-                                       kept.data_ptr(), kept_up.data_ptr(), stream)
-    if rc:
-        L.check(rc, "act_forward")
+    y, kept, kept_up = native().act_forward(x, _act_kind(kind), up)
     return y, ActCheckpoint(x.shape, x.dtype, kept, kept_up)
 
 
 def act_backward(dy, checkpoint, kind, recompute=False):
     """The gradient of act_forward at the checkpoint's values: dx, or (dx, dup) of a gated activation; with recompute, a
     tuple that ends with the activation's output at those values (for the gradient of what used it)."""
-    code, k = _dtype_code(dy.dtype), _act_kind(kind)
-    T = _torch
     if dy.shape != checkpoint.shape or dy.dtype is not checkpoint.dtype:
         raise ValueError("dy and the checkpoint differ in shape or type")
-    kept, kept_up = checkpoint.kept, checkpoint.kept_up
-    L, stream = _on_gpu(dy, kept, kept_up)
-    d2, rows, cols, ldd = _flat(dy)
-    dx = T.empty_like(dy, memory_format=T.contiguous_format)
-    got, dup, y = [dx], None, None
-    if kept_up is not None:
-        got.append(T.empty_like(dx))
-        dup = got[-1].data_ptr()
-        kept_up = kept_up.data_ptr()
-    if recompute:
-        got.append(T.empty_like(dx))
-        y = got[-1].data_ptr()
-    rc = L.L.dc_act_backward_device(k, code, rows, cols, d2.data_ptr(), ldd, kept.data_ptr(), kept_up, dx.data_ptr(), cols, dup, cols,
-                                    y, cols, stream)
-    if rc:
-        L.check(rc, "act_backward")
-    return tuple(got) if len(got) > 1 else dx
+    got = native().act_backward(dy, checkpoint.kept, checkpoint.kept_up, _act_kind(kind), recompute)
+    return got if len(got) > 1 else got[0]
 
 
 _activation = None
@@ -1555,9 +1383,9 @@ def activation(x, kind, up=None):
     of its inputs, and its gradient is that at the checkpoint's values.  Not differentiable twice."""
     global _activation
     if _activation is None:
-        T = _need_torch()
+        native()
 
-        class Activation(T.autograd.Function):
+        class Activation(_torch.autograd.Function):
             @staticmethod
             def forward(ctx, x, up, kind):
                 y, c = act_forward(x, kind, up)
@@ -1566,7 +1394,7 @@ def activation(x, kind, up=None):
                 return y
 
             @staticmethod
-            @T.autograd.function.once_differentiable
+            @_torch.autograd.function.once_differentiable
             def backward(ctx, dy):
                 c = ActCheckpoint(ctx.shape, ctx.dtype, *ctx.saved_tensors)
                 got = act_backward(dy, c, ctx.kind)

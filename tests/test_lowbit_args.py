@@ -155,3 +155,31 @@ def test_tensor_calls(d):
               lambda: d.act_backward(x, d.ActCheckpoint((4, 8), torch.float32, torch.zeros(33, dtype=torch.uint8)), "silu")):
         with pytest.raises(ValueError):
             f()
+
+
+def test_tensors_exchanged(d):
+    """What a cache or a checkpoint was made with is looked at again by each call; wrong kinds of arguments are errors."""
+    page = d.KVCache.page_bytes(16, 2, 64, 4)
+    room = torch.zeros(3 * page + 16, dtype=torch.uint8)
+    room = room[-room.data_ptr() % 16:][:3 * page]
+    k, q = torch.zeros(1, 3, 2, 64), torch.zeros(1, 3, 4, 64, dtype=torch.float16)
+    s = torch.zeros(1, dtype=torch.int32)
+    c = d.KVCache(1, 16, 2, 64, buffer=room[:page])
+    c.buffer = room[2 * page:]
+    for f in (lambda: c.write(k, k, s), lambda: c.read(s, 3), lambda: c.attention(q, s)):
+        with pytest.raises(ValueError, match="buffer"):
+            f()
+    a = d.ActCheckpoint((4, 8), torch.float32, torch.zeros(33, dtype=torch.uint8))
+    a.shape = torch.Size((4, 16))
+    for f in (lambda: a.load(), lambda: d.act_backward(torch.zeros(4, 16), a, "silu")):
+        with pytest.raises(ValueError, match="66"):
+            f()
+    c = d.KVCache(1, 16, 2, 64, buffer=room[:page])
+    for f in (lambda: c.write(1, k, s), lambda: c.write(k, None, s), lambda: c.read(s, 2.5), lambda: c.read(s, 3, table=[[0]]),
+              lambda: c.attention(q, s, max_context="all"), lambda: d.act_forward([1.0], "silu")):
+        with pytest.raises((TypeError, AttributeError)):
+            f()
+    for f in (lambda: c.read(s, -1), lambda: c.read(s, 1 << 31), lambda: c.read(s, 3, out=(k,)), lambda: c.attention(q[0], s),
+              lambda: c.write(k, k, torch.zeros((), dtype=torch.int32))):
+        with pytest.raises(ValueError):
+            f()
