@@ -361,8 +361,8 @@ static __device__ __forceinline__ float over_groups_sum(float x) {
 
 union Frag { h8 v; uint32_t u[4]; };
 
-// the codes in both halves of x times 1 / UNIT: 4 bits, four pairs of nibbles 0..3; 8 bits, two of bytes 0..1
 template <int BITS> constexpr float UNIT = BITS == 4 ? 1048576.0f : 16777216.0f;
+// the codes in both halves of x times 1 / UNIT: 4 bits, four pairs of nibbles 0..3; 8 bits, two of bytes 0..1
 template <int BITS> static __device__ __forceinline__ void codes_of(uint32_t x, uint32_t* o) {
     if constexpr (BITS == 4) {
         o[0] = (x << 4) & 0x00F000F0u;
@@ -371,17 +371,12 @@ template <int BITS> static __device__ __forceinline__ void codes_of(uint32_t x, 
         o[3] = (x >> 8) & 0x00F000F0u;
     } else {
         o[0] = x & 0x00FF00FFu;
-        o[1] = (x >> 8) & 0x00FF00FFu;
+        o[1] = __builtin_amdgcn_perm(0, x, 0x0C030C01u);
     }
 }
-// the 16 bits at byte offset o of w[] (offsets are known when this is compiled); those at two offsets, one per half
-static __device__ __forceinline__ uint32_t at16(const uint32_t* w, int o) {
-    return (o & 3) == 3 ? __builtin_amdgcn_alignbyte(w[o / 4 + 1], w[o / 4], 3) : w[o / 4] >> (8 * (o & 3));
-}
-static __device__ __forceinline__ uint32_t pair16(const uint32_t* w, int oa, int ob) {
-    const uint32_t x = oa & 3, y = ob & 3;
-    if (x == 3 || y == 3) return __builtin_amdgcn_perm(at16(w, ob), at16(w, oa), 0x05040100u);
-    return __builtin_amdgcn_perm(w[ob / 4], w[oa / 4], x | (x + 1) << 8 | (y + 4) << 16 | (y + 5) << 24);
+// the bytes at offsets oa and ob of w[] (known when this is compiled), one per half
+static __device__ __forceinline__ uint32_t byte_pair(const uint32_t* w, int oa, int ob) {
+    return __builtin_amdgcn_perm(w[ob / 4], w[oa / 4], (uint32_t)(oa & 3) | 0x0C00u | (uint32_t)((ob & 3) + 4) << 16 | 0x0C000000u);
 }
 
 // the d (within 8) that element e of a key operand holds
@@ -391,7 +386,7 @@ template <int BITS> static __device__ __forceinline__ constexpr int key_order(in
 }
 
 template <int U> struct Stage {         // what a lane holds of 32 tokens: 2 blocks of 16
-    uint32_t k[2][U], v[2][U + 1];      // (one word more: a 16-bit piece may end in it; never used)
+    uint32_t k[2][U], v[2][U];
     uint32_t kw, vw;                    // of token 16 j + 4 g + r, j and r the bits of lane % 8
 };
 // where a step's two blocks lie: the first byte of their keys' codes and of their words (uniform over a wave), and
@@ -448,10 +443,19 @@ static __device__ __forceinline__ void attend(Stage<D * BITS / 128>& c, const Fr
                                               const bool* hole, const Where& next, uint64_t codes_to_values,
                                               uint32_t words_to_values, uint32_t lane_codes, bool second, uint32_t lane_words,
                                               f4 (*acc)[D / 16], float* M, float* L, float* Z, float& R) {
-    constexpr int N = D / 16, U = N * BITS / 8, KS = D / 32, PER = 16 / BITS;
-    f4 s[NT][2];
+    constexpr int N = D / 16, U = N * BITS / 8, KS = D / 32;
+    // the lane's token's words.  (Behind the last position that is seen there may be anything)
+    if (EDGE) {
+        const int at = t0 + (second ? 16 : 0) + (int)(lane_words >> 2);
+        if (at >= most || hole[second]) c.kw = c.vw = 0;
+    }
+    const float ks = asf(c.kw << 16), kz = (float)(int16_t)(c.kw >> 16), vs = asf(c.vw << 16), vz = (float)(int16_t)(c.vw >> 16);
+    f4 s[NT][2];                                            // from z sum(q) on
+    each_of(std::make_integer_sequence<int, 8>{}, [&](auto I) {
+        constexpr int t = I.value;
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) s[nt][0] = s[nt][1] = (f4){0, 0, 0, 0};
+        for (int nt = 0; nt < NT; nt++) s[nt][t >> 2][t & 3] = row_lane<t>(kz) * qsum[nt];
+    });
 #pragma unroll
     for (int st = 0; st < KS; st++)
 #pragma unroll
@@ -463,13 +467,7 @@ static __device__ __forceinline__ void attend(Stage<D * BITS / 128>& c, const Fr
             for (int nt = 0; nt < NT; nt++) s[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k.v, q[nt][st].v, s[nt][j], 0, 0, 0);
         }
     load_keys(c, next, lane_codes);
-    // the lane's token's words.  (Behind the last position that is seen there may be anything)
-    if (EDGE) {
-        const int at = t0 + (second ? 16 : 0) + (int)(lane_words >> 2);
-        if (at >= most || hole[second]) c.kw = c.vw = 0;
-    }
-    const float ks = asf(c.kw << 16), kz = ks * (float)(int16_t)(c.kw >> 16), vs = asf(c.vw << 16), vz = (float)(int16_t)(c.vw >> 16);
-    float ref[NT][8], mx[NT];
+    float ref[NT][8], mx[NT];                               // (in units of 1 / unit: one multiply-add takes a score to its power)
     int left[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
@@ -481,7 +479,7 @@ static __device__ __forceinline__ void attend(Stage<D * BITS / 128>& c, const Fr
         constexpr int t = I.value;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            float y = fmaf(s[nt][t >> 2][t & 3], row_lane<t>(ks) * unit[nt], row_lane<t>(kz) * qsum[nt]);
+            float y = s[nt][t >> 2][t & 3] * row_lane<t>(ks);
             if (EDGE && (t & 3) >= left[nt][t >> 2]) y = -INFINITY;
             ref[nt][t] = y;
             mx[nt] = fmaxf(mx[nt], y);
@@ -490,10 +488,7 @@ static __device__ __forceinline__ void attend(Stage<D * BITS / 128>& c, const Fr
     // a score that passes its maximum by 8, or a step as large as the unit (not a NaN): new references
     bool raise = vs >= R;
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-        mx[nt] = over_groups_max(mx[nt]);
-        raise |= mx[nt] > M[nt] + 8.0f;
-    }
+    for (int nt = 0; nt < NT; nt++) raise |= mx[nt] * unit[nt] > M[nt] + 8.0f;
     if (__any(raise)) {
         float top = vs >= R ? vs : 0.0f;
         for (int k = 32; k; k >>= 1) top = fmaxf(top, __shfl_xor(top, k));
@@ -502,7 +497,8 @@ static __device__ __forceinline__ void attend(Stage<D * BITS / 128>& c, const Fr
         R = r;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            const float m = mx[nt] > M[nt] + 8.0f ? mx[nt] : M[nt], al = __builtin_amdgcn_exp2f(M[nt] - m);
+            const float most = over_groups_max(mx[nt]) * unit[nt];
+            const float m = most > M[nt] + 8.0f ? most : M[nt], al = __builtin_amdgcn_exp2f(M[nt] - m);
             M[nt] = m;
             L[nt] *= al;
             Z[nt] *= al * down;
@@ -512,38 +508,55 @@ static __device__ __forceinline__ void attend(Stage<D * BITS / 128>& c, const Fr
     }
     const float vr = vs * asf(0x7F000000u - asu(R)) * 128.0f;       // 2^7 / R
     Frag w[NT];
-    each_of(std::make_integer_sequence<int, 8>{}, [&](auto I) {
-        constexpr int t = I.value;
+    each_of(std::make_integer_sequence<int, 4>{}, [&](auto I) {
+        constexpr int t = 2 * I.value;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            const float p = __builtin_amdgcn_exp2f(ref[nt][t] - M[nt]);
-            float x = p * row_lane<t>(vr);
-            if (EDGE && (t & 3) >= left[nt][t >> 2]) x = 0.0f;      // (0 times a NaN)
-            const _Float16 wt = (_Float16)x;
-            L[nt] += p;
-            Z[nt] = fmaf((float)wt, row_lane<t>(vz), Z[nt]);
-            w[nt].v[t] = wt;
+            float p[2], x[2];
+#pragma unroll
+            for (int k = 0; k < 2; k++) p[k] = __builtin_amdgcn_exp2f(fmaf(ref[nt][t + k], unit[nt], -M[nt]));
+            if (EDGE) {                                     // (a unit of 0)
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+                    if (((t + k) & 3) >= left[nt][t >> 2]) p[k] = 0.0f;
+            }
+            x[0] = p[0] * row_lane<t>(vr);
+            x[1] = p[1] * row_lane<t + 1>(vr);
+            if (EDGE) {                                     // (0 times a NaN)
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+                    if (((t + k) & 3) >= left[nt][t >> 2]) x[k] = 0.0f;
+            }
+            asm("" : "+v"(x[0]), "+v"(x[1]));               // (or each weight is rounded twice, for either use)
+            uint32_t both = __builtin_bit_cast(uint32_t, (h2){(_Float16)x[0], (_Float16)x[1]});
+            asm("" : "+v"(both));
+            const h2 wt = __builtin_bit_cast(h2, both);
+            L[nt] += p[0] + p[1];
+            Z[nt] = fmaf((float)wt[0], row_lane<t>(vz), Z[nt]);
+            Z[nt] = fmaf((float)wt[1], row_lane<t + 1>(vz), Z[nt]);
+            w[nt].u[t / 2] = both;
         }
     });
     load_words(c, next, words_to_values, second, lane_words);
-    // values: unit lane % 16, tokens 4 g .. 4 g + 3 of both blocks, 16 bits of each token at a time
+    // values: unit lane % 16, tokens 4 g .. 4 g + 3 of both blocks; 4 bits: even and odd codes in bits 4..7 of their bytes
+    constexpr int ODD = BITS == 4;
+    uint32_t v[2][1 + ODD][U];
 #pragma unroll
-    for (int i0 = 0; i0 < N; i0 += PER) {
-        uint32_t got[4][PER];
+    for (int j = 0; j < 2; j++)
+#pragma unroll
+        for (int k = 0; k < U; k++) {
+            v[j][0][k] = ODD ? (c.v[j][k] << 4) & 0xF0F0F0F0u : c.v[j][k];
+            if (ODD) v[j][ODD][k] = c.v[j][k] & 0xF0F0F0F0u;
+        }
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        Frag f;
 #pragma unroll
         for (int j = 0; j < 2; j++)
 #pragma unroll
-            for (int r = 0; r < 2; r++)
-                codes_of<BITS>(pair16(c.v[j], 2 * r * U + i0 * BITS / 8, (2 * r + 1) * U + i0 * BITS / 8), got[2 * j + r]);
+            for (int r = 0; r < 2; r++) f.u[2 * j + r] = byte_pair(v[j][i & ODD], 2 * r * U + i * BITS / 8, (2 * r + 1) * U + i * BITS / 8);
 #pragma unroll
-        for (int i = 0; i < PER && i0 + i < N; i++) {
-            Frag f;
-#pragma unroll
-            for (int k = 0; k < 4; k++) f.u[k] = got[k][i];
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-                acc[nt][i0 + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.v, w[nt].v, acc[nt][i0 + i], 0, 0, 0);
-        }
+        for (int nt = 0; nt < NT; nt++) acc[nt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.v, w[nt].v, acc[nt][i], 0, 0, 0);
     }
     load_values(c, next, codes_to_values, lane_codes);
 }
@@ -618,7 +631,8 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256, NT == 1 && 
     const long long lo64 = (long long)split * chunk;
     const int lo = lo64 < most ? (int)lo64 : most, hi = (int)min((long long)most, lo64 + chunk);
 
-    // queries, as f16 in the keys' order; their sum and the factor that takes a score to log2 units
+    // queries, as f16 in the keys' order; with the scale's sign; their sum and the factor
+    // that takes a score to log2 units
     Frag q[NT][KS];
     float qsum[NT], unit[NT];
 #pragma unroll
@@ -647,7 +661,7 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256, NT == 1 && 
         for (int j = 0; j < D / 4; j++) top = max(top, asu(f[j]) & 0x7FFFFFFFu);
         const float big = over_groups_max(asf(min(top, 0x7F7FFFFFu)));
         const int e = min(268 - (int)(asu(big) >> 23), 253);            // 2^(14 - exponent of the largest)
-        const float up = asf((uint32_t)e << 23), down = asf((uint32_t)(254 - e) << 23);
+        const float up = copysignf(asf((uint32_t)e << 23), a.scale), down = asf((uint32_t)(254 - e) << 23);
         float sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < KS; j++)
@@ -657,9 +671,8 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256, NT == 1 && 
                 q[nt][j].v[k] = v;
                 sum += (float)v;
             }
-        const float u = a.scale * 1.44269504088896340736f * down;
-        qsum[nt] = over_groups_sum(sum) * u;
-        unit[nt] = u * UNIT<BITS>;
+        qsum[nt] = over_groups_sum(sum) * (1.0f / UNIT<BITS>);
+        unit[nt] = fabsf(a.scale) * 1.44269504088896340736f * down * UNIT<BITS>;
     }
 
     f4 acc[NT][N];
