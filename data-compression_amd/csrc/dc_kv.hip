@@ -420,13 +420,18 @@ static __device__ __forceinline__ float log_sum(float m, float l) { return (m + 
 // 1 / l; NaN where it is NaN, or nothing of what a query sees is in the cache
 static __device__ __forceinline__ float inverse_sum(float l) { return l > 0.0f ? 1.0f / l : asf(0x7FC00000u); }
 
-template <int U> static __device__ __forceinline__ void load_keys(Stage<U>& c, const Where& at, uint32_t lane_codes) {
-#pragma unroll
-    for (int j = 0; j < 2; j++) load_n<uint32_t, U, 4 * (U & -U)>((const uint32_t*)(at.codes[j] + lane_codes), c.k[j]);
+// a lane's codes of a block: U words.  PAST (U = 4, an instruction takes whole cache lines): past the caches
+template <int U, bool PAST> static __device__ __forceinline__ void load_codes(const uint8_t* p, uint32_t* x) {
+    if constexpr (PAST) *(u4*)x = __builtin_nontemporal_load((const u4*)p);
+    else load_n<uint32_t, U, 4 * (U & -U)>((const uint32_t*)p, x);
 }
-template <int U> static __device__ __forceinline__ void load_values(Stage<U>& c, const Where& at, uint64_t to_values, uint32_t lane_codes) {
+template <bool PAST, int U> static __device__ __forceinline__ void load_keys(Stage<U>& c, const Where& at, uint32_t lane_codes) {
 #pragma unroll
-    for (int j = 0; j < 2; j++) load_n<uint32_t, U, 4 * (U & -U)>((const uint32_t*)(at.codes[j] + to_values + lane_codes), c.v[j]);
+    for (int j = 0; j < 2; j++) load_codes<U, PAST>(at.codes[j] + lane_codes, c.k[j]);
+}
+template <bool PAST, int U> static __device__ __forceinline__ void load_values(Stage<U>& c, const Where& at, uint64_t to_values, uint32_t lane_codes) {
+#pragma unroll
+    for (int j = 0; j < 2; j++) load_codes<U, PAST>(at.codes[j] + to_values + lane_codes, c.v[j]);
 }
 template <int U> static __device__ __forceinline__ void load_words(Stage<U>& c, const Where& at, uint32_t to_values, bool second, uint32_t lane_words) {
     const uint8_t* p = (second ? at.words[1] : at.words[0]) + lane_words;
@@ -437,7 +442,7 @@ template <int U> static __device__ __forceinline__ void load_words(Stage<U>& c, 
 // One step of a wave: 32 tokens from t0 on against NT tiles of 16 queries.  EDGE: some of them may not be seen.  What the
 // registers of `c` held is replaced by the next step's as soon as it is used, so that those loads are under way during the
 // rest of this step and the beginning of the next.
-template <int D, int BITS, int NT, bool EDGE>
+template <int D, int BITS, int NT, bool PAST, bool EDGE>
 static __device__ __forceinline__ void attend(Stage<D * BITS / 128>& c, const Frag (*q)[D / 32], const float* qsum,
                                               const float* unit, const int* sees, int t0, int most, int g,
                                               const bool* hole, const Where& next, uint64_t codes_to_values,
@@ -466,7 +471,7 @@ static __device__ __forceinline__ void attend(Stage<D * BITS / 128>& c, const Fr
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) s[nt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k.v, q[nt][st].v, s[nt][j], 0, 0, 0);
         }
-    load_keys(c, next, lane_codes);
+    load_keys<PAST>(c, next, lane_codes);
     float ref[NT][8], mx[NT];                               // (in units of 1 / unit: one multiply-add takes a score to its power)
     int left[NT][2];
 #pragma unroll
@@ -558,7 +563,7 @@ static __device__ __forceinline__ void attend(Stage<D * BITS / 128>& c, const Fr
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) acc[nt][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.v, w[nt].v, acc[nt][i], 0, 0, 0);
     }
-    load_values(c, next, codes_to_values, lane_codes);
+    load_values<PAST>(c, next, codes_to_values, lane_codes);
 }
 
 static __device__ __forceinline__ int context_of(const KvArgs& a, uint32_t b) {
@@ -584,7 +589,7 @@ static __device__ __forceinline__ int cut(const KvArgs& a, int context, int& pie
 }
 
 // (codes of up to 64 bytes a row: four waves per SIMD, 88 us against 92 with three at 48 x 8192 positions)
-template <int D, int BITS, int NT> __global__ __launch_bounds__(256, NT == 1 && D * BITS <= 512 ? 4 : 1) void kv_attention(KvArgs a) {
+template <int D, int BITS, int NT, bool PAST> __global__ __launch_bounds__(256, NT == 1 && D * BITS <= 512 ? 4 : 1) void kv_attention(KvArgs a) {
     constexpr int N = D / 16, U = N * BITS / 8, ROW = 16 * U, KS = D / 32, COLS = 16 * NT;
     constexpr bool ALL = D * NT <= 256;                     // every wave its own sums in LDS, or one after the other
     __shared__ float acc_lds[(ALL ? 4 : 1) * N * 16 * COLS];
@@ -722,9 +727,9 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256, NT == 1 && 
     if (first < hi) {
         find(first);
         where(now);
-        load_keys(c, now, lane_codes);
+        load_keys<PAST>(c, now, lane_codes);
         load_words(c, now, words_to_values, second, lane_words);
-        load_values(c, now, codes_to_values, lane_codes);
+        load_values<PAST>(c, now, codes_to_values, lane_codes);
         if (first + 128 < hi) find(first + 128);
     }
     int t0 = first;
@@ -738,7 +743,7 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256, NT == 1 && 
     while (t0 < hi && t0 + 32 <= least && t0 + 32 <= hi && !now.hole[0] && !now.hole[1]) {
         next = now;
         advance();
-        attend<D, BITS, NT, false>(c, q, qsum, unit, sees, t0, most, g, now.hole, next, codes_to_values, words_to_values,
+        attend<D, BITS, NT, PAST, false>(c, q, qsum, unit, sees, t0, most, g, now.hole, next, codes_to_values, words_to_values,
                                    lane_codes, second, lane_words, acc, M, L, Z, R);
         now = next;
         t0 += 128;
@@ -747,7 +752,7 @@ template <int D, int BITS, int NT> __global__ __launch_bounds__(256, NT == 1 && 
         if ((now.hole[0] || now.hole[1]) && lane == 0) atomicOr(a.status, 1u);
         next = now;
         advance();
-        attend<D, BITS, NT, true>(c, q, qsum, unit, sees, t0, most, g, now.hole, next, codes_to_values, words_to_values,
+        attend<D, BITS, NT, PAST, true>(c, q, qsum, unit, sees, t0, most, g, now.hole, next, codes_to_values, words_to_values,
                                   lane_codes, second, lane_words, acc, M, L, Z, R);
         now = next;
         t0 += 128;
@@ -931,9 +936,10 @@ template <int D, int BITS> int go_attention(const KvArgs& a, hipStream_t st) {
     const unsigned grid = (unsigned)((long long)a.splits * a.tiles * a.heads * a.batch);
     constexpr int WIDE = wide_tiles(D);
     if constexpr (WIDE > 1) {
-        if (a.cols == 16) kv_attention<D, BITS, 1><<<grid, 256, 0, st>>>(a);
-        else kv_attention<D, BITS, WIDE><<<grid, 256, 0, st>>>(a);
-    } else kv_attention<D, BITS, 1><<<grid, 256, 0, st>>>(a);
+        if (a.cols > 16) kv_attention<D, BITS, WIDE, false><<<grid, 256, 0, st>>>(a);
+        else if (D * BITS == 512 && a.past) kv_attention<D, BITS, 1, D * BITS == 512><<<grid, 256, 0, st>>>(a);
+        else kv_attention<D, BITS, 1, false><<<grid, 256, 0, st>>>(a);
+    } else kv_attention<D, BITS, 1, false><<<grid, 256, 0, st>>>(a);
     constexpr int ROWS = D <= 128 ? 8 : 4;                  // (kv_join_few)
     if (a.splits > 16) kv_join<D><<<(unsigned)((long long)a.row_slots * a.heads * a.batch * (D / 32)), 256, 0, st>>>(a);
     else if (a.splits > 1)

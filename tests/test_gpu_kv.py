@@ -579,3 +579,22 @@ def test_far_pages(kv):
     f.k, f.ks, f.kz, f.kc = held(torch.cat((z, k.float()), 1), bits)
     f.v, f.vs, f.vz, f.vc = held(torch.cat((z, v.float()), 1), bits)
     check(f, torch.randn(1, 1, H, D, generator=g).bfloat16(), [940])
+
+
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1e-30, 3.0])
+def test_attention_scales(kv, scale):
+    """A scale's sign goes with the queries, and none of what a causal query does not see comes back through a scale of 0."""
+    f = Filled(kv, 90, 2, 200, 2, 64, 16, 8)
+    check(f, torch.randn(2, 1, 4, 64, generator=gen(91)).half(), [200, 33], scale=scale)
+    check(f, torch.randn(2, 19, 4, 64, generator=gen(92)).half(), [150, 19], lens=[19, 7], scale=scale)
+
+
+@pytest.mark.parametrize("bits,dim", [(4, 128), (8, 64), (4, 64)])
+def test_attention_room_for_many(kv, bits, dim):
+    """Tables that allow more than the caches hold (where codes are read past them), of sequences of all lengths."""
+    f = Filled(kv, 93, 3, 900, 2, dim, 16, bits)
+    f.table = torch.cat((f.table, torch.full((3, 40000), -1, dtype=torch.int32, device=DEV)), 1)
+    q = torch.randn(3, 1, 8, dim, generator=gen(94)).bfloat16()
+    for context in ([900, 1, 0], [900, 900, 900], [129, 640, 641]):
+        check(f, q, context)
+    check(f, torch.randn(3, 4, 8, dim, generator=gen(95)).bfloat16(), [900, 3, 77], lens=[4, 3, 2])
