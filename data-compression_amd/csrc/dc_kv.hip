@@ -137,13 +137,13 @@ static __device__ __forceinline__ float step_up(float v, float inv_n, float n, f
     return c;
 }
 
-// rint(x / s) of the exact quotient: an estimate within one, put right by the remainder, which is exact (r s has 24 bits).
-// It is right to move where the remainder is above half a step, or half a step and r odd: above the float before it.
-// (1.5 * 2^23 added to the estimate rounds it, and leaves it as a whole number in the low bits.)
-static __device__ __forceinline__ float rint_div(float x, float s, float inv, float half) {
-    const float y = fmaf(x, inv, 12582912.0f), r = y - 12582912.0f, d = fmaf(-r, s, x);
-    const float far = asf(asu(half) - (asu(y) & 1u));
-    return r + (fabsf(d) > far ? copysignf(1.0f, d) : 0.0f);
+// 1.5 * 2^23 + rint(x / s) of the exact quotient (|x / s| < 2^15), the whole number in the low bits.  The quotient is put
+// right by its remainder, which is exact (s has 8 bits), and rounded as x / s itself would be but for 2^-22 of a unit.  That
+// is half between two whole numbers only if x / s is: these can be told to a bit, and any other x / s is further from one
+// than half a unit, by 2^-8 of it or more (x - s (k + 1/2) is a multiple of x's unit or of half of s's).
+static __device__ __forceinline__ uint32_t rint_div(float x, float s, float inv) {
+    const float q = x * inv;
+    return asu(fmaf(fmaf(-q, s, x), inv, q) + 12582912.0f);
 }
 
 // ---- write and read ----------------------------------------------------------------------------------------------------
@@ -237,12 +237,11 @@ template <class E, int D, int BITS, bool VEC> __global__ __launch_bounds__(256) 
     const float l = own & 2 ? (own & 1 ? lo[3] : lo[2]) : own & 1 ? lo[1] : lo[0];
     const float h = own & 2 ? (own & 1 ? hi[3] : hi[2]) : own & 1 ? hi[1] : hi[0];
     const float s = step_up(0.5f * h - 0.5f * l, 2.0f / (float)CODES, 0.5f * (float)CODES, fmaxf(h, -l), 1.0f / 32512.0f, 32512.0f);
-    float inv = __builtin_amdgcn_rcpf(s), z = rint_div(l, s, inv, 0.5f * s);
-    uint32_t word = (asu(s) >> 16) | ((uint32_t)(int)z << 16);
-    if (!(most(fabsf(l), fabsf(h)) < INFINITY)) {           // a value that is not finite: a step of NaN, codes of 0
-        inv = z = 0.0f;
-        word = 0x7FC0u;
-    }
+    const float inv = __builtin_amdgcn_rcpf(s);
+    const uint32_t z = rint_div(l, s, inv);
+    const bool finite = most(fabsf(l), fabsf(h)) < INFINITY;
+    const uint32_t word = finite ? (asu(s) >> 16) | z << 16 : 0x7FC0u;     // (else a step of NaN, codes of 0)
+    const float top = asf(finite ? CODES : 0);
     uint8_t* codes = (uint8_t*)k.base + (k.kv ? (long long)a.page * ROW : 0) + (long long)k.at * ROW;
     uint32_t* words = (uint32_t*)((uint8_t*)k.base + 2ll * a.page * ROW + (k.kv ? 4ll * a.page : 0)) + k.at + 4 * g;
     if (u < 4 && t + u >= 0 && t + u < k.n) words[u] = word;
@@ -250,13 +249,15 @@ template <class E, int D, int BITS, bool VEC> __global__ __launch_bounds__(256) 
     each_of(std::make_integer_sequence<int, 4>{}, [&](auto I) {
         constexpr int r = I.value;
         if (!__any(on[r])) return;
-        const float sr = row_lane<r>(s), ir = row_lane<r>(inv), zr = row_lane<r>(z), half = 0.5f * sr;
+        const float sr = row_lane<r>(s), ir = row_lane<r>(inv);
+        float zr = row_lane<r>(asf(z)), most = row_lane<r>(top);
+        asm("" : "+v"(zr), "+v"(most));                     // (kept as moves: within v_sub_u32 and v_min_i32 the broadcast gave wrong codes)
 #pragma unroll
         for (int i = 0; i < N; i += 8 / BITS) {
             uint32_t q = 0;
 #pragma unroll
             for (int j = 0; j < 8 / BITS; j++)
-                q |= (uint32_t)__builtin_amdgcn_fmed3f(rint_div(x[r][i + j], sr, ir, half) - zr, 0.0f, (float)CODES) << (j * BITS);
+                q |= (uint32_t)min(max((int)(rint_div(x[r][i + j], sr, ir) - asu(zr)), 0), (int)asu(most)) << (j * BITS);
             out[r][i * BITS / 8] = (uint8_t)q;
         }
         if (!all && on[r])
