@@ -1271,7 +1271,7 @@ class KVCache:
     Sequences are rows of a batch: `table` (batch, n) int32 names each one's pages (None: page b is sequence b's only one),
     `start` / `context` and `lens` are int32 of (batch,).  Rows from lens[b] on are padding and are not touched.
     Calls go to torch's current stream, allocate what they return (and the attention its workspace) from torch, and can be
-    captured into a graph."""
+    captured into a graph.  They have no gradient."""
 
     def __init__(self, pages, page_size, heads, head_dim, bits=4, buffer=None, device="cuda"):
         self._native = native()
@@ -1345,7 +1345,8 @@ class ActCheckpoint:
     def load(self):
         """The kept values as floats: a tuple of one tensor, or two of a gated activation."""
         code = _dtype_code(self.dtype)
-        return tuple(_native.act_load(t, code, *self.shape) for t in (self.kept, self.kept_up) if t is not None)
+        x = _native.act_load(self.kept, code, *self.shape)
+        return (x,) if self.kept_up is None else (x, _native.act_load(self.kept_up, code, *self.shape))
 
 
 def _act_kind(kind):
@@ -1363,7 +1364,9 @@ def act_save(x):
 def act_forward(x, kind, up=None):
     """y = f(x) (kind 'silu' or 'gelu', the exact one) or f(x) * up, and the ActCheckpoint of x (and up), in one pass."""
     y, kept, kept_up = native().act_forward(x, _act_kind(kind), up)
-    return y, ActCheckpoint(x.shape, x.dtype, kept, kept_up)
+    c = ActCheckpoint.__new__(ActCheckpoint)                # (what is new needs no checks)
+    c.shape, c.dtype, c.kept, c.kept_up = x.shape, x.dtype, kept, kept_up
+    return y, c
 
 
 def act_backward(dy, checkpoint, kind, recompute=False):
