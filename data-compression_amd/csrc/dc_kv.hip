@@ -616,7 +616,7 @@ template <int D, int BITS, int NT, bool PAST> __global__ __launch_bounds__(256) 
     const uint32_t h = x % a.heads; x /= a.heads;
     const uint32_t b = x % a.batch, split = x / a.batch;
     const int context = context_of(a, b);
-    if (context != a.start[b] && threadIdx.x == 0) atomicOr(a.status, 1u);
+    if (context != ((const Const*)a.start)[b] && threadIdx.x == 0) atomicOr(a.status, 1u);
     const int len = a.lens ? min(max(((const Const*)a.lens)[b], 0), a.tokens) : a.tokens;
     const int rows = len * a.group;
     const int row0 = tile * COLS;
@@ -647,6 +647,50 @@ template <int D, int BITS, int NT, bool PAST> __global__ __launch_bounds__(256) 
     }
     const long long lo64 = (long long)split * chunk;
     const int lo = lo64 < most ? (int)lo64 : most, hi = (int)min((long long)most, lo64 + chunk);
+
+    // the wave's tokens: 32 of each 128.  Their pages are followed from step to step: a table entry and a block of 16
+    // within its page, for the first block and for the one behind it.  (The first ones are loaded before the queries are
+    // waited for)
+    const Const* table = a.table ? (const Const*)a.table + (long long)b * a.table_stride : nullptr;
+    const uint32_t blocks = (uint32_t)a.page >> 4, slot_step = div_by(8u, a.blocks_inv), in_step = 8u - slot_step * blocks;
+    const int first = lo + wave * 32;
+    uint32_t slot = div_by((uint32_t)first >> 4, a.blocks_inv), in = ((uint32_t)first >> 4) - slot * blocks;
+    const uint32_t lane_codes = (uint32_t)(col * ROW + g * (4 * U)), lane_words = (uint32_t)(g * 4 + (lane & 3)) * 4;
+    const bool second = lane & 4;
+    const uint64_t codes_to_values = (uint64_t)a.page * ROW;
+    const uint32_t words_to_values = 4u * (uint32_t)a.page;
+    int page[2];
+    uint32_t place[2];
+    auto find = [&](int t) {                                // (the second block may lie past the end: then the first again)
+        const uint32_t s1 = in + 1 == blocks ? slot + 1 : slot;
+        const bool two = t + 16 < hi;
+        place[0] = in;
+        place[1] = !two ? in : in + 1 == blocks ? 0 : in + 1;
+        page[0] = table ? table[slot] : (int)b;
+        page[1] = table ? table[two ? s1 : slot] : (int)b;
+        in += in_step;
+        slot += slot_step;
+        if (in >= blocks) { in -= blocks; slot++; }
+    };
+    auto where = [&](Where& w) {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            w.hole[j] = page[j] < 0 || page[j] >= a.pages;
+            const uint8_t* base = a.data + ((long long)(w.hole[j] ? 0 : page[j]) * a.heads + h) * a.head_bytes;
+            w.codes[j] = base + (uint64_t)place[j] * (16 * ROW);
+            w.words[j] = base + 2 * codes_to_values + (uint64_t)place[j] * 64;
+        }
+    };
+    Stage<U> c;
+    Where now, next;
+    if (first < hi) {
+        find(first);
+        where(now);
+        load_keys<PAST>(c, now, lane_codes);
+        load_words(c, now, words_to_values, second, lane_words);
+        load_values<PAST>(c, now, codes_to_values, lane_codes);
+        if (first + 128 < hi) find(first + 128);
+    }
 
     // queries, as f16 in the keys' order; with the scale's sign; their sum and the factor
     // that takes a score to log2 units
@@ -702,48 +746,6 @@ template <int D, int BITS, int NT, bool PAST> __global__ __launch_bounds__(256) 
         for (int i = 0; i < N; i++) acc[nt][i] = (f4){0, 0, 0, 0};
     }
 
-    // the wave's tokens: 32 of each 128.  Their pages are followed from step to step: a table entry and a block of 16
-    // within its page, for the first block and for the one behind it
-    const Const* table = a.table ? (const Const*)a.table + (long long)b * a.table_stride : nullptr;
-    const uint32_t blocks = (uint32_t)a.page >> 4, slot_step = div_by(8u, a.blocks_inv), in_step = 8u - slot_step * blocks;
-    const int first = lo + wave * 32;
-    uint32_t slot = div_by((uint32_t)first >> 4, a.blocks_inv), in = ((uint32_t)first >> 4) - slot * blocks;
-    const uint32_t lane_codes = (uint32_t)(col * ROW + g * (4 * U)), lane_words = (uint32_t)(g * 4 + (lane & 3)) * 4;
-    const bool second = lane & 4;
-    const uint64_t codes_to_values = (uint64_t)a.page * ROW;
-    const uint32_t words_to_values = 4u * (uint32_t)a.page;
-    int page[2];
-    uint32_t place[2];
-    auto find = [&](int t) {                                // (the second block may lie past the end: then the first again)
-        const uint32_t s1 = in + 1 == blocks ? slot + 1 : slot;
-        const bool two = t + 16 < hi;
-        place[0] = in;
-        place[1] = !two ? in : in + 1 == blocks ? 0 : in + 1;
-        page[0] = table ? table[slot] : (int)b;
-        page[1] = table ? table[two ? s1 : slot] : (int)b;
-        in += in_step;
-        slot += slot_step;
-        if (in >= blocks) { in -= blocks; slot++; }
-    };
-    auto where = [&](Where& w) {
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-            w.hole[j] = page[j] < 0 || page[j] >= a.pages;
-            const uint8_t* base = a.data + ((long long)(w.hole[j] ? 0 : page[j]) * a.heads + h) * a.head_bytes;
-            w.codes[j] = base + (uint64_t)place[j] * (16 * ROW);
-            w.words[j] = base + 2 * codes_to_values + (uint64_t)place[j] * 64;
-        }
-    };
-    Stage<U> c;
-    Where now, next;
-    if (first < hi) {
-        find(first);
-        where(now);
-        load_keys<PAST>(c, now, lane_codes);
-        load_words(c, now, words_to_values, second, lane_words);
-        load_values<PAST>(c, now, codes_to_values, lane_codes);
-        if (first + 128 < hi) find(first + 128);
-    }
     int t0 = first;
     auto advance = [&] {                                    // (behind the last step its own tokens are loaded once more)
         if (t0 + 128 < hi) {
