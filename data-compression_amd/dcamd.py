@@ -1383,7 +1383,8 @@ _activation = None
 
 def activation(x, kind, up=None):
     """act_forward's output as a differentiable torch function: between the passes it holds the 8-bit checkpoint instead
-    of its inputs, and its gradient is that at the checkpoint's values.  Not differentiable twice."""
+    of its inputs, and its gradient is that at the checkpoint's values.  Not differentiable twice.  A capture of its backward
+    pass follows torch's rule: no eager graph of the same leaves is alive."""
     global _activation
     if _activation is None:
         native()

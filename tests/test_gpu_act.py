@@ -297,3 +297,54 @@ def test_graph(act):
         got = [t.clone() for t in out]
         for a, b in zip(got, step()):
             assert same(a, b)
+
+
+def test_graph_of_the_function(act):
+    """The differentiable function and its gradient captured (no eager graph of the leaf alive) and replayed."""
+    x, up, dy = (torch.randn(40, 96, device=DEV).half() for _ in range(3))
+    x.requires_grad_()
+
+    def step():
+        y = act.activation(x, "silu", up=up)
+        return y.detach(), torch.autograd.grad(y, x, dy)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):
+        with torch.no_grad():
+            x.copy_(torch.randn(40, 96, generator=torch.Generator().manual_seed(i)))
+        graph.replay()
+        torch.cuda.synchronize()
+        y, kept = act.act_forward(x.detach(), "silu", up=up)
+        assert same(out[0], y) and same(out[1], act.act_backward(dy, kept, "silu")[0])
+
+
+def test_threads(act):
+    """Calls of several threads, each on its own stream."""
+    import threading
+    xs = [torch.randn(300 + 7 * i, 64, device=DEV) for i in range(4)]
+    want = [act.act_forward(x, "gelu") for x in xs]
+    torch.cuda.synchronize()
+    got = [None] * 4
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                y, kept = act.act_forward(xs[i], "gelu")
+                back, = kept.load()
+            torch.cuda.current_stream().synchronize()
+            got[i] = y, kept.kept, back
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for (y, kept), (z, k, back) in zip(want, got):
+        assert same(y, z) and torch.equal(kept.kept, k) and same(back, kept.load()[0])
