@@ -95,8 +95,9 @@ static int rows_call(const dc_kv_cache* c, const dc_kv_batch* at, int dtype, con
     memcpy(a.ks, ks, sizeof a.ks);
     memcpy(a.vs, vs, sizeof a.vs);
     a.dtype = dtype;
-    /* an output that no cache holds is written past them (4 sequences of 16384, bf16: 62 us, so 47); a smaller one is
-       not (3 of 4095, f16: 12.1 us, so 12.8), and its reader finds it there */
+    /* floats that no cache holds pass them (4 sequences of 16384 read, bf16: 62 us, so 47; 16 of 4095 written, f16, and read
+       back: 112, so 103); fewer do not (3 of 4095, f16, read: 12.1 us, so 12.8, written: 17.0, so 18.0), and what uses them next
+       finds them there */
     a.past = 2.0 * at->batch * at->tokens * c->heads * c->head_dim * size > 128e6;
     const unsigned piece = low_bit((unsigned)(c->head_dim / 16 * size));
     a.vec = fits(k, ks, size, piece > 16 ? 16 : piece) && fits(v, vs, size, piece > 16 ? 16 : piece);

@@ -95,6 +95,11 @@ template <class T, int N, int A> static __device__ __forceinline__ void store_n(
 }
 
 // the same past the caches, 16 bytes at a time
+template <class T, int N> static __device__ __forceinline__ void load_past(const T* p, T* x) {
+    static_assert(N * (int)sizeof(T) % 16 == 0, "whole pieces");
+#pragma unroll
+    for (int i = 0; i < N * (int)sizeof(T) / 16; i++) ((u4*)x)[i] = __builtin_nontemporal_load((const u4*)p + i);
+}
 template <class T, int N> static __device__ __forceinline__ void store_past(T* p, const T* x) {
     static_assert(N * (int)sizeof(T) % 16 == 0, "whole pieces");
 #pragma unroll
@@ -188,7 +193,8 @@ template <bool WRITE> static __device__ __forceinline__ bool block_of(const KvAr
     return true;
 }
 
-template <class E, int D, int BITS, bool VEC> __global__ __launch_bounds__(256) void kv_write(KvArgs a) {
+// PAST: the input passes the caches
+template <class E, int D, int BITS, bool VEC, bool PAST> __global__ __launch_bounds__(256) void kv_write(KvArgs a) {
     constexpr int N = D / 16, U = N * BITS / 8, ROW = 16 * U;
     constexpr int BYTES = N * (int)sizeof(typename E::T);
     constexpr int AL = VEC ? (BYTES & -BYTES) : (int)sizeof(typename E::T);
@@ -219,7 +225,10 @@ template <class E, int D, int BITS, bool VEC> __global__ __launch_bounds__(256) 
     }
 #pragma unroll
     for (int r = 0; r < 4; r++)
-        if (on[r]) load_n<typename E::T, N, AL>(src + (t + r) * stride, raw[r]);
+        if (on[r]) {
+            if constexpr (PAST && VEC && BYTES % 16 == 0) load_past<typename E::T, N>(src + (t + r) * stride, raw[r]);
+            else load_n<typename E::T, N, AL>(src + (t + r) * stride, raw[r]);
+        }
     // the four rows' smallest and largest values; then their steps and zero points, row u % 4 by lane u for all
     float x[4][N], lo[4], hi[4];
 #pragma unroll
@@ -356,9 +365,10 @@ template <class E, int D, int BITS, bool VEC, bool PAST> __global__ __launch_bou
 // step of 32 tokens x 32 queries of 64 values is 200 vector instructions (302 before), 16 of them exponentials.
 //
 // 48 sequences of up to 8192 positions, 8 heads of 128 in 4 bits: 61 us and 4.7 for the join, 5.0 TB/s; bound by HBM, in
-// pieces of 2 KiB.  One of 262143, 2 heads: 16.6 + 4.6 us, 4.2 TB/s.  517 positions: 9.6 us, the chain of lengths, pages,
-// codes, scores and sums.  Prompts (two of 509 queries behind 8192, 16 heads of 64, 8 bits): 65 to 73 us, 345 TFLOP/s, 84 % of
-// the vector instructions' rate while the waves run, uneven lengths the rest.
+// pieces of 2 KiB.  One of 262143, 2 heads: 16.6 + 4.6 us, 4.2 TB/s.  517 positions: 9.2 us, the chain of lengths, pages,
+// codes, scores and sums.  Prompts (two of up to 509 queries behind 8192, 16 heads of 64, 8 bits): 64 to 80 us by their
+// lengths, 316 to 390 TFLOP/s, 84 % of the vector instructions' rate while the waves run; the longer one's workgroups are
+// waited for (cut in pieces they cost their prologues and the join: 72 us, so 72 to 78).
 static __device__ __forceinline__ float over_groups_max(float x) {     // over the 4 groups of 16 lanes
     auto p = __builtin_amdgcn_permlane32_swap((int)asu(x), (int)asu(x), false, false);
     x = fmaxf(asf((uint32_t)p[0]), asf((uint32_t)p[1]));
@@ -925,8 +935,10 @@ template <class E, int BITS, bool VEC> int go_rows(const KvArgs& a, bool write, 
     const unsigned grid = (unsigned)((a.rows + 3) / 4);
 #define DC_ROWS(D) \
     case D: \
-        if (write) kv_write<E, D, BITS, VEC><<<grid, 256, 0, st>>>(a); \
-        else if (VEC && a.past) kv_read<E, D, BITS, VEC, VEC><<<grid, 256, 0, st>>>(a); \
+        if (VEC && a.past) { \
+            if (write) kv_write<E, D, BITS, VEC, VEC><<<grid, 256, 0, st>>>(a); \
+            else kv_read<E, D, BITS, VEC, VEC><<<grid, 256, 0, st>>>(a); \
+        } else if (write) kv_write<E, D, BITS, VEC, false><<<grid, 256, 0, st>>>(a); \
         else kv_read<E, D, BITS, VEC, false><<<grid, 256, 0, st>>>(a); \
         break
     switch (a.dim) {

@@ -118,7 +118,7 @@ typedef struct KvArgs {
     const void* k;                 /* write: keys, read: keys out, attention: queries; strides (batch, token, head) in elements */
     const void* v;                 /* write: values, read: values out, attention: the output */
     long long ks[3], vs[3];
-    int past;                      /* read: the output passes the caches; attention: the codes do */
+    int past;                      /* write, read: the floats pass the caches; attention: the codes do */
     int zero_padding;              /* outputs behind lens[b]: 0 (1) or left as they are */
     int dtype, vec, vec_out;       /* vec: pointers and strides allow whole-lane accesses */
     int blocks;                    /* write / read: blocks of 16 places that a sequence's tokens can touch */

@@ -608,3 +608,18 @@ def test_attention_queries_of_all_sizes(kv, k):
     want = check(f, q, [300], scale=0.125)
     got = f.cache.attention((q.float() * 2.0 ** k).bfloat16().to(DEV), i32(300), table=f.table, scale=0.125 * 2.0 ** -k)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype,n", [(torch.float32, 9000), (torch.bfloat16, 17000)])
+def test_large_write(kv, dtype, n):
+    """An input that is read past the caches (over 128 MB) as the same in parts."""
+    H, D, P = 16, 128, 48
+    pages = -(-n // P)
+    table = torch.randperm(pages, generator=gen(98)).to(torch.int32).to(DEV)[None]
+    k, v = (torch.randn(1, n, H, D, device=DEV).to(dtype) for _ in range(2))
+    whole, parts = (make(kv, pages, P, H, D, 4) for _ in range(2))
+    whole.write(k, v, i32(0), table=table)
+    for first in range(0, n, 3001):
+        m = min(3001, n - first)
+        parts.write(k[:, first:first + m], v[:, first:first + m], i32(first), table=table)
+    assert torch.equal(whole.buffer, parts.buffer)
