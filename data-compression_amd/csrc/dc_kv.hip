@@ -351,10 +351,12 @@ template <class E, int D, int BITS, bool VEC, bool PAST> __global__ __launch_bou
 // exponent on, in which a subnormal counts as 2^-14: it is exact to 2^-18 (4 bits; 2^-14: 8 bits) of a code's unit times the
 // largest weight.  (In bits 0..3 that were 2^-14 of 15.)
 //
-// The weights w_t = p_t vs_t go into the product as f16, vs_t in units of the power of two 2^(R - 7) above the largest
-// step that the wave has met: p_t <= 2^8 (the running maximum of the scores is raised only when a score passes it by 8),
-// so w_t < 2^15, and 11 bits are kept down to 2^-21 of that step's full weight, fewer below: a weight is off by 2^-11 of
-// itself, half a unit of what f16 outputs round to, or by 2^-32 of the largest step.  The sum of p_t is kept in f32.
+// The weights w_t = p_t vs_t go into the product as f16, in units of each query row's own: p_t is 2 to the power of the score less
+// a reference M, and vs_t counts in 2^(R - 7), one power of two for a wave.  M is raised only by what its row sees (`refer`)
+// and so that the largest weight yet is 16 or more and below 2^15.  So 11 bits are kept down to 2^-14, fewer below: a weight
+// is off by 2^-11 of itself, half a unit of what f16 outputs round to, or by 2^-29 of its row's largest; whatever the steps
+// of tokens that a row does not see, or sees with no weight.  (Steps 2^-100 of the largest in a tile of rows lose bits.)  The
+// sum of p_t is kept in f32.
 // Queries are scaled to 2^14..2^15 by a power of two (exact); elements 2^-30 of a row's largest lose bits.
 //
 // A token's words are wanted by the 16 lanes that share its 4 tokens of a block: lane % 8 decodes one of the group's 8
@@ -440,6 +442,9 @@ template <int N, bool LSE = true> static __device__ __forceinline__ void put(con
 }
 // the log of a row's sum l with the reference m
 static __device__ __forceinline__ float log_sum(float m, float l) { return (m + log2f(l)) * 0.69314718055994530942f; }
+// 2^(x / 2): the references of waves and pieces may lie so far apart that only the product with what they refer to, taken
+// with the root twice, stays in f32's range
+static __device__ __forceinline__ float root_exp(float x) { return __builtin_amdgcn_exp2f(0.5f * x); }
 // 1 / l; NaN where it is NaN, or nothing of what a query sees is in the cache
 static __device__ __forceinline__ float inverse_sum(float l) { return l > 0.0f ? 1.0f / l : asf(0x7FC00000u); }
 
@@ -460,6 +465,48 @@ template <int U> static __device__ __forceinline__ void load_words(Stage<U>& c, 
     const uint8_t* p = (second ? at.words[1] : at.words[0]) + lane_words;
     c.kw = *(const uint32_t*)p;
     c.vw = *(const uint32_t*)(p + to_values);
+}
+
+// New references for a step whose weights may not fit f16 (or are the first).  `ref` times `unit` are its scores.
+//
+// R follows the steps where they drift (a largest one below 2^8 R) or may pass what f32 holds (above 2^64 R); one far above the
+// others in between is left to its row's reference, as its weights may be nothing.  R does not change what a row's
+// weights are in units of its own: M goes down with 1 / R, as far as L then stays in f32's range.  Then M is raised
+// to the row's largest score where that token's weight is still 16 or more, and to what makes the largest weight 2^7 ..
+// 2^8 where it would pass 2^15; it is never more than 80 below the largest score, so that p and L stay below 2^118.
+template <int NT, int N>
+static __device__ __forceinline__ void refer(const float (*ref)[8], const float* mx, const float* unit, float vs,
+                                             f4 (*acc)[N], float* M, float* L, float* Z, float& R) {
+    const float top = over_groups_max(max16(vs >= R ? vs : 0.0f));
+    int up = 0;                                             // R is raised by 2^up
+    if (top >= R && (top < R * 256.0f || top > R * 1.8446744e19f)) {
+        const uint32_t r = (asu(top) & 0x7F800000u) + 0x00800000u;
+        up = (int)(r - asu(R)) >> 23;
+        R = asf(r);
+    }
+    const float vr = vs * asf(0x7F000000u - asu(R)) * 128.0f;
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        const float hi = over_groups_max(mx[nt]) * unit[nt];
+        float m = M[nt];
+        if (up) m -= (float)min(min(up, 120), max(217 - (int)(asu(over_groups_max(L[nt])) >> 23), 0));    // (L < 2^91)
+        const float base = fmaxf(m, hi);
+        float x = 0.0f;                                     // the largest weight, with the reference `base`  (a NaN shows in the sums, or is of a score of -inf)
+        each_of(std::make_integer_sequence<int, 8>{}, [&](auto I) {
+            constexpr int t = I.value;
+            x = fmaxf(x, __builtin_amdgcn_exp2f(fmaf(ref[nt][t], unit[nt], -base)) * row_lane<t>(vr));
+        });
+        x = over_groups_max(x);
+        if (hi > m + 8.0f && x >= 16.0f) m = hi;
+        if (x * __builtin_amdgcn_exp2f(base - m) > 32768.0f) m = base + (float)((int)(asu(x) >> 23) - 134);
+        m = fmaxf(m, hi - 80.0f);
+        const float al = M[nt] - m, be = __builtin_amdgcn_exp2f(al - (float)up);
+        M[nt] = m;
+        L[nt] *= __builtin_amdgcn_exp2f(al);
+        Z[nt] *= be;
+#pragma unroll
+        for (int i = 0; i < N; i++) acc[nt][i] *= be;
+    }
 }
 
 // One step of a wave: 32 tokens from t0 on against NT tiles of 16 queries.  EDGE: some of them may not be seen.  What the
@@ -513,27 +560,11 @@ static __device__ __forceinline__ void attend(Stage<D * BITS / 128>& c, const Fr
             mx[nt] = fmaxf(mx[nt], y);
         }
     });
-    // a score that passes its maximum by 8, or a step as large as the unit (not a NaN): new references
+    // a score that passes its row's reference by 8, or a step as large as the unit (not a NaN): new references
     bool raise = vs >= R;
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) raise |= mx[nt] * unit[nt] > M[nt] + 8.0f;
-    if (__any(raise)) {
-        float top = vs >= R ? vs : 0.0f;
-        for (int k = 32; k; k >>= 1) top = fmaxf(top, __shfl_xor(top, k));
-        const float r = fmaxf(R, asf((asu(top) & 0x7F800000u) + 0x00800000u));
-        const float down = asf((uint32_t)max((int)(0x3F800000u + asu(R) - asu(r)), 0));     // R / r, powers of two
-        R = r;
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            const float most = over_groups_max(mx[nt]) * unit[nt];
-            const float m = most > M[nt] + 8.0f ? most : M[nt], al = __builtin_amdgcn_exp2f(M[nt] - m);
-            M[nt] = m;
-            L[nt] *= al;
-            Z[nt] *= al * down;
-#pragma unroll
-            for (int i = 0; i < N; i++) acc[nt][i] *= al * down;
-        }
-    }
+    if (__any(raise)) refer<NT, N>(ref, mx, unit, vs, acc, M, L, Z, R);
     const float vr = vs * asf(0x7F000000u - asu(R)) * 128.0f;       // 2^7 / R
     Frag w[NT];
     each_of(std::make_integer_sequence<int, 4>{}, [&](auto I) {
@@ -747,7 +778,7 @@ template <int D, int BITS, int NT, bool PAST> __global__ __launch_bounds__(256) 
     }
 
     f4 acc[NT][N];
-    float M[NT], L[NT], Z[NT], R = 1.17549435e-38f;         // (2^-126: below every step)
+    float M[NT], L[NT], Z[NT], R = 7.888609052210118e-31f;  // (2^-100: the smallest step)
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
         M[nt] = -1e30f;
@@ -799,7 +830,7 @@ template <int D, int BITS, int NT, bool PAST> __global__ __launch_bounds__(256) 
     for (int nt = 0; nt < NT; nt++) {
         float m = ml[0][0][nt * 16 + col];
         for (int v = 1; v < 4; v++) m = fmaxf(m, ml[0][v][nt * 16 + col]);
-        f[nt] = __builtin_amdgcn_exp2f(M[nt] - m) * (R * 0.0078125f) * UNIT<BITS>;
+        f[nt] = root_exp(M[nt] - m) * (R * 0.0078125f) * root_exp(M[nt] - m) * UNIT<BITS>;
     }
     for (int v = 0; v < (ALL ? 1 : 4); v++) {
         if (ALL || wave == v)
@@ -823,9 +854,9 @@ template <int D, int BITS, int NT, bool PAST> __global__ __launch_bounds__(256) 
         float m = ml[0][0][nt * 16 + oc], l = 0.0f, z = 0.0f;
         for (int v = 1; v < 4; v++) m = fmaxf(m, ml[0][v][nt * 16 + oc]);
         for (int v = 0; v < 4; v++) {
-            const float sc = __builtin_amdgcn_exp2f(ml[0][v][nt * 16 + oc] - m);
-            l = fmaf(ml[1][v][nt * 16 + oc], sc, l);
-            z = fmaf(ml[2][v][nt * 16 + oc], sc, z);
+            const float sc = root_exp(ml[0][v][nt * 16 + oc] - m);
+            l = fmaf(ml[1][v][nt * 16 + oc] * sc, sc, l);
+            z = fmaf(ml[2][v][nt * 16 + oc] * sc, sc, z);
         }
         float o[N];
 #pragma unroll
@@ -871,9 +902,9 @@ template <int D> __global__ __launch_bounds__(256) void kv_join_few(KvArgs a) {
     f4 o = {0, 0, 0, 0};
 #pragma unroll 4
     for (int s = 0; s < pieces; s++) {
-        const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * (at + s)] - m);
-        l = fmaf(a.part_ml[2 * (at + s) + 1], f, l);
-        o += *(const f4*)(a.part + (at + s) * D + d0) * f;
+        const float f = root_exp(a.part_ml[2 * (at + s)] - m);
+        l = fmaf(a.part_ml[2 * (at + s) + 1] * f, f, l);
+        o += *(const f4*)(a.part + (at + s) * D + d0) * f * f;
     }
     const bool none = (a.causal ? context - len + 1 + (int)div_by((uint32_t)rw, a.group_inv) : context) <= 0;
     const float inv = none ? 0.0f : inverse_sum(l);
@@ -908,9 +939,9 @@ template <int D> __global__ __launch_bounds__(256) void kv_join(KvArgs a) {
     if ((tid & 63) == 0) red[0][tid >> 6] = top;
     __syncthreads();
     top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-    const float scale = __builtin_amdgcn_exp2f(m - top);
+    const float scale = root_exp(m - top);
     f[tid] = scale;
-    l *= scale;
+    l = l * scale * scale;
     for (int k = 32; k; k >>= 1) l += __shfl_xor(l, k);
     if ((tid & 63) == 0) red[1][tid >> 6] = l;
     __syncthreads();
@@ -919,7 +950,7 @@ template <int D> __global__ __launch_bounds__(256) void kv_join(KvArgs a) {
     f4 o = {0, 0, 0, 0};
     const float* p = a.part + at * D + d0 + dl * 4;
 #pragma unroll 4
-    for (int s = sl; s < pieces; s += 32) o += *(const f4*)(p + (long long)s * D) * f[s];
+    for (int s = sl; s < pieces; s += 32) o += *(const f4*)(p + (long long)s * D) * f[s] * f[s];
     sums[sl][dl] = o;
     __syncthreads();
     if (tid < 32) {

@@ -328,7 +328,9 @@ int dc_kv_read_device(const dc_kv_cache* cache, const dc_kv_batch* at, int dtype
  * [batch][tokens][q_heads], may be NULL) receives the log of the softmax's sum.  max_context: no start[b] is expected above it (it
  * sizes the split along the cache; a longer one is still computed in full).  d_workspace: dc_kv_attention_workspace
  * bytes (16-byte aligned; NULL where that is 0), in use until the call's work is done: calls that may run at once need
- * one each.  Outputs must not overlap the inputs.  Scores are formed in f32 from queries and steps below 2^100. */
+ * one each.  Outputs must not overlap the inputs.  Scores are formed in f32 from queries and steps below 2^100.  A position's
+ * softmax weight times the step of its values is held to 2^-11 of itself or 2^-29 of its query's largest, whichever is more;
+ * positions that a query does not see have no part in that. */
 size_t dc_kv_attention_workspace(const dc_kv_cache* cache, int batch, int tokens, int q_heads, long long max_context);
 int dc_kv_attention_device(const dc_kv_cache* cache, const dc_kv_batch* at, int dtype, int q_heads, const void* d_q,
                            const long long* q_strides, float scale, int causal, long long max_context, void* d_out,
