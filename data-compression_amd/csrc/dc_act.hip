@@ -35,20 +35,27 @@ template <> struct Elem<DC_BF16> { typedef __bf16 T; typedef b8 V; static conste
 
 // 1 / x and e^x by the hardware's instructions; WIDE (f32 results): with the rounding error of the exponent's argument
 static __device__ __forceinline__ float over(float x) { return __builtin_amdgcn_rcpf(x); }
-template <bool WIDE> static __device__ __forceinline__ float exp_of(float x) {                  // e^x
-    const float hi = x * 1.44269504088896340736f, e = __builtin_amdgcn_exp2f(hi);
+template <bool WIDE> static __device__ __forceinline__ float exp_of(float x, float k = 0.0f) {  // e^x 2^k
+    const float hi = x * 1.44269504088896340736f, e = __builtin_amdgcn_exp2f(hi + k);           // (k is not 0 where |hi| > k alone: an exact sum)
     if constexpr (!WIDE) return e;
     const float lo = fmaf(x, 1.44269504088896340736f, -hi) + x * 1.925963033500e-8f;
     return fabsf(lo) < 1.0f ? fmaf(e, lo * 0.69314718055994530942f, e) : e;                     // (x infinite: lo is NaN)
 }
 
-// silu: f = x sigma, f' = sigma (1 + x (1 - sigma))
+// silu: f = x sigma, f' = sigma (1 + x (1 - sigma)).  f32: from e^-|x|, in units of 2^-64 where it is small, so that the tail
+// keeps its precision down to the smallest normal result and no power overflows; 16 bits: from e^-x, whose reciprocal is 0
+// below -87 (results of less than 2^-119).
 // gelu: f = x Phi(x), f' = Phi(x) + x phi(x).  With t = 1 / (1 + c |x|) the upper tail is Phi(-|x|) = e^(-x^2/2) t p(t), p a
 // polynomial fitted to it, for f32 of degree 8 (relative error below 5e-8 for every x), for 16 bits of degree 5 (8e-6: the
 // forward pass is bound by its arithmetic, not by HBM, with the longer one).
 template <int KIND, bool WIDE> static __device__ __forceinline__ void value_slope(float x, float& f, float& df) {
-    if constexpr (KIND == DC_ACT_SILU) {
-        const float e = exp_of<WIDE>(-x), s = over(1.0f + e);
+    if constexpr (KIND == DC_ACT_SILU && WIDE) {
+        const float a = fabsf(x), unit = a > 64.0f ? 5.421010862427522e-20f : 1.0f;
+        const float e = exp_of<true>(-a, a > 64.0f ? 64.0f : 0.0f), s = over(fmaf(e, unit, 1.0f)), r = e * s, small = r * unit;
+        f = x < 0.0f ? x * r * unit : x * s;
+        df = fmaf(f, x < 0.0f ? s : small, x < 0.0f ? small : s);
+    } else if constexpr (KIND == DC_ACT_SILU) {
+        const float e = exp_of<false>(-x), s = over(1.0f + e);
         f = x * s;
         df = fmaf(f, 1.0f - s, s);                          // (x sigma (1 - sigma): finite wherever f is)
     } else {
