@@ -386,6 +386,8 @@ static __device__ __forceinline__ float over_groups_sum(float x) {
 
 union Frag { h8 v; uint32_t u[4]; };
 
+constexpr float NOTHING = -3.402823466e38f;                 // the reference of a row that has seen nothing: below every score, and finite
+
 template <int BITS> constexpr float UNIT = BITS == 4 ? 1048576.0f : 16777216.0f;
 // the codes in both halves of x times 1 / UNIT: 4 bits, four pairs of nibbles 0..3; 8 bits, two of bytes 0..1
 template <int BITS> static __device__ __forceinline__ void codes_of(uint32_t x, uint32_t* o) {
@@ -469,17 +471,25 @@ template <int U> static __device__ __forceinline__ void load_words(Stage<U>& c, 
 
 // New references for a step whose weights may not fit f16 (or are the first).  `ref` times `unit` are its scores.
 //
-// R follows the steps where they drift (a largest one below 2^8 R) or may pass what f32 holds (above 2^64 R); one far above the
-// others in between is left to its row's reference, as its weights may be nothing.  R does not change what a row's
-// weights are in units of its own: M goes down with 1 / R, as far as L then stays in f32's range.  Then M is raised
-// to the row's largest score where that token's weight is still 16 or more, and to what makes the largest weight 2^7 ..
-// 2^8 where it would pass 2^15; it is never more than 80 below the largest score, so that p and L stay below 2^118.
+// R follows the steps where they drift (a largest one below 2^8 R), may pass what f32 holds (above 2^64 R) or scores are so
+// large that a reference cannot be moved by single bits; one far above the others is else left to its row's reference, as its
+// weights may be nothing.  R does not change what a row's weights are in units of its own: M goes down with 1 / R, as far as L
+// then stays below 2^91.  Then M is raised to the row's largest score where that token's weight is still 16 or more, and to
+// what makes the largest weight 2^7 .. 2^8 where it would pass 2^15; it is never more than 80 below the largest score, so
+// that p and L stay below 2^118.
 template <int NT, int N>
 static __device__ __forceinline__ void refer(const float (*ref)[8], const float* mx, const float* unit, float vs,
                                              f4 (*acc)[N], float* M, float* L, float* Z, float& R) {
     const float top = over_groups_max(max16(vs >= R ? vs : 0.0f));
+    bool far = false;
+    float hi[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        hi[nt] = over_groups_max(mx[nt]) * unit[nt];
+        far |= fabsf(hi[nt]) > 1048576.0f && fabsf(hi[nt]) < INFINITY;
+    }
     int up = 0;                                             // R is raised by 2^up
-    if (top >= R && (top < R * 256.0f || top > R * 1.8446744e19f)) {
+    if (top >= R && (top < R * 256.0f || top > R * 1.8446744e19f || __any(far))) {
         const uint32_t r = (asu(top) & 0x7F800000u) + 0x00800000u;
         up = (int)(r - asu(R)) >> 23;
         R = asf(r);
@@ -487,19 +497,18 @@ static __device__ __forceinline__ void refer(const float (*ref)[8], const float*
     const float vr = vs * asf(0x7F000000u - asu(R)) * 128.0f;
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-        const float hi = over_groups_max(mx[nt]) * unit[nt];
         float m = M[nt];
-        if (up) m -= (float)min(min(up, 120), max(217 - (int)(asu(over_groups_max(L[nt])) >> 23), 0));    // (L < 2^91)
-        const float base = fmaxf(m, hi);
-        float x = 0.0f;                                     // the largest weight, with the reference `base`  (a NaN shows in the sums, or is of a score of -inf)
+        if (up && fabsf(m) < 1048576.0f) m -= (float)min(min(up, 120), max(217 - (int)(asu(over_groups_max(L[nt])) >> 23), 0));
+        const float base = fmaxf(m, hi[nt]);
+        float x = 0.0f;                                     // the largest weight, with the reference `base`  (NaNs show in the sums)
         each_of(std::make_integer_sequence<int, 8>{}, [&](auto I) {
             constexpr int t = I.value;
             x = fmaxf(x, __builtin_amdgcn_exp2f(fmaf(ref[nt][t], unit[nt], -base)) * row_lane<t>(vr));
         });
         x = over_groups_max(x);
-        if (hi > m + 8.0f && x >= 16.0f) m = hi;
+        if (hi[nt] > m + 8.0f && x >= 16.0f) m = hi[nt];
         if (x * __builtin_amdgcn_exp2f(base - m) > 32768.0f) m = base + (float)((int)(asu(x) >> 23) - 134);
-        m = fmaxf(m, hi - 80.0f);
+        m = fmaxf(m, hi[nt] - 80.0f);
         const float al = M[nt] - m, be = __builtin_amdgcn_exp2f(al - (float)up);
         M[nt] = m;
         L[nt] *= __builtin_amdgcn_exp2f(al);
@@ -514,7 +523,7 @@ static __device__ __forceinline__ void refer(const float (*ref)[8], const float*
 // rest of this step and the beginning of the next.
 template <int D, int BITS, int NT, bool PAST, bool EDGE>
 static __device__ __forceinline__ void attend(Stage<D * BITS / 128>& c, const Frag (*q)[D / 32], const float* qsum,
-                                              const float* unit, const int* sees, int t0, int most, int g,
+                                              const float* unit, float significand, const int* sees, int t0, int most, int g,
                                               const bool* hole, const Where& next, uint64_t codes_to_values,
                                               uint32_t words_to_values, uint32_t lane_codes, bool second, uint32_t lane_words,
                                               f4 (*acc)[D / 16], float* M, float* L, float* Z, float& R) {
@@ -524,7 +533,7 @@ static __device__ __forceinline__ void attend(Stage<D * BITS / 128>& c, const Fr
         const int at = t0 + (second ? 16 : 0) + (int)(lane_words >> 2);
         if (at >= most || hole[second]) c.kw = c.vw = 0;
     }
-    const float ks = asf(c.kw << 16), kz = (float)(int16_t)(c.kw >> 16), vs = asf(c.vw << 16), vz = (float)(int16_t)(c.vw >> 16);
+    const float ks = asf(c.kw << 16) * significand, kz = (float)(int16_t)(c.kw >> 16), vs = asf(c.vw << 16), vz = (float)(int16_t)(c.vw >> 16);
     f4 s[NT][2];                                            // from z sum(q) on
     each_of(std::make_integer_sequence<int, 8>{}, [&](auto I) {
         constexpr int t = I.value;
@@ -574,11 +583,6 @@ static __device__ __forceinline__ void attend(Stage<D * BITS / 128>& c, const Fr
             float p[2], x[2];
 #pragma unroll
             for (int k = 0; k < 2; k++) p[k] = __builtin_amdgcn_exp2f(fmaf(ref[nt][t + k], unit[nt], -M[nt]));
-            if (EDGE) {                                     // (a unit of 0)
-#pragma unroll
-                for (int k = 0; k < 2; k++)
-                    if (((t + k) & 3) >= left[nt][t >> 2]) p[k] = 0.0f;
-            }
             x[0] = p[0] * row_lane<t>(vr);
             x[1] = p[1] * row_lane<t + 1>(vr);
             if (EDGE) {                                     // (0 times a NaN)
@@ -733,8 +737,11 @@ template <int D, int BITS, int NT, bool PAST> __global__ __launch_bounds__(256) 
         if (first + 128 < hi) find(first + 128);
     }
 
-    // queries, as f16 in the keys' order; with the scale's sign; their sum and the factor
-    // that takes a score to log2 units
+    // queries, as f16 in the keys' order, with the scale's sign; their sum; and the power of two that takes a score to log2
+    // units.  (The scale's significand goes with the keys' steps.  A score times its unit is then exact, and its difference
+    // from a reference 0 for the score that was made the reference, however large it is)
+    const float per_score = fabsf(a.scale) * 1.44269504088896340736f, significand = __builtin_amdgcn_frexp_mantf(per_score);
+    const int exponent = __builtin_amdgcn_frexp_expf(per_score) + (BITS == 4 ? 20 : 24);    // (and UNIT's)
     Frag q[NT][KS];
     float qsum[NT], unit[NT];
 #pragma unroll
@@ -774,14 +781,14 @@ template <int D, int BITS, int NT, bool PAST> __global__ __launch_bounds__(256) 
                 sum += (float)v;
             }
         qsum[nt] = over_groups_sum(sum) * (1.0f / UNIT<BITS>);
-        unit[nt] = fabsf(a.scale) * (4096.0f * 1.44269504088896340736f) * down * (UNIT<BITS> / 4096.0f);    // (in normal numbers)
+        unit[nt] = fmaxf(__builtin_amdgcn_ldexpf(down, exponent), 1.17549435e-38f);     // (not 0: -inf times it is -inf)
     }
 
     f4 acc[NT][N];
     float M[NT], L[NT], Z[NT], R = 7.888609052210118e-31f;  // (2^-100: the smallest step)
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-        M[nt] = -1e30f;
+        M[nt] = NOTHING;
         L[nt] = Z[nt] = 0.0f;
 #pragma unroll
         for (int i = 0; i < N; i++) acc[nt][i] = (f4){0, 0, 0, 0};
@@ -798,7 +805,7 @@ template <int D, int BITS, int NT, bool PAST> __global__ __launch_bounds__(256) 
     while (t0 < hi && t0 + 32 <= least && t0 + 32 <= hi && !now.hole[0] && !now.hole[1]) {
         next = now;
         advance();
-        attend<D, BITS, NT, PAST, false>(c, q, qsum, unit, sees, t0, most, g, now.hole, next, codes_to_values, words_to_values,
+        attend<D, BITS, NT, PAST, false>(c, q, qsum, unit, significand, sees, t0, most, g, now.hole, next, codes_to_values, words_to_values,
                                    lane_codes, second, lane_words, acc, M, L, Z, R);
         now = next;
         t0 += 128;
@@ -807,7 +814,7 @@ template <int D, int BITS, int NT, bool PAST> __global__ __launch_bounds__(256) 
         if ((now.hole[0] || now.hole[1]) && lane == 0) atomicOr(a.status, 1u);
         next = now;
         advance();
-        attend<D, BITS, NT, PAST, true>(c, q, qsum, unit, sees, t0, most, g, now.hole, next, codes_to_values, words_to_values,
+        attend<D, BITS, NT, PAST, true>(c, q, qsum, unit, significand, sees, t0, most, g, now.hole, next, codes_to_values, words_to_values,
                                   lane_codes, second, lane_words, acc, M, L, Z, R);
         now = next;
         t0 += 128;
@@ -897,7 +904,7 @@ template <int D> __global__ __launch_bounds__(256) void kv_join_few(KvArgs a) {
     const int d0 = (int)threadIdx.x % LANES * 4;
     if (rw >= len * a.group || pieces == 1 || d0 >= D) return;
     const long long at = (((long long)b * a.heads + h) * a.row_slots + rw) * a.splits;
-    float m = -1e30f, l = 0.0f;
+    float m = NOTHING, l = 0.0f;
     for (int s = 0; s < pieces; s++) m = fmaxf(m, a.part_ml[2 * (at + s)]);
     f4 o = {0, 0, 0, 0};
 #pragma unroll 4
@@ -929,7 +936,7 @@ template <int D> __global__ __launch_bounds__(256) void kv_join(KvArgs a) {
     if ((int)rw >= len * a.group || pieces == 1) return;
     const int tid = threadIdx.x;
     const long long at = (((long long)b * a.heads + h) * a.row_slots + rw) * a.splits;
-    float m = -1e30f, l = 0.0f;
+    float m = NOTHING, l = 0.0f;
     if (tid < pieces) {
         m = a.part_ml[2 * (at + tid)];
         l = a.part_ml[2 * (at + tid) + 1];

@@ -1,0 +1,38 @@
+"""Calls of the key/value cache at the edges of what its documentation allows."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+from test_gpu_kv import DEV, Filled, gen, held, i32, kv, make, rounded, same  # noqa: E402,F401
+from test_gpu_kv_weights import check, filled  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("n", [1, 40, 3000])
+@pytest.mark.parametrize("size", [-1e25, -1e15, -30.0, 30.0, 1e15, 1e25])
+def test_scores_of_all_sizes(kv, bits, n, size):
+    """Scores of 1e8 to 1e33 of both signs.  Equal keys have equal scores, so the mean of the values is wanted: f16 weights
+    are off by 2^-11 of themselves, the matrix instructions cut 33 terms at 2^-18 or 2^-14 of a code's step times the largest
+    weight (n / 32 of them, and one for each wave and piece), sums are f32, the output has 8 bits: half a unit is 2^-8 (torch.finfo(bfloat16).eps / 2) of a value at most.  Then keys of which one has
+    the largest score by far: its values, exactly."""
+    g = gen(n)
+    key = torch.randn(1, 1, 1, 64, generator=g).abs() * 1e7
+    v = torch.randn(1, n, 1, 64, generator=g)
+    f = filled(kv, key.expand(1, n, 1, 64), v, bits)
+    q = ((0.5 + torch.rand(1, 1, 2, 64, generator=g)) * size).bfloat16()
+    got = f.cache.attention(q.to(DEV), i32(n), table=f.table).cpu().double()
+    x = f.v[0, :, 0]
+    want, mag = x.mean(0), x.abs().mean(0)
+    cut = 33 * (2.0 ** -18 if bits == 4 else 2.0 ** -14) * (n / 32 + 4 * (1 + n / 256)) * f.vs.max() / n
+    err = (2.0 ** -11 + (n + 80) * 2.0 ** -24) * mag + cut
+    assert bool(((got - want).abs() <= err + torch.finfo(torch.bfloat16).eps / 2 * (want.abs() + err)).all())
+    other = torch.full((n,), 1.0 if size > 0 else 1.5)
+    other[n // 3] = 1.5 if size > 0 else 1.0
+    f = filled(kv, key * other[None, :, None, None], v, bits)
+    assert torch.equal(torch.argmax(f.k[0, :, 0] @ q[0, 0].double().t(), 0), torch.full((2,), n // 3))
+    got = f.cache.attention(q.to(DEV), i32(n), table=f.table)
+    for h in range(2):
+        assert same(got[0, 0, h], f.v[0, n // 3, 0].to(torch.bfloat16))
