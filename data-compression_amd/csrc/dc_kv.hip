@@ -447,8 +447,8 @@ static __device__ __forceinline__ float log_sum(float m, float l) { return (m + 
 // 2^(x / 2): the references of waves and pieces may lie so far apart that only the product with what they refer to, taken
 // with the root twice, stays in f32's range
 static __device__ __forceinline__ float root_exp(float x) { return __builtin_amdgcn_exp2f(0.5f * x); }
-// 1 / l; NaN where it is NaN, or nothing of what a query sees is in the cache
-static __device__ __forceinline__ float inverse_sum(float l) { return l > 0.0f ? 1.0f / l : asf(0x7FC00000u); }
+// 1 / l; 0 where nothing of what a query sees is in the cache (a token that is has a p of 2^-100 or more), NaN where l is
+static __device__ __forceinline__ float inverse_sum(float l) { return l > 0.0f ? 1.0f / l : l; }
 
 // a lane's codes of a block: U words.  PAST (U = 4, an instruction takes whole cache lines): past the caches
 template <int U, bool PAST> static __device__ __forceinline__ void load_codes(const uint8_t* p, uint32_t* x) {

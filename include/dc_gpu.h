@@ -324,13 +324,13 @@ int dc_kv_read_device(const dc_kv_cache* cache, const dc_kv_batch* at, int dtype
 /* Attention over the cache as it is held: out = softmax(scale q k^T) v for queries [batch][tokens][q_heads][head_dim] (f16
  * or bf16; q_heads a multiple of the cache's heads, consecutive ones share a head).  causal: query token i sees positions
  * < start[b] - lens[b] + 1 + i, otherwise all start[b].  A query that sees nothing has output 0 and lse -inf.  Tokens in
- * pages outside the cache are left out, and a start[b] outside it is held at its bounds (status bit 0).  d_lse (f32
- * [batch][tokens][q_heads], may be NULL) receives the log of the softmax's sum.  max_context: no start[b] is expected above it (it
- * sizes the split along the cache; a longer one is still computed in full).  d_workspace: dc_kv_attention_workspace
- * bytes (16-byte aligned; NULL where that is 0), in use until the call's work is done: calls that may run at once need
- * one each.  Outputs must not overlap the inputs.  Scores are formed in f32 from queries and steps below 2^100.  A position's
- * softmax weight times the step of its values is held to 2^-11 of itself or 2^-29 of its query's largest, whichever is more;
- * positions that a query does not see have no part in that. */
+ * pages outside the cache are left out (a query that sees no others sees nothing), and a start[b] outside it is held at its
+ * bounds (status bit 0).  d_lse (f32 [batch][tokens][q_heads], may be NULL) receives the log of the softmax's sum.
+ * max_context: no start[b] is expected above it (it sizes the split along the cache; a longer one is still computed in
+ * full).  d_workspace: dc_kv_attention_workspace bytes (16-byte aligned; NULL where that is 0), in use until the call's work
+ * is done: calls that may run at once need one each.  Outputs must not overlap the inputs.  Scores are formed in f32 from
+ * queries and steps below 2^100.  A position's softmax weight times the step of its values is held to 2^-11 of itself or
+ * 2^-29 of its query's largest, whichever is more; positions that a query does not see have no part in that. */
 size_t dc_kv_attention_workspace(const dc_kv_cache* cache, int batch, int tokens, int q_heads, long long max_context);
 int dc_kv_attention_device(const dc_kv_cache* cache, const dc_kv_batch* at, int dtype, int q_heads, const void* d_q,
                            const long long* q_strides, float scale, int causal, long long max_context, void* d_out,

@@ -36,3 +36,18 @@ def test_scores_of_all_sizes(kv, bits, n, size):
     got = f.cache.attention(q.to(DEV), i32(n), table=f.table)
     for h in range(2):
         assert same(got[0, 0, h], f.v[0, n // 3, 0].to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("n,tokens", [(1, 1), (40, 1), (40, 7), (3000, 1), (3000, 5)])
+def test_nothing_in_the_cache(kv, n, tokens):
+    """Every page outside the cache: what is left out is not seen, so 0 and -inf; a sequence beside it is as it was."""
+    f = Filled(kv, 61, 2, n, 1, 64, 16, 4)
+    q = torch.randn(2, tokens, 2, 64, generator=gen(62)).half()
+    want = f.cache.attention(q.to(DEV), i32(n, n), table=f.table)
+    table = f.table.clone()
+    table[0] = torch.where(torch.arange(f.width, device=DEV) % 2 == 0, -1, 1 << 30)
+    lse = torch.zeros(2, tokens, 2, device=DEV)
+    got = f.cache.attention(q.to(DEV), i32(n, n), table=table, lse=lse)
+    assert kv.KVCache.status(reset=True) == 1
+    assert bool((got[0] == 0).all()) and bool((lse[0] == -math.inf).all())
+    assert same(got[1], want[1]) and bool(torch.isfinite(lse[1]).all())
