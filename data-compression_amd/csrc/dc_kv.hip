@@ -650,7 +650,7 @@ template <int D, int BITS, int NT, bool PAST> __global__ __launch_bounds__(256) 
     constexpr int N = D / 16, U = N * BITS / 8, ROW = 16 * U, KS = D / 32, COLS = 16 * NT;
     constexpr bool ALL = D * NT <= 256;                     // every wave its own sums in LDS, or one after the other
     __shared__ float acc_lds[(ALL ? 4 : 1) * N * 16 * COLS];
-    __shared__ float ml[3][4][COLS];
+    __shared__ float ml[2][4][COLS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
     // Workgroup -> (piece, sequence, head, tile of query rows), the tile fastest: workgroups go round the 8 XCDs one by
@@ -820,7 +820,8 @@ template <int D, int BITS, int NT, bool PAST> __global__ __launch_bounds__(256) 
         t0 += 128;
     }
 
-    // the four waves' sums, in a fixed order
+    // the four waves' sums, in a fixed order; each divided by their common sum of weights first, as without that they pass
+    // f32's range where values come near to it
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
         L[nt] = over_groups_sum(L[nt]);
@@ -828,16 +829,24 @@ template <int D, int BITS, int NT, bool PAST> __global__ __launch_bounds__(256) 
         if (g == 0) {
             ml[0][wave][nt * 16 + col] = M[nt];
             ml[1][wave][nt * 16 + col] = L[nt];
-            ml[2][wave][nt * 16 + col] = Z[nt] * (R * 0.0078125f);
         }
     }
     __syncthreads();
+    auto sums = [&](int c, float& m, float& l) {            // a column's reference and sum of weights
+        m = ml[0][0][c];
+        l = 0.0f;
+        for (int v = 1; v < 4; v++) m = fmaxf(m, ml[0][v][c]);
+        for (int v = 0; v < 4; v++) {
+            const float sc = root_exp(ml[0][v][c] - m);
+            l = fmaf(ml[1][v][c] * sc, sc, l);
+        }
+    };
     float f[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-        float m = ml[0][0][nt * 16 + col];
-        for (int v = 1; v < 4; v++) m = fmaxf(m, ml[0][v][nt * 16 + col]);
-        f[nt] = root_exp(M[nt] - m) * (R * 0.0078125f) * root_exp(M[nt] - m) * UNIT<BITS>;
+        float m, l;
+        sums(nt * 16 + col, m, l);
+        f[nt] = root_exp(M[nt] - m) * (R * 0.0078125f) * (root_exp(M[nt] - m) * inverse_sum(l));
     }
     for (int v = 0; v < (ALL ? 1 : 4); v++) {
         if (ALL || wave == v)
@@ -848,7 +857,7 @@ template <int D, int BITS, int NT, bool PAST> __global__ __launch_bounds__(256) 
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
                         float* p = &acc_lds[(((ALL ? wave : 0) * NT + nt) * N + i) * 256 + (g * 4 + r) * 16 + col];
-                        const float y = acc[nt][i][r] * f[nt];
+                        const float y = fmaf(acc[nt][i][r], UNIT<BITS>, Z[nt]) * f[nt];
                         *p = ALL || v == 0 ? y : *p + y;
                     }
         __syncthreads();
@@ -858,21 +867,16 @@ template <int D, int BITS, int NT, bool PAST> __global__ __launch_bounds__(256) 
     for (int nt = 0; nt < NT; nt++) {
         const int rw = row0 + nt * 16 + oc;
         if (rw >= rows) continue;
-        float m = ml[0][0][nt * 16 + oc], l = 0.0f, z = 0.0f;
-        for (int v = 1; v < 4; v++) m = fmaxf(m, ml[0][v][nt * 16 + oc]);
-        for (int v = 0; v < 4; v++) {
-            const float sc = root_exp(ml[0][v][nt * 16 + oc] - m);
-            l = fmaf(ml[1][v][nt * 16 + oc] * sc, sc, l);
-            z = fmaf(ml[2][v][nt * 16 + oc] * sc, sc, z);
-        }
         float o[N];
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            float y = z;
+            float y = 0.0f;
             for (int v = 0; v < (ALL ? 4 : 1); v++) y += acc_lds[((v * NT + nt) * N + i) * 256 + ou * 16 + oc];
             o[i] = y;
         }
-        if (pieces > 1) {                                   // unnormalised, with its maximum and sum
+        float m = 0.0f, l = 0.0f;
+        if (ou == 0) sums(nt * 16 + oc, m, l);
+        if (pieces > 1) {                                   // with its reference and sum
             const long long at = ((((long long)b * a.heads + h) * a.row_slots + rw) * a.splits + split);
             float* p = a.part + at * D + ou * N;
             for (int k = 0; k < N; k++) p[k] = o[k];
@@ -883,9 +887,8 @@ template <int D, int BITS, int NT, bool PAST> __global__ __launch_bounds__(256) 
             continue;
         }
         const bool none = (a.causal ? context - len + 1 + (int)div_by((uint32_t)rw, a.group_inv) : context) <= 0;
-        const float inv = inverse_sum(l);
-#pragma unroll
-        for (int k = 0; k < N; k++) o[k] = none ? 0.0f : o[k] * inv;
+        if (none)
+            for (int k = 0; k < N; k++) o[k] = 0.0f;
         put<N>(a, b, h, rw, ou * N, o, none ? -INFINITY : log_sum(m, l));
     }
 }
@@ -906,18 +909,21 @@ template <int D> __global__ __launch_bounds__(256) void kv_join_few(KvArgs a) {
     const long long at = (((long long)b * a.heads + h) * a.row_slots + rw) * a.splits;
     float m = NOTHING, l = 0.0f;
     for (int s = 0; s < pieces; s++) m = fmaxf(m, a.part_ml[2 * (at + s)]);
+    for (int s = 0; s < pieces; s++) {
+        const float f = root_exp(a.part_ml[2 * (at + s)] - m);
+        l = fmaf(a.part_ml[2 * (at + s) + 1] * f, f, l);
+    }
+    const float inv = inverse_sum(l);
     f4 o = {0, 0, 0, 0};
 #pragma unroll 4
     for (int s = 0; s < pieces; s++) {
         const float f = root_exp(a.part_ml[2 * (at + s)] - m);
-        l = fmaf(a.part_ml[2 * (at + s) + 1] * f, f, l);
-        o += *(const f4*)(a.part + (at + s) * D + d0) * f * f;
+        o += *(const f4*)(a.part + (at + s) * D + d0) * (a.part_ml[2 * (at + s) + 1] * f * f * inv);
     }
     const bool none = (a.causal ? context - len + 1 + (int)div_by((uint32_t)rw, a.group_inv) : context) <= 0;
-    const float inv = none ? 0.0f : inverse_sum(l);
     float y[4];
 #pragma unroll
-    for (int k = 0; k < 4; k++) y[k] = none ? 0.0f : o[k] * inv;
+    for (int k = 0; k < 4; k++) y[k] = none ? 0.0f : o[k];
     put<4>(a, b, h, rw, d0, y, none ? -INFINITY : log_sum(m, l));
 }
 
@@ -946,25 +952,26 @@ template <int D> __global__ __launch_bounds__(256) void kv_join(KvArgs a) {
     if ((tid & 63) == 0) red[0][tid >> 6] = top;
     __syncthreads();
     top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-    const float scale = root_exp(m - top);
-    f[tid] = scale;
-    l = l * scale * scale;
+    const float scale = root_exp(m - top), own = l * scale * scale;
+    l = own;
     for (int k = 32; k; k >>= 1) l += __shfl_xor(l, k);
     if ((tid & 63) == 0) red[1][tid >> 6] = l;
     __syncthreads();
     l = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+    f[tid] = own * inverse_sum(l);
+    __syncthreads();
     const int dl = tid & 7, sl = tid >> 3;
     f4 o = {0, 0, 0, 0};
     const float* p = a.part + at * D + d0 + dl * 4;
 #pragma unroll 4
-    for (int s = sl; s < pieces; s += 32) o += *(const f4*)(p + (long long)s * D) * f[s] * f[s];
+    for (int s = sl; s < pieces; s += 32) o += *(const f4*)(p + (long long)s * D) * f[s];
     sums[sl][dl] = o;
     __syncthreads();
     if (tid < 32) {
         float y = 0.0f;
         for (int k = 0; k < 32; k++) y += ((const float*)&sums[k][0])[tid];
         const bool none = (a.causal ? context - len + 1 + (int)div_by(rw, a.group_inv) : context) <= 0;
-        y = none ? 0.0f : y * inverse_sum(l);
+        if (none) y = 0.0f;
         put<1>(a, b, h, (int)rw, (int)d0 + tid, &y, none ? -INFINITY : log_sum(top, l));
     }
 }

@@ -51,3 +51,20 @@ def test_nothing_in_the_cache(kv, n, tokens):
     assert kv.KVCache.status(reset=True) == 1
     assert bool((got[0] == 0).all()) and bool((lse[0] == -math.inf).all())
     assert same(got[1], want[1]) and bool(torch.isfinite(lse[1]).all())
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("n,tokens", [(1, 1), (40, 1), (40, 9), (3000, 1), (3000, 3), (5000, 1)])
+def test_values_of_all_sizes(kv, bits, n, tokens):
+    """Values up to 1e38, of one sign or of both: sums without their division would pass f32's range."""
+    g = gen(n)
+    k, v = (torch.randn(1, n, 2, 64, generator=g) for _ in range(2))
+    v = v / v.abs().max() * 1e38
+    v[:, :, 1] = v[:, :, 1].abs()
+    q = torch.randn(1, tokens, 4, 64, generator=g).bfloat16()
+    check(filled(kv, k, v, bits), q, [n])
+    if n == 1:
+        v[0, 0, 0, 0], v[0, 0, 0, 1] = 3e38, -3e38                    # (a row that spans more than f32's largest number)
+        f = filled(kv, k, v, bits)
+        got = f.cache.attention(q.to(DEV), i32(1), table=f.table)
+        assert same(got[0, 0, :2], f.v[0, 0, :1].to(torch.bfloat16).expand(2, 64))
