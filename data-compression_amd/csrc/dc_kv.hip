@@ -463,7 +463,7 @@ template <bool PAST, int U> static __device__ __forceinline__ void load_values(S
 #pragma unroll
     for (int j = 0; j < 2; j++) load_codes<U, PAST>(at.codes[j] + to_values + lane_codes, c.v[j]);
 }
-template <int U> static __device__ __forceinline__ void load_words(Stage<U>& c, const Where& at, uint32_t to_values, bool second, uint32_t lane_words) {
+template <int U> static __device__ __forceinline__ void load_words(Stage<U>& c, const Where& at, uint64_t to_values, bool second, uint32_t lane_words) {
     const uint8_t* p = (second ? at.words[1] : at.words[0]) + lane_words;
     c.kw = *(const uint32_t*)p;
     c.vw = *(const uint32_t*)(p + to_values);
@@ -525,7 +525,7 @@ template <int D, int BITS, int NT, bool PAST, bool EDGE>
 static __device__ __forceinline__ void attend(Stage<D * BITS / 128>& c, const Frag (*q)[D / 32], const float* qsum,
                                               const float* unit, float significand, const int* sees, int t0, int most, int g,
                                               const bool* hole, const Where& next, uint64_t codes_to_values,
-                                              uint32_t words_to_values, uint32_t lane_codes, bool second, uint32_t lane_words,
+                                              uint64_t words_to_values, uint32_t lane_codes, bool second, uint32_t lane_words,
                                               f4 (*acc)[D / 16], float* M, float* L, float* Z, float& R) {
     constexpr int N = D / 16, U = N * BITS / 8, KS = D / 32;
     // the lane's token's words.  (Behind the last position that is seen there may be anything)
@@ -703,7 +703,7 @@ template <int D, int BITS, int NT, bool PAST> __global__ __launch_bounds__(256) 
     const uint32_t lane_codes = (uint32_t)(col * ROW + g * (4 * U)), lane_words = (uint32_t)(g * 4 + (lane & 3)) * 4;
     const bool second = lane & 4;
     const uint64_t codes_to_values = (uint64_t)a.page * ROW;
-    const uint32_t words_to_values = 4u * (uint32_t)a.page;
+    const uint64_t words_to_values = 4ull * (uint32_t)a.page;
     int page[2];
     uint32_t place[2];
     auto find = [&](int t) {                                // (the second block may lie past the end: then the first again)

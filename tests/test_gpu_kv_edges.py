@@ -68,3 +68,22 @@ def test_values_of_all_sizes(kv, bits, n, tokens):
         f = filled(kv, k, v, bits)
         got = f.cache.attention(q.to(DEV), i32(1), table=f.table)
         assert same(got[0, 0, :2], f.v[0, 0, :1].to(torch.bfloat16).expand(2, 64))
+
+
+def test_one_page_of_all_positions(kv):
+    """Pages of 2^30 tokens (43 GB in 4 bits): the values' words lie 2^32 bytes behind the keys'."""
+    P, D = 1 << 30, 32
+    room = torch.empty(kv.KVCache.page_bytes(P, 1, D, 4), dtype=torch.uint8, device=DEV)
+    c = kv.KVCache(1, P, 1, D, bits=4, buffer=room)
+    g = gen(3)
+    k, v = torch.randn(1, 40, 1, D, generator=g), torch.randn(1, 40, 1, D, generator=g) * 100
+    for first in (0, P - 40):
+        c.write(k.to(DEV), v.to(DEV), i32(first))
+        got = c.read(i32(first), 40, dtype=torch.float32)
+        assert same(got[0], held(k, 4)[0].float()) and same(got[1], held(v, 4)[0].float())
+    f = Filled.__new__(Filled)
+    f.cache, f.table = c, None
+    f.k, f.ks, f.kz, f.kc = held(k, 4)
+    f.v, f.vs, f.vz, f.vc = held(v, 4)
+    for tokens in (1, 40):
+        check(f, torch.randn(1, tokens, 2, D, generator=g).half(), [40], max_context=40)
