@@ -195,9 +195,12 @@ int dc_kv_attention_device(const dc_kv_cache* cache, const dc_kv_batch* at, int 
        16 of 16384, 0.29 GB: 58, so 53; 2 of 65536, 0.14 GB: 34, so 37) */
     const long long longest = max_context < a.capacity ? max_context : a.capacity;
     a.past = 1.0 * at->batch * longest * a.head_bytes / a.page * a.heads > 256e6;
-    const unsigned piece = low_bit((unsigned)(cache->head_dim / 16 * 2));
+    /* outputs are stored by units of head_dim / 16 values, and by the join of few pieces four values at once */
+    unsigned piece = low_bit((unsigned)(cache->head_dim / 16 * 2));
+    if (piece > 16) piece = 16;
+    if (piece < 8 && a.splits > 1 && a.splits <= DC_KV_JOIN_FEW) piece = 8;
     a.vec = fits(d_q, q_strides, 2, 16);
-    a.vec_out = fits(d_out, out_strides, 2, piece > 16 ? 16 : piece);
+    a.vec_out = fits(d_out, out_strides, 2, piece);
     a.causal = causal != 0;
     a.scale = scale;
     a.lse = d_lse;

@@ -1012,7 +1012,7 @@ template <int D, int BITS> int go_attention(const KvArgs& a, hipStream_t st) {
         else kv_attention<D, BITS, 1, false><<<grid, 256, 0, st>>>(a);
     } else kv_attention<D, BITS, 1, false><<<grid, 256, 0, st>>>(a);
     constexpr int ROWS = D <= 128 ? 8 : 4;                  // (kv_join_few)
-    if (a.splits > 16) kv_join<D><<<(unsigned)((long long)a.row_slots * a.heads * a.batch * (D / 32)), 256, 0, st>>>(a);
+    if (a.splits > dc::DC_KV_JOIN_FEW) kv_join<D><<<(unsigned)((long long)a.row_slots * a.heads * a.batch * (D / 32)), 256, 0, st>>>(a);
     else if (a.splits > 1)
         kv_join_few<D><<<(unsigned)((long long)((a.row_slots + ROWS - 1) / ROWS) * a.heads * a.batch), 256, 0, st>>>(a);
     return hipGetLastError() != hipSuccess;

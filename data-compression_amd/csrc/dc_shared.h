@@ -104,6 +104,7 @@ typedef struct Dec3Bufs {
                                       (zero between launches: the launch's last wave resets them) */
 } Dec3Bufs;
 
+enum { DC_KV_JOIN_FEW = 16 };     /* up to so many pieces of a sequence are joined one after the other */
 /* key/value cache operators (dc_kv.hip): one struct for the write, the read and the attention */
 typedef struct KvArgs {
     uint8_t* data;                 /* the cache */

@@ -1,0 +1,60 @@
+/* Stands in for the GPU side of dc_host_lowbit.c: the launches are recorded instead of made, HIP says what the test sets.
+ * Linked with that file into a library for tests/test_lowbit_host.py. */
+#define __HIP_PLATFORM_AMD__ 1
+#include <hip/hip_runtime_api.h>
+#include <string.h>
+
+#include "../../data-compression_amd/csrc/dc_shared.h"
+#include "../../include/dc_gpu.h"
+
+static KvArgs last_kv;
+static ActArgs last_act;
+static int launches;
+static unsigned word;
+static char message[256];
+
+int dc_init(int device) { (void)device; return DC_OK; }
+unsigned* dc_kv_status_word(void) { return &word; }
+int dc_set_error(int code, const char* msg) {
+    strncpy(message, msg, sizeof message - 1);
+    return code;
+}
+int dc_kv_wide_cols(int dim) { return dim <= 160 ? 32 : 16; }
+int dc_launch_kv_rows(const KvArgs* a, int write, dc_hip_stream st) {
+    (void)write; (void)st;
+    last_kv = *a;
+    launches++;
+    return 0;
+}
+int dc_launch_kv_attention(const KvArgs* a, dc_hip_stream st) { return dc_launch_kv_rows(a, 0, st); }
+int dc_launch_act(const ActArgs* a, int back, dc_hip_stream st) {
+    (void)back; (void)st;
+    last_act = *a;
+    launches++;
+    return 0;
+}
+hipError_t hipStreamIsCapturing(hipStream_t st, hipStreamCaptureStatus* s) {
+    (void)st;
+    *s = hipStreamCaptureStatusNone;
+    return hipSuccess;
+}
+hipError_t hipMemcpyAsync(void* d, const void* s, size_t n, hipMemcpyKind k, hipStream_t st) {
+    (void)k; (void)st;
+    memcpy(d, s, n);
+    return hipSuccess;
+}
+hipError_t hipMemsetAsync(void* d, int v, size_t n, hipStream_t st) {
+    (void)st;
+    memset(d, v, n);
+    return hipSuccess;
+}
+hipError_t hipStreamSynchronize(hipStream_t st) { (void)st; return hipSuccess; }
+
+/* for the test */
+int stub_launches(void) { return launches; }
+const char* stub_message(void) { return message; }
+int stub_vec(void) { return last_kv.vec; }
+int stub_vec_out(void) { return last_kv.vec_out; }
+unsigned stub_splits(void) { return last_kv.splits; }
+long long stub_rows(void) { return last_kv.rows; }
+int stub_act_mode(void) { return last_act.mode; }

@@ -87,3 +87,19 @@ def test_one_page_of_all_positions(kv):
     f.v, f.vs, f.vz, f.vc = held(v, 4)
     for tokens in (1, 40):
         check(f, torch.randn(1, tokens, 2, D, generator=g).half(), [40], max_context=40)
+
+
+@pytest.mark.parametrize("dim", [32, 64, 96, 160, 224])
+@pytest.mark.parametrize("n", [900, 3000, 20000])
+@pytest.mark.parametrize("off", [2, 4, 8])
+def test_joined_outputs_off_their_alignment(kv, dim, n, off):
+    """Pieces joined into heads that start anywhere: as into a new tensor, and nothing beside them is written."""
+    f = Filled(kv, dim + n, 1, n, 1, dim, 16, 4)
+    q = torch.randn(1, 3, 2, dim, generator=gen(dim)).bfloat16()
+    want = check(f, q, [n])
+    room = torch.full((1, 3, 2, dim + 8), -3.0, dtype=torch.bfloat16, device=DEV)
+    out = room[..., off // 2:off // 2 + dim]
+    f.cache.attention(q.to(DEV), i32(n), table=f.table, out=out)
+    assert same(out, want)
+    out.fill_(-3.0)
+    assert bool((room == -3).all())

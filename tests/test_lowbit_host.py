@@ -1,0 +1,52 @@
+"""The host side of the fixed-rate operators (csrc/dc_host_lowbit.c) with recorded launches in place of the GPU's: what is
+chosen for a call, and what is refused before it."""
+import ctypes as C
+import os
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+P, ARG = 0x10000, -2
+
+
+@pytest.fixture(scope="module")
+def host(tmp_path_factory):
+    so = str(tmp_path_factory.mktemp("lowbit") / "host.so")
+    subprocess.check_call(["gcc", "-O1", "-Wall", "-shared", "-fPIC", "-I/opt/rocm/include", "-o", so,
+                           os.path.join(ROOT, "tests", "native", "lowbit_host_stubs.c"),
+                           os.path.join(ROOT, "data-compression_amd", "csrc", "dc_host_lowbit.c")])
+    L = C.CDLL(so)
+    vp, ll = C.c_void_p, C.c_longlong
+    import dcamd
+    kvc, kvb, strides = C.POINTER(dcamd.KvCacheDesc), C.POINTER(dcamd.KvBatchDesc), C.POINTER(ll)
+    L.dc_kv_write_device.argtypes = L.dc_kv_read_device.argtypes = [kvc, kvb, C.c_int, vp, strides, vp, strides, vp]
+    L.dc_kv_attention_device.argtypes = [kvc, kvb, C.c_int, C.c_int, vp, strides, C.c_float, C.c_int, ll, vp, strides, vp, vp, C.c_size_t, vp]
+    L.dc_kv_attention_workspace.argtypes = [kvc, C.c_int, C.c_int, C.c_int, ll]
+    L.dc_kv_attention_workspace.restype = C.c_size_t
+    L.dc_act_forward_device.argtypes = [C.c_int, C.c_int, ll, ll, vp, ll, vp, ll, vp, ll, vp, vp, vp]
+    L.stub_message.restype = C.c_char_p
+    L.stub_rows.restype = ll
+    L.desc, L.at = dcamd.KvCacheDesc, dcamd.KvBatchDesc
+    return L
+
+
+def three(*v):
+    return (C.c_longlong * 3)(*v)
+
+
+@pytest.mark.parametrize("dim", range(32, 257, 32))
+@pytest.mark.parametrize("context", [100, 3000, 1 << 20])
+def test_whole_stores_of_outputs(host, dim, context):
+    """Whole-lane stores only where the output's base and strides allow the widest: a unit's dim / 16 values by the attention
+    (in the largest power of two that divides them, at most 16 bytes), four values, 8 bytes, by the join of up to 16
+    pieces."""
+    cache, at = host.desc(P, 2, 1 << 20, 4, dim, 4), host.at(2, 1, P, None, None, 0, 0, 0)
+    width = dim // 16 * 2
+    piece = min(width & -width, 16)
+    for off in (0, 2, 4, 8, 16):
+        for pad in (0, 1, 2, 4, 8):
+            st = three(8 * (dim + pad), 8 * (dim + pad), dim + pad)
+            assert host.dc_kv_attention_device(cache, at, 1, 8, P, st, 1.0, 1, context, P + off, st, None, P, 1 << 40, None) == 0, host.stub_message()
+            need = max(piece, 8) if 1 < host.stub_splits() <= 16 else piece
+            assert host.stub_vec_out() == (off % need == 0 and pad * 2 % need == 0), (off, pad, host.stub_splits())
