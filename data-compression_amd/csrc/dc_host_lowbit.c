@@ -17,6 +17,10 @@ unsigned* dc_kv_status_word(void);
 
 #define REFUSE(msg) return dc_set_error(DC_ERR_ARG, msg)
 
+/* a launch has fewer than 2^32 threads, here in workgroups of 256 */
+enum { MOST_GROUPS = (1 << 24) - 1 };
+#define MOST_ACT (2048ll * MOST_GROUPS)
+
 /* the high half of n times this is n / d where n d < 2^64 (2^64 / d, rounded up); 0 stands for d = 1 */
 static unsigned long long inverse(unsigned long long d) { return d <= 1 ? 0 : ~0ull / d + 1; }
 
@@ -90,6 +94,7 @@ static int rows_call(const dc_kv_cache* c, const dc_kv_batch* at, int dtype, con
     a.blocks = (int)(((long long)at->tokens + 30) / 16);        /* at any place within the first block */
     a.tokens_inv = inverse((unsigned long long)a.blocks);
     a.rows = (long long)at->batch * a.blocks * c->heads * (write ? 2 : 1);
+    if ((a.rows + 3) / 4 > MOST_GROUPS) REFUSE("cache: too many rows in one call");
     a.k = k;
     a.v = v;
     memcpy(a.ks, ks, sizeof a.ks);
@@ -180,8 +185,8 @@ int dc_kv_attention_device(const dc_kv_cache* cache, const dc_kv_batch* at, int 
     if (((uintptr_t)d_q | (uintptr_t)d_out) & 1u || (uintptr_t)d_lse & 3u)
         REFUSE("attention: queries, output and lse are aligned to their types");
     if (plan(cache, at->batch, at->tokens, q_heads, max_context, &a)) REFUSE("attention: too many query rows in one call");
-    if ((long long)a.splits * a.tiles * a.heads * a.batch > (1ll << 31) - 1 ||
-        (a.splits > 1 && (long long)a.row_slots * a.heads * a.batch * 8 > (1ll << 31) - 1))
+    if ((long long)a.splits * a.tiles * a.heads * a.batch > MOST_GROUPS ||
+        (a.splits > 1 && (long long)a.row_slots * a.heads * a.batch * 8 > MOST_GROUPS))
         REFUSE("attention: too many query rows in one call");
     const size_t need = workspace_of(&a, at->batch);
     if (need && (!d_workspace || workspace_bytes < need || ((uintptr_t)d_workspace & 15u)))
@@ -227,7 +232,7 @@ int dc_kv_status(void* stream, unsigned* status_out, int reset) {
 }
 
 /* ---- activation checkpoints ------------------------------------------------------------------------------ */
-size_t dc_act_bytes(long long n) { return n < 0 || n >= (1ll << 35) ? 0 : (size_t)((n + 31) / 32) * 33u; }
+size_t dc_act_bytes(long long n) { return n < 0 || n > MOST_ACT ? 0 : (size_t)((n + 31) / 32) * 33u; }
 
 /* one array of the call: 0 flat and aligned, 1 rows apart in whole 8s and aligned, 2 neither */
 static int shape_of(const void* p, long long ld, long long rows, long long cols, int size) {
@@ -241,7 +246,7 @@ static int act_call(ActArgs* a, int back, void* stream) {
     const int size = size_of(a->dtype);
     if (!size) REFUSE("activation: dtype is DC_F32, DC_F16 or DC_BF16");
     if (a->kind != DC_ACT_NONE && a->kind != DC_ACT_SILU && a->kind != DC_ACT_GELU) REFUSE("activation: unknown kind");
-    if (a->rows < 0 || a->cols < 0 || (a->cols && a->rows > ((1ll << 35) - 1) / a->cols)) REFUSE("activation: fewer than 2^35 values");
+    if (a->rows < 0 || a->cols < 0 || (a->cols && a->rows > MOST_ACT / a->cols)) REFUSE("activation: at most 2^35 - 2048 values");
     if (a->rows == 0 || a->cols == 0) return DC_OK;
     const int works = a->kind != DC_ACT_NONE;
     if (!a->kept || (a->gated && !a->kept_up)) REFUSE("activation: a checkpoint is missing");

@@ -314,7 +314,8 @@ typedef struct dc_kv_batch {
 size_t dc_kv_page_bytes(int page_size, int heads, int head_dim, int bits);
 /* Quantise keys and values [batch][tokens][heads][head_dim] (strides of batch, token and head in elements; the head's
  * values are consecutive) into the cache.  No two tokens of one call may have the same place (that place then holds a
- * mix).  Tokens at a position or in a page outside the cache are dropped (status bit 0). */
+ * mix).  Tokens at a position or in a page outside the cache are dropped (status bit 0).  batch x heads x (tokens + 30) / 16 is
+ * below 2^25 (a read: 2^26; attention: batch x query rows / 16 below 2^24). */
 int dc_kv_write_device(const dc_kv_cache* cache, const dc_kv_batch* at, int dtype, const void* d_k,
                        const long long* k_strides, const void* d_v, const long long* v_strides, void* stream);
 /* Read them back (rounded to dtype, held at its largest finite value).  Positions and pages outside the cache read as
@@ -342,7 +343,8 @@ int dc_kv_status(void* stream, unsigned* status_out, int reset);
 
 /* Activation checkpoints: rows x cols values, groups of 32 consecutive ones (in the order of the rows) share a power of
  * two 2^k, the smallest with amax <= 127.5 * 2^k and k >= -126; code = rint(x / 2^k) held to [-127, 127], so |x - x^| <=
- * 2^(k-1).  A value that is not finite comes back as NaN.  Bytes of a checkpoint of n values (n < 2^35): */
+ * 2^(k-1).  A value that is not finite comes back as NaN.  Bytes of a checkpoint of n values
+ * (n <= 2^35 - 2048): */
 enum { DC_ACT_NONE = 0, DC_ACT_SILU = 1, DC_ACT_GELU = 2 };
 size_t dc_act_bytes(long long n);
 /* y = f(x) (d_up NULL) or f(x) up, and the checkpoints of x (and up); kind DC_ACT_NONE: the checkpoint alone (d_up and d_y

@@ -50,3 +50,25 @@ def test_whole_stores_of_outputs(host, dim, context):
             assert host.dc_kv_attention_device(cache, at, 1, 8, P, st, 1.0, 1, context, P + off, st, None, P, 1 << 40, None) == 0, host.stub_message()
             need = max(piece, 8) if 1 < host.stub_splits() <= 16 else piece
             assert host.stub_vec_out() == (off % need == 0 and pad * 2 % need == 0), (off, pad, host.stub_splits())
+
+
+def test_calls_of_most_rows(host):
+    """A launch has fewer than 2^32 threads: larger calls are refused before it, as an argument that is wrong."""
+    st = three(64, 64, 64)
+    for f, most in ((host.dc_kv_write_device, (1 << 25) - 2), (host.dc_kv_read_device, (1 << 26) - 4)):
+        for rows, rc in ((most, 0), (most + 1, ARG), (1 << 28, ARG)):
+            before = host.stub_launches()                              # (batches of one token: a block of 16 and head each)
+            assert f(host.desc(P, 1 << 40, 16, 1, 32, 4), host.at(rows, 1, P, None, P, 1, 1, 0), 1, P, st, P, st, None) == rc, rows
+            assert host.stub_launches() == before + (rc == 0)
+    for batch, rc in (((1 << 24) - 1, 0), (1 << 24, ARG), (1 << 29, ARG)):
+        before = host.stub_launches()
+        assert host.dc_kv_attention_device(host.desc(P, 1 << 40, 16, 1, 32, 4), host.at(batch, 1, P, None, P, 1, 1, 0), 1, 1, P, st, 1.0, 1, 16, P, st,
+                                           None, None, 0, None) == rc, batch
+        assert host.stub_launches() == before + (rc == 0)
+    most = (1 << 35) - 2048
+    for rows, cols, rc in ((1, most, 0), (most, 1, 0), (1, most + 1, ARG), (most // 8 + 1, 8, ARG), ((1 << 35) - 1, 1, ARG)):
+        before = host.stub_launches()
+        assert host.dc_act_forward_device(1, 1, rows, cols, P, cols, None, 0, P, cols, P, None, None) == rc, (rows, cols)
+        assert host.stub_launches() == before + (rc == 0)
+    host.dc_act_bytes.restype, host.dc_act_bytes.argtypes = C.c_size_t, [C.c_longlong]
+    assert host.dc_act_bytes(most) == most // 32 * 33 and host.dc_act_bytes(most + 1) == 0
