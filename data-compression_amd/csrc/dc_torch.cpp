@@ -49,22 +49,24 @@ bool known(const Tensor& t) {
     return false;
 }
 
-// all tensors on the library's device, and that the current one (the library starts on the first call's device)
+// all tensors on one GPU, the library's and the current one.  The library starts on the first call's device, which has to be the
+// current one before it does, as starting makes it that
 bool on_gpu(std::initializer_list<const Tensor*> ts) {
-    const Tensor* first = *ts.begin();
     int dev = dc_get_device();
-    if (dev < 0 && first->is_cuda()) {
-        if (dc_init(first->get_device())) {
+    const bool starts = dev < 0;
+    if (starts && (*ts.begin())->is_cuda()) dev = c10::hip::current_device();
+    for (const Tensor* t : ts)
+        if (t && (!t->is_cuda() || t->get_device() != dev)) {
+            PyErr_SetString(PyExc_ValueError, starts ? "tensors must lie on the GPU, on the current device" : "tensors must lie on the GPU, on the library's device");
+            return false;
+        }
+    if (starts) {
+        if (dc_init(dev)) {
             PyErr_Format(g_error, "dc_init: %s", dc_last_error());
             return false;
         }
-        dev = dc_get_device();
+        dev = dc_get_device();                              // (another thread may have been first)
     }
-    for (const Tensor* t : ts)
-        if (t && (!t->is_cuda() || t->get_device() != dev)) {
-            PyErr_SetString(PyExc_ValueError, "tensors must lie on the GPU, on the library's device");
-            return false;
-        }
     if (c10::hip::current_device() != dev) {
         PyErr_Format(PyExc_ValueError, "the current device must be the library's (cuda:%d)", dev);
         return false;
