@@ -7,6 +7,7 @@
 
 #include <ATen/ops/empty.h>
 #include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 
 #include "../../include/dc_gpu.h"
@@ -50,7 +51,7 @@ bool known(const Tensor& t) {
 }
 
 // all tensors on one GPU, the library's and the current one.  The library starts on the first call's device, which has to be the
-// current one before it does, as starting makes it that
+// current one before it does, as starting makes it that; and not in a capture, as starting allocates
 bool on_gpu(std::initializer_list<const Tensor*> ts) {
     int dev = dc_get_device();
     const bool starts = dev < 0;
@@ -61,6 +62,10 @@ bool on_gpu(std::initializer_list<const Tensor*> ts) {
             return false;
         }
     if (starts) {
+        if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None) {
+            PyErr_SetString(PyExc_ValueError, "the library's first call cannot be captured: make one before");
+            return false;
+        }
         if (dc_init(dev)) {
             PyErr_Format(g_error, "dc_init: %s", dc_last_error());
             return false;

@@ -30,6 +30,15 @@ if case == "device":                # a tensor of a device that is not the curre
         x = torch.empty(4, 8, device="cuda:1")
     refused(lambda: dcamd.act_forward(x, "silu"), "current device")
     assert torch.cuda.current_device() == 0
+elif case == "capture":
+    x = torch.ones(4, 8, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = x + 1
+        refused(lambda: dcamd.act_forward(x, "silu"), "captured")
+    graph.replay()
+    torch.cuda.synchronize()
+    assert float(y.sum()) == 64
 want = torch.nn.functional.silu(torch.ones(4, 8))
 got, _ = dcamd.act_forward(torch.ones(4, 8, device="cuda"), "silu")
 assert torch.allclose(got.cpu(), want) and started() == 0
