@@ -388,6 +388,7 @@ PyObject* kv_status(PyObject*, PyObject* const* args, Py_ssize_t count) {
     ARGS(1);
     unsigned word = 0;
     const int reset = PyObject_IsTrue(args[0]);
+    if (dc_get_device() < 0) return PyLong_FromLong(0);     // (nothing has run)
     void* stream = stream_of();
     int rc;
     Py_BEGIN_ALLOW_THREADS

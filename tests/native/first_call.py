@@ -30,6 +30,8 @@ if case == "device":                # a tensor of a device that is not the curre
         x = torch.empty(4, 8, device="cuda:1")
     refused(lambda: dcamd.act_forward(x, "silu"), "current device")
     assert torch.cuda.current_device() == 0
+elif case == "status":              # a status before any call: nothing has run
+    assert dcamd.KVCache.status() == 0 and started() == -1
 elif case == "capture":
     x = torch.ones(4, 8, device="cuda")
     graph = torch.cuda.CUDAGraph()
