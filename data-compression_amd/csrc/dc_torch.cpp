@@ -141,7 +141,9 @@ bool positions_of(const dc_kv_cache& c, int64_t batch, int64_t tokens, const Ten
     const dc_kv_cache& c = *(const dc_kv_cache*)PyLong_AsVoidPtr(args[0]); \
     if (PyErr_Occurred()) return nullptr; \
     TENSOR(1, buffer, false); \
-    if (buffer->data_ptr() != c.data) REFUSE("buffer: the one the cache was made with is needed")
+    if (buffer->data_ptr() != c.data || !buffer->is_contiguous() || \
+        buffer->nbytes() < (size_t)c.pages * dc_kv_page_bytes(c.page_size, c.heads, c.head_dim, c.bits)) \
+        REFUSE("buffer: the one the cache was made with is needed")
 
 // write(cache, buffer, k, v, start, table, lens)
 PyObject* kv_write(PyObject*, PyObject* const* args, Py_ssize_t count) {
