@@ -6,6 +6,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ops/empty.h>
+#include <algorithm>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
@@ -84,6 +85,30 @@ PyObject* failed(const char* what, int rc) {
     return nullptr;
 }
 
+// whether two places of a tensor, or of two tensors of these sizes and strides `apart` elements apart, are the same one.  The
+// dimensions, ordered by their strides, have to lie within one another (else true: such layouts are not taken)
+bool nested(const Tensor& x, int (&order)[4]) {
+    int n = 0;
+    for (int i = 0; i < 4; i++)
+        if (x.size(i) > 1) order[n++] = i;
+    for (int i = n; i < 4; i++) order[i] = -1;
+    std::sort(order, order + n, [&](int a, int b) { return x.stride(a) < x.stride(b); });
+    int64_t reach = 0;                                      // of the dimensions so far
+    for (int i = 0; i < n; i++) {
+        if (x.stride(order[i]) <= reach) return false;
+        reach += (x.size(order[i]) - 1) * x.stride(order[i]);
+    }
+    return true;
+}
+bool meets(const Tensor& x, const int (&order)[4], int from, int64_t apart) {
+    if (from < 0) return apart == 0;
+    if (order[from] < 0) return meets(x, order, from - 1, apart);
+    const int64_t s = x.stride(order[from]), most = x.size(order[from]) - 1, c = apart / s;
+    for (int64_t k = c - 1; k <= c + 1; k++)
+        if (k >= -most && k <= most && meets(x, order, from - 1, apart - k * s)) return true;
+    return false;
+}
+
 // (batch, tokens, heads, head_dim) rows: their strides; heads 0: any number.  Outputs' rows do not lie on one another
 bool rows_of(const Tensor& x, const char* name, int64_t heads, int64_t dim, bool output, long long* s) {
     if (x.dim() != 4 || x.size(3) != dim || (heads && x.size(2) != heads)) {
@@ -96,12 +121,11 @@ bool rows_of(const Tensor& x, const char* name, int64_t heads, int64_t dim, bool
         PyErr_Format(PyExc_ValueError, "%s: a head's values must be consecutive", name);
         return false;
     }
-    for (int i = 0; i < 3; i++) {
-        s[i] = st[i];
-        if (output && st[i] == 0 && x.size(i) > 1) {
-            PyErr_Format(PyExc_ValueError, "%s: rows must not lie on one another", name);
-            return false;
-        }
+    for (int i = 0; i < 3; i++) s[i] = st[i];
+    int order[4];
+    if (output && x.numel() && !nested(x, order)) {
+        PyErr_Format(PyExc_ValueError, "%s: rows must not lie on one another", name);
+        return false;
     }
     return true;
 }
@@ -196,6 +220,10 @@ PyObject* kv_read(PyObject*, PyObject* const* args, Py_ssize_t count) {
         if (k->sizes() != v->sizes() || k->scalar_type() != v->scalar_type() || k->size(0) != batch || k->size(1) != tokens ||
             (code >= 0 && code != code_of(k->scalar_type())))
             REFUSE("out: two tensors (batch, tokens, heads, head_dim) of the type asked for are needed");
+        int order[4];
+        const int64_t apart = (const char*)v->data_ptr() - (const char*)k->data_ptr(), size = (int64_t)k->element_size();
+        if (k->numel() && k->strides() == v->strides() && apart % size == 0 && nested(*k, order) && meets(*k, order, 3, apart / size))
+            REFUSE("out: keys and values must not lie on one another");
         if (!positions_of(c, batch, tokens, *start, "start", table, lens, false, &at) || !on_gpu({buffer, start, table, lens, k, v}))
             return nullptr;
     } else {
