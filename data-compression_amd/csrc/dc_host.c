@@ -145,15 +145,15 @@ typedef struct {
     void* c1_codes; size_t c1_codes_cap;
     void* c1_pos; size_t c1_pos_cap;
     void* c1_out; size_t c1_out_cap;
-    char msg[512];
 } dc_ctx;
 
 static dc_ctx G;
+static _Thread_local char last_error[512];   /* of the calling thread */
 
 static int seterr(int code, const char* fmt, ...) {
     va_list ap;
     va_start(ap, fmt);
-    vsnprintf(G.msg, sizeof G.msg, fmt, ap);
+    vsnprintf(last_error, sizeof last_error, fmt, ap);
     va_end(ap);
     return code;
 }
@@ -164,7 +164,7 @@ static int seterr(int code, const char* fmt, ...) {
         if (e_ != hipSuccess) return seterr(DC_ERR_HIP, "%s: %s", #call, hipGetErrorString(e_)); \
     } while (0)
 
-const char* dc_last_error(void) { return G.msg; }
+const char* dc_last_error(void) { return last_error; }
 #define ENC_ST (G.enc_st ? G.enc_st : G.st)
 /* the decoder build of the current decode: 1024-bit chunks, or 256-bit chunks (symbols with _s) */
 #define DV(fn) (G.dec_small ? fn##_s : fn)
@@ -2087,7 +2087,7 @@ static uint32_t mask_from_chars(const char* mask) {
 
 static void abi_fail(const char* fn, int rc) {
     G.abi_rc = rc;
-    fprintf(stderr, "libdcamd: %s failed (%d): %s\n", fn, rc, G.msg);
+    fprintf(stderr, "libdcamd: %s failed (%d): %s\n", fn, rc, last_error);
 }
 
 /* add_bit_to_bytes-compatible append of a GPU-encoded stream (:5456-5489 semantics) */

@@ -1,8 +1,8 @@
 /*
  * dc_host_lowbit.c -- entry points of the fixed-rate operators (include/dc_gpu.h): the key/value cache in 4 or 8 bits
  * (dc_kv.hip) and the 8-bit activation checkpoints (dc_act.hip).  Checks of arguments, the choice of a kernel's variant
- * and the launch; no state but the sticky status word, so that calls on several streams and from several threads do not
- * meet.
+ * and the launch; no state but the sticky status word (and the calling thread's error message), so that calls on several
+ * streams and from several threads do not meet.
  */
 #define __HIP_PLATFORM_AMD__ 1
 #include <hip/hip_runtime_api.h>

@@ -6,7 +6,7 @@
  * multi-GPU all-gather path) can run the codec without PCIe copies.  Plain C, no HIP/torch types:
  * device pointers are void*, the HIP stream is the library's per-process stream (dc_get_stream).
  *
- * Every function returns 0 on success or a negative DC_ERR_* code; dc_last_error() explains.
+ * Every function returns 0 on success or a negative DC_ERR_* code; dc_last_error() explains the calling thread's last one.
  */
 #ifndef DC_GPU_H
 #define DC_GPU_H
