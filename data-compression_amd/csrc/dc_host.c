@@ -11,6 +11,7 @@
 #define __HIP_PLATFORM_AMD__ 1
 #include <hip/hip_runtime_api.h>
 #include <math.h>
+#include <pthread.h>
 #include <stdarg.h>
 #include <stdio.h>
 #include <stdlib.h>
@@ -197,7 +198,8 @@ int dc_abi_status(void) { return G.abi_rc; }
 void dc_abi_set_status(int rc) { G.abi_rc = rc; }      /* the double ABI (dc_host64.c) reports through it too */
 int dc_set_error(int code, const char* msg) { return seterr(code, "%s", msg); }
 unsigned* dc_kv_status_word(void) { return G.d_kv_status; }   /* (dc_host_lowbit.c) */
-int dc_get_device(void) { return G.inited ? G.device : -1; }
+static int is_inited(void) { return __atomic_load_n(&G.inited, __ATOMIC_ACQUIRE); }
+int dc_get_device(void) { return is_inited() ? G.device : -1; }
 void* dc_get_stream(void) { return (void*)G.st; }
 void dc_set_abs_error_bound(double bound) { absErrBound = bound; absErrorBound_binary = -100; }
 double dc_get_abs_error_bound(void) { return absErrBound; }
@@ -241,8 +243,7 @@ static uint32_t h_xpow8n(unsigned long long n, const uint32_t* x2n) {
     return p;
 }
 
-int dc_init(int device) {
-    if (G.inited) return DC_OK;
+static int init_once(int device) {
     {   /* run-time override of the compile-time bound, so an unchanged app binary can run at another
          * bound (the reference recompiles after impl/set-parameter.sh edits the header) */
         const char* eb = getenv("DC_ABS_ERROR_BOUND");
@@ -304,11 +305,21 @@ int dc_init(int device) {
     HIPCHK(hipMalloc((void**)&G.d_kv_status, 64));
     HIPCHK(hipMemset(G.d_kv_status, 0, 64));
     G.dec_epoch = 1;
-    G.inited = 1;
+    __atomic_store_n(&G.inited, 1, __ATOMIC_RELEASE);
     return DC_OK;
 }
 
-static int ensure_init(void) { return G.inited ? DC_OK : dc_init(0); }
+/* (calls of several threads that are all the first: one starts the library, the others wait for it) */
+int dc_init(int device) {
+    static pthread_mutex_t lock = PTHREAD_MUTEX_INITIALIZER;
+    if (is_inited()) return DC_OK;
+    pthread_mutex_lock(&lock);
+    const int rc = is_inited() ? DC_OK : init_once(device);
+    pthread_mutex_unlock(&lock);
+    return rc;
+}
+
+static int ensure_init(void) { return is_inited() ? DC_OK : dc_init(0); }
 
 int dc_synchronize(void) {
     int rc = ensure_init();

@@ -41,6 +41,24 @@ elif case == "capture":
     graph.replay()
     torch.cuda.synchronize()
     assert float(y.sum()) == 64
+elif case == "threads":             # several at once, from C: one start, the same stream for all
+    import ctypes
+    import threading
+    torch.zeros(1, device="cuda")
+    L, gate, got = dcamd.lib().L, threading.Barrier(8), []
+
+    def first():
+        word = ctypes.c_uint(7)
+        gate.wait()
+        rc = L.dc_kv_status(None, ctypes.byref(word), 0)
+        got.append((rc, word.value, L.dc_get_stream(), L.dc_get_device()))
+
+    threads = [threading.Thread(target=first) for _ in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(got) == 8 and len(set(got)) == 1 and got[0][:2] == (0, 0) and got[0][2] and got[0][3] == 0, got
 want = torch.nn.functional.silu(torch.ones(4, 8))
 got, _ = dcamd.act_forward(torch.ones(4, 8, device="cuda"), "silu")
 assert torch.allclose(got.cpu(), want) and started() == 0

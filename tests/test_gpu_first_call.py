@@ -8,7 +8,7 @@ import pytest
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("case", ["device", "status", "capture"])
+@pytest.mark.parametrize("case", ["device", "status", "capture", "threads"])
 def test_first_call(case):
     at = os.path.join(os.path.dirname(os.path.abspath(__file__)), "native", "first_call.py")
     got = subprocess.run([sys.executable, at, case], capture_output=True, text=True, timeout=100)
