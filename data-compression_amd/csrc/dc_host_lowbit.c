@@ -6,6 +6,7 @@
  */
 #define __HIP_PLATFORM_AMD__ 1
 #include <hip/hip_runtime_api.h>
+#include <pthread.h>
 #include <stdint.h>
 #include <string.h>
 
@@ -223,12 +224,16 @@ int dc_kv_status(void* stream, unsigned* status_out, int reset) {
     hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
     if (hipStreamIsCapturing((hipStream_t)stream, &cap) != hipSuccess || cap != hipStreamCaptureStatusNone)
         REFUSE("status: the stream is being captured");
+    /* a reset takes the word and clears it in one step, into the word beside it: a bit that another stream's call sets
+     * meanwhile is in this answer or in the next (the lock is for that place) */
+    static pthread_mutex_t lock = PTHREAD_MUTEX_INITIALIZER;
     unsigned* w = dc_kv_status_word();
-    if (hipMemcpyAsync(status_out, w, 4, hipMemcpyDeviceToHost, (hipStream_t)stream) != hipSuccess ||
-        (reset && hipMemsetAsync(w, 0, 4, (hipStream_t)stream) != hipSuccess) ||
-        hipStreamSynchronize((hipStream_t)stream) != hipSuccess)
-        return dc_set_error(DC_ERR_HIP, "status: the read failed");
-    return DC_OK;
+    if (reset) pthread_mutex_lock(&lock);
+    const int bad = (reset && dc_launch_kv_take(w, (dc_hip_stream)stream)) ||
+                    hipMemcpyAsync(status_out, w + (reset != 0), 4, hipMemcpyDeviceToHost, (hipStream_t)stream) != hipSuccess ||
+                    hipStreamSynchronize((hipStream_t)stream) != hipSuccess;
+    if (reset) pthread_mutex_unlock(&lock);
+    return bad ? dc_set_error(DC_ERR_HIP, "status: the read failed") : DC_OK;
 }
 
 /* ---- activation checkpoints ------------------------------------------------------------------------------ */

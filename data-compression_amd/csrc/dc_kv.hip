@@ -976,6 +976,8 @@ template <int D> __global__ __launch_bounds__(256) void kv_join(KvArgs a) {
     }
 }
 
+__global__ void kv_take(unsigned* word) { word[1] = atomicExch(word, 0u); }
+
 template <class E, int BITS, bool VEC> int go_rows(const KvArgs& a, bool write, hipStream_t st) {
     const unsigned grid = (unsigned)((a.rows + 3) / 4);
 #define DC_ROWS(D) \
@@ -1024,6 +1026,11 @@ extern "C" int dc_launch_kv_rows(const dc::KvArgs* a, int write, dc_hip_stream s
     if (a->dtype == DC_F32) return go_bits<F32>(*a, write, st);
     if (a->dtype == DC_F16) return go_bits<F16>(*a, write, st);
     return go_bits<BF16>(*a, write, st);
+}
+
+extern "C" int dc_launch_kv_take(unsigned* word, dc_hip_stream st) {
+    kv_take<<<1, 1, 0, st>>>(word);
+    return hipGetLastError() != hipSuccess;
 }
 
 extern "C" int dc_kv_wide_cols(int dim) { return 16 * wide_tiles(dim); }

@@ -337,6 +337,7 @@ int dc_launch_crc_resend(const uint32_t* crc, const uint8_t* src, uint8_t* dst, 
                          unsigned* count, dc_hip_stream st);
 int dc_launch_kv_rows(const DC_NS KvArgs* a, int write, dc_hip_stream st);
 int dc_launch_kv_attention(const DC_NS KvArgs* a, dc_hip_stream st);
+int dc_launch_kv_take(unsigned* word, dc_hip_stream st);        /* word[1] = word[0], which is then 0 */
 int dc_kv_wide_cols(int dim);
 int dc_launch_act(const DC_NS ActArgs* a, int back, dc_hip_stream st);
 int dc_launch_ham_syndrome(const uint8_t* s, long long nbytes, unsigned long long* d_syn_ones, dc_hip_stream st);

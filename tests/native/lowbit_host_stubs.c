@@ -10,11 +10,12 @@
 static KvArgs last_kv;
 static ActArgs last_act;
 static int launches;
-static unsigned word;
+static unsigned word[16];
 static char message[256];
+static unsigned takes_bits;
 
 int dc_init(int device) { (void)device; return DC_OK; }
-unsigned* dc_kv_status_word(void) { return &word; }
+unsigned* dc_kv_status_word(void) { return word; }
 int dc_set_error(int code, const char* msg) {
     strncpy(message, msg, sizeof message - 1);
     return code;
@@ -33,6 +34,12 @@ int dc_launch_act(const ActArgs* a, int back, dc_hip_stream st) {
     launches++;
     return 0;
 }
+int dc_launch_kv_take(unsigned* w, dc_hip_stream st) {
+    (void)st;
+    w[1] = w[0];
+    w[0] = takes_bits;                  /* (of a call on another stream) */
+    return 0;
+}
 hipError_t hipStreamIsCapturing(hipStream_t st, hipStreamCaptureStatus* s) {
     (void)st;
     *s = hipStreamCaptureStatusNone;
@@ -43,16 +50,12 @@ hipError_t hipMemcpyAsync(void* d, const void* s, size_t n, hipMemcpyKind k, hip
     memcpy(d, s, n);
     return hipSuccess;
 }
-hipError_t hipMemsetAsync(void* d, int v, size_t n, hipStream_t st) {
-    (void)st;
-    memset(d, v, n);
-    return hipSuccess;
-}
 hipError_t hipStreamSynchronize(hipStream_t st) { (void)st; return hipSuccess; }
 
 /* for the test */
 int stub_launches(void) { return launches; }
 const char* stub_message(void) { return message; }
+void stub_word(unsigned now, unsigned then) { word[0] = now; takes_bits = then; }
 int stub_vec(void) { return last_kv.vec; }
 int stub_vec_out(void) { return last_kv.vec_out; }
 unsigned stub_splits(void) { return last_kv.splits; }

@@ -103,3 +103,19 @@ def test_joined_outputs_off_their_alignment(kv, dim, n, off):
     assert same(out, want)
     out.fill_(-3.0)
     assert bool((room == -3).all())
+
+
+def test_status_beside_other_streams(kv):
+    """A bit that is set while the word is taken is in that answer or in the next."""
+    c = make(kv, 1, 16, 1, 32, 4)
+    x, side = torch.zeros(1, 1, 1, 32, device=DEV), torch.cuda.Stream()
+    outside, pos = torch.full((1, 1), 5, dtype=torch.int32, device=DEV), i32(0)
+    torch.cuda.synchronize()
+    kv.KVCache.status(reset=True)
+    for _ in range(200):
+        with torch.cuda.stream(side):
+            c.write(x, x, pos, table=outside)
+        got = kv.KVCache.status(reset=True)
+        side.synchronize()
+        assert got | kv.KVCache.status(reset=True) == 1
+        assert kv.KVCache.status() == 0

@@ -72,3 +72,13 @@ def test_calls_of_most_rows(host):
         assert host.stub_launches() == before + (rc == 0)
     host.dc_act_bytes.restype, host.dc_act_bytes.argtypes = C.c_size_t, [C.c_longlong]
     assert host.dc_act_bytes(most) == most // 32 * 33 and host.dc_act_bytes(most + 1) == 0
+
+
+def test_status_taken_in_one_step(host):
+    """What another stream's call reports while the word is taken is there for the next."""
+    word = C.c_uint(9)
+    for now, then in ((0, 0), (1, 0), (0, 1), (1, 1)):
+        host.stub_word(now, then)
+        assert host.dc_kv_status(None, C.byref(word), 0) == 0 and word.value == now
+        assert host.dc_kv_status(None, C.byref(word), 1) == 0 and word.value == now
+        assert host.dc_kv_status(None, C.byref(word), 0) == 0 and word.value == then
