@@ -25,6 +25,18 @@ enum { MOST_GROUPS = (1 << 24) - 1 };
 /* the high half of n times this is n / d where n d < 2^64 (2^64 / d, rounded up); 0 stands for d = 1 */
 static unsigned long long inverse(unsigned long long d) { return d <= 1 ? 0 : ~0ull / d + 1; }
 
+/* the library is started and the stream is one of its device; HIP's default stream belongs to whichever is the current one */
+static int ready(void* stream) {
+    const int rc = dc_init(0);
+    if (rc) return rc;
+    int device = 0;                                             /* (hipGetDevice is the shorter call) */
+    if ((stream ? hipStreamGetDevice((hipStream_t)stream, &device) : hipGetDevice(&device)) != hipSuccess)
+        (void)hipGetLastError();                                /* (the launch will say) */
+    else if (device != dc_get_device())
+        REFUSE("the stream (the default stream: the current device) is not of the library's device");
+    return DC_OK;
+}
+
 static int size_of(int dtype) { return dtype == DC_F32 ? 4 : dtype == DC_F16 || dtype == DC_BF16 ? 2 : 0; }
 
 size_t dc_kv_page_bytes(int page_size, int heads, int head_dim, int bits) {
@@ -107,7 +119,7 @@ static int rows_call(const dc_kv_cache* c, const dc_kv_batch* at, int dtype, con
     a.past = 2.0 * at->batch * at->tokens * c->heads * c->head_dim * size > 128e6;
     const unsigned piece = low_bit((unsigned)(c->head_dim / 16 * size));
     a.vec = fits(k, ks, size, piece > 16 ? 16 : piece) && fits(v, vs, size, piece > 16 ? 16 : piece);
-    if ((rc = dc_init(0))) return rc;
+    if ((rc = ready(stream))) return rc;
     a.status = dc_kv_status_word();
     return dc_launch_kv_rows(&a, write, (dc_hip_stream)stream) ? dc_set_error(DC_ERR_HIP, "cache: the launch failed") : DC_OK;
 }
@@ -212,14 +224,14 @@ int dc_kv_attention_device(const dc_kv_cache* cache, const dc_kv_batch* at, int 
     a.lse = d_lse;
     a.part = (float*)d_workspace;
     a.part_ml = need ? a.part + (size_t)at->batch * (size_t)a.heads * a.row_slots * a.splits * (size_t)a.dim : NULL;
-    if ((rc = dc_init(0))) return rc;
+    if ((rc = ready(stream))) return rc;
     a.status = dc_kv_status_word();
     return dc_launch_kv_attention(&a, (dc_hip_stream)stream) ? dc_set_error(DC_ERR_HIP, "attention: the launch failed") : DC_OK;
 }
 
 int dc_kv_status(void* stream, unsigned* status_out, int reset) {
     if (!status_out) REFUSE("status: nowhere to put it");
-    int rc = dc_init(0);
+    int rc = ready(stream);
     if (rc) return rc;
     hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
     if (hipStreamIsCapturing((hipStream_t)stream, &cap) != hipSuccess || cap != hipStreamCaptureStatusNone)
@@ -283,7 +295,7 @@ static int act_call(ActArgs* a, int back, void* stream) {
     a->past = (double)a->n * size * (!!a->y + !!a->dx + !!a->dup) > 128e6;
     a->groups = (a->n + 31) / 32;
     a->cols8_inv = inverse((unsigned long long)(a->cols / 8));
-    const int rc = dc_init(0);
+    const int rc = ready(stream);
     if (rc) return rc;
     return dc_launch_act(a, back, (dc_hip_stream)stream) ? dc_set_error(DC_ERR_HIP, "activation: the launch failed") : DC_OK;
 }

@@ -282,7 +282,8 @@ int dc64_med_device(const void* d_x, long long n, double* mean_out, int* type_ou
  * place.  A key/value cache of a decoder (4 or 8 bits) with the attention that reads it, and 8-bit checkpoints of
  * activations with the backward pass that uses them.  All calls are asynchronous on `stream`, a hipStream_t (NULL is
  * HIP's default stream, dc_get_stream() the library's); they keep no state between calls but the sticky status word,
- * read nothing back and may be recorded into a graph (call dc_init first).  Arrays lie on the library's device.
+ * read nothing back and may be recorded into a graph (call dc_init first).  Arrays and the stream are of the library's device;
+ * for the default stream that has to be the current one.
  *
  * Element types of arrays: */
 enum { DC_F32 = 0, DC_F16 = 1, DC_BF16 = 2 };

@@ -13,8 +13,17 @@ static int launches;
 static unsigned word[16];
 static char message[256];
 static unsigned takes_bits;
+static int device_of_streams;
 
 int dc_init(int device) { (void)device; return DC_OK; }
+int dc_get_device(void) { return 0; }
+hipError_t hipGetLastError(void) { return hipSuccess; }
+hipError_t hipStreamGetDevice(hipStream_t st, hipDevice_t* d) {
+    (void)st;
+    *d = device_of_streams;
+    return device_of_streams < 0 ? hipErrorInvalidHandle : hipSuccess;
+}
+hipError_t hipGetDevice(int* d) { return hipStreamGetDevice(NULL, d); }
 unsigned* dc_kv_status_word(void) { return word; }
 int dc_set_error(int code, const char* msg) {
     strncpy(message, msg, sizeof message - 1);
@@ -56,6 +65,7 @@ hipError_t hipStreamSynchronize(hipStream_t st) { (void)st; return hipSuccess; }
 int stub_launches(void) { return launches; }
 const char* stub_message(void) { return message; }
 void stub_word(unsigned now, unsigned then) { word[0] = now; takes_bits = then; }
+void stub_device(int d) { device_of_streams = d; }
 int stub_vec(void) { return last_kv.vec; }
 int stub_vec_out(void) { return last_kv.vec_out; }
 unsigned stub_splits(void) { return last_kv.splits; }

@@ -119,3 +119,24 @@ def test_status_beside_other_streams(kv):
         side.synchronize()
         assert got | kv.KVCache.status(reset=True) == 1
         assert kv.KVCache.status() == 0
+
+
+def test_streams_of_all_kinds(kv):
+    """HIP's default stream, its stream of the thread, the library's and one of torch's, through the C entry points."""
+    import ctypes as C
+    L = kv.lib()
+    c = make(kv, 1, 16, 2, 32, 4)
+    k, v = torch.randn(1, 5, 2, 32, device=DEV), torch.randn(1, 5, 2, 32, device=DEV)
+    want = [rounded(held(x.cpu(), 4)[0].float(), torch.float32) for x in (k, v)]
+    start, st = i32(0), (C.c_longlong * 3)(320, 64, 32)
+    at = kv.KvBatchDesc(1, 5, start.data_ptr(), None, None, 0, 0, 0)
+    torch.cuda.synchronize()
+    for stream in (None, 2, L.L.dc_get_stream(), torch.cuda.Stream().cuda_stream):      # (2: hipStreamPerThread)
+        c.buffer.zero_()
+        got = [torch.full((1, 5, 2, 32), -1.0, device=DEV) for _ in range(2)]
+        torch.cuda.synchronize()
+        L.check(L.L.dc_kv_write_device(c._desc, at, 0, k.data_ptr(), st, v.data_ptr(), st, stream), "write")
+        L.check(L.L.dc_kv_read_device(c._desc, at, 0, got[0].data_ptr(), st, got[1].data_ptr(), st, stream), "read")
+        word = C.c_uint(7)
+        L.check(L.L.dc_kv_status(stream, C.byref(word), 0), "status")                   # (waits for the stream)
+        assert word.value == 0 and same(got[0], want[0]) and same(got[1], want[1])

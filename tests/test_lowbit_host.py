@@ -82,3 +82,20 @@ def test_status_taken_in_one_step(host):
         assert host.dc_kv_status(None, C.byref(word), 0) == 0 and word.value == now
         assert host.dc_kv_status(None, C.byref(word), 1) == 0 and word.value == now
         assert host.dc_kv_status(None, C.byref(word), 0) == 0 and word.value == then
+
+
+def test_streams_of_other_devices(host):
+    """A stream that is not of the library's device, or the default one while another is current: refused before a launch.  (One
+    that HIP does not tell about is left to the launch.)"""
+    st, word = three(64, 64, 64), C.c_uint()
+    cache, at = host.desc(P, 4, 16, 1, 32, 4), host.at(1, 1, P, None, None, 0, 0, 0)
+    calls = [lambda: host.dc_kv_write_device(cache, at, 1, P, st, P, st, on), lambda: host.dc_kv_read_device(cache, at, 1, P, st, P, st, on),
+             lambda: host.dc_kv_attention_device(cache, at, 1, 1, P, st, 1.0, 1, 16, P, st, None, None, 0, on),
+             lambda: host.dc_act_forward_device(1, 1, 4, 8, P, 8, None, 0, P, 8, P, None, on), lambda: host.dc_kv_status(on, C.byref(word), 0)]
+    for device, rc in ((1, ARG), (0, 0), (-1, 0)):
+        host.stub_device(device)
+        for on in (None, P):
+            before = host.stub_launches()
+            for f in calls:
+                assert f() == rc
+            assert host.stub_launches() == before + (4 if rc == 0 else 0)
