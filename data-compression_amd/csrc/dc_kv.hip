@@ -112,9 +112,10 @@ static __device__ __forceinline__ uint32_t div_by(uint32_t n, unsigned long long
 }
 
 // lane T of the row's 16
-template <int T> static __device__ __forceinline__ float row_lane(float x) {
-    return asf((uint32_t)__builtin_amdgcn_update_dpp(0, (int)asu(x), 0x150 + T, 0xF, 0xF, true));
+template <int T> static __device__ __forceinline__ uint32_t row_lane(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x150 + T, 0xF, 0xF, true);
 }
+template <int T> static __device__ __forceinline__ float row_lane(float x) { return asf(row_lane<T>(asu(x))); }
 template <int... I, class F> static __device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F f) {
     (f(std::integral_constant<int, I>{}), ...);
 }
@@ -254,7 +255,7 @@ template <class E, int D, int BITS, bool VEC, bool PAST> __global__ __launch_bou
     const uint32_t z = rint_div(l, s, inv);
     const bool finite = most(fabsf(l), fabsf(h)) < INFINITY;
     const uint32_t word = finite ? (asu(s) >> 16) | z << 16 : 0x7FC0u;     // (else a step of NaN, codes of 0)
-    const float top = asf(finite ? CODES : 0);
+    const uint32_t top = finite ? CODES : 0;
     uint8_t* codes = (uint8_t*)k.base + (k.kv ? (long long)a.page * ROW : 0) + (long long)k.at * ROW;
     uint32_t* words = (uint32_t*)((uint8_t*)k.base + 2ll * a.page * ROW + (k.kv ? 4ll * a.page : 0)) + k.at + 4 * g;
     if (u < 4 && t + u >= 0 && t + u < k.n) words[u] = word;
@@ -263,14 +264,15 @@ template <class E, int D, int BITS, bool VEC, bool PAST> __global__ __launch_bou
         constexpr int r = I.value;
         if (!__any(on[r])) return;
         const float sr = row_lane<r>(s), ir = row_lane<r>(inv);
-        float zr = row_lane<r>(asf(z)), most = row_lane<r>(top);
-        asm("" : "+v"(zr), "+v"(most));                     // (kept as moves: within v_sub_u32 and v_min_i32 the broadcast gave wrong codes)
+        // added as its negative: x less a lane's whole number becomes v_subrev_u32 with DPP, which moves the other
+        // operand instead (of any control, measured; sums, minima and the f32 forms move the one that is named)
+        const uint32_t zr = row_lane<r>(0u - z), most = row_lane<r>(top);
 #pragma unroll
         for (int i = 0; i < N; i += 8 / BITS) {
             uint32_t q = 0;
 #pragma unroll
             for (int j = 0; j < 8 / BITS; j++)
-                q |= (uint32_t)min(max((int)(rint_div(x[r][i + j], sr, ir) - asu(zr)), 0), (int)asu(most)) << (j * BITS);
+                q |= (uint32_t)min(max((int)(rint_div(x[r][i + j], sr, ir) + zr), 0), (int)most) << (j * BITS);
             out[r][i * BITS / 8] = (uint8_t)q;
         }
         if (!all && on[r])
