@@ -153,6 +153,7 @@ static int plan(const dc_kv_cache* c, int batch, int tokens, int q_heads, long l
     a->row_slots = (unsigned)rows;
     const long long base = (long long)batch * c->heads * a->tiles;
     if (base > (1ll << 30)) return 1;
+    if (max_context > 1ll << 30) max_context = 1ll << 30;       /* (positions are 32-bit) */
     const int AIM = a->cols == 16 && c->head_dim <= 128 ? 768 : 384;
     enum { SHORT = 640, LEAST = 256, MOST = 256 };
     long long splits = 1;

@@ -99,3 +99,14 @@ def test_streams_of_other_devices(host):
             for f in calls:
                 assert f() == rc
             assert host.stub_launches() == before + (4 if rc == 0 else 0)
+
+
+def test_any_context_may_be_expected(host):
+    """max_context up to the largest number: as the largest context that there can be."""
+    cache, st = host.desc(P, 4, 16, 2, 64, 4), three(64, 64, 64)
+    most = host.dc_kv_attention_workspace(cache, 1, 1, 4, 1 << 30)
+    assert most > 0
+    for context in ((1 << 30) + 1, 1 << 40, (1 << 63) - 200, (1 << 63) - 1):
+        assert host.dc_kv_attention_workspace(cache, 1, 1, 4, context) == most
+        assert host.dc_kv_attention_device(cache, host.at(1, 1, P, None, None, 0, 0, 0), 1, 4, P, st, 1.0, 1, context, P, st, None, P, most, None) == 0
+        assert host.stub_splits() == 256
