@@ -235,8 +235,9 @@ int dc_kv_status(void* stream, unsigned* status_out, int reset) {
     int rc = ready(stream);
     if (rc) return rc;
     hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing((hipStream_t)stream, &cap) != hipSuccess || cap != hipStreamCaptureStatusNone)
-        REFUSE("status: the stream is being captured");
+    const int unsure = hipStreamIsCapturing((hipStream_t)stream, &cap) != hipSuccess;   /* (the default stream beside a capture) */
+    if (unsure) (void)hipGetLastError();                        /* (not for the next launch to find) */
+    if (unsure || cap != hipStreamCaptureStatusNone) REFUSE("status: the stream is being captured");
     /* a reset takes the word and clears it in one step, into the word beside it: a bit that another stream's call sets
      * meanwhile is in this answer or in the next (the lock is for that place) */
     static pthread_mutex_t lock = PTHREAD_MUTEX_INITIALIZER;

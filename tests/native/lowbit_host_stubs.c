@@ -13,11 +13,16 @@ static int launches;
 static unsigned word[16];
 static char message[256];
 static unsigned takes_bits;
-static int device_of_streams;
+static int device_of_streams, capture_beside;
 
 int dc_init(int device) { (void)device; return DC_OK; }
 int dc_get_device(void) { return 0; }
-hipError_t hipGetLastError(void) { return hipSuccess; }
+static hipError_t left;                     /* what HIP's last error is */
+hipError_t hipGetLastError(void) {
+    const hipError_t e = left;
+    left = hipSuccess;
+    return e;
+}
 hipError_t hipStreamGetDevice(hipStream_t st, hipDevice_t* d) {
     (void)st;
     *d = device_of_streams;
@@ -52,7 +57,7 @@ int dc_launch_kv_take(unsigned* w, dc_hip_stream st) {
 hipError_t hipStreamIsCapturing(hipStream_t st, hipStreamCaptureStatus* s) {
     (void)st;
     *s = hipStreamCaptureStatusNone;
-    return hipSuccess;
+    return left = capture_beside ? hipErrorStreamCaptureImplicit : hipSuccess;
 }
 hipError_t hipMemcpyAsync(void* d, const void* s, size_t n, hipMemcpyKind k, hipStream_t st) {
     (void)k; (void)st;
@@ -66,6 +71,8 @@ int stub_launches(void) { return launches; }
 const char* stub_message(void) { return message; }
 void stub_word(unsigned now, unsigned then) { word[0] = now; takes_bits = then; }
 void stub_device(int d) { device_of_streams = d; }
+void stub_capture_beside(int on) { capture_beside = on; }
+int stub_left(void) { return left; }
 int stub_vec(void) { return last_kv.vec; }
 int stub_vec_out(void) { return last_kv.vec_out; }
 unsigned stub_splits(void) { return last_kv.splits; }

@@ -110,3 +110,12 @@ def test_any_context_may_be_expected(host):
         assert host.dc_kv_attention_workspace(cache, 1, 1, 4, context) == most
         assert host.dc_kv_attention_device(cache, host.at(1, 1, P, None, None, 0, 0, 0), 1, 4, P, st, 1.0, 1, context, P, st, None, P, most, None) == 0
         assert host.stub_splits() == 256
+
+
+def test_status_beside_a_capture(host):
+    """Refused, and HIP's error of the question does not stay for the next launch's check."""
+    word = C.c_uint()
+    host.stub_capture_beside(1)
+    assert host.dc_kv_status(None, C.byref(word), 0) == ARG and host.stub_left() == 0
+    host.stub_capture_beside(0)
+    assert host.dc_kv_status(None, C.byref(word), 0) == 0
