@@ -36,6 +36,10 @@ bool tensor_of(PyObject* o, const char* name, bool optional, const Tensor** t) {
         return false;
     }
     *t = &THPVariable_Unpack(o);
+    if ((*t)->is_neg()) {                                   // (its memory holds the other sign)
+        PyErr_Format(PyExc_ValueError, "%s: a negative view is not taken (resolve_neg() it)", name);
+        return false;
+    }
     return true;
 }
 #define TENSOR(i, name, optional) \

@@ -84,3 +84,17 @@ def test_what_is_on_one_another_by_trying(d):
         both = torch.isin(a, b).any()
         with pytest.raises(ValueError, match="keys and values must not" if both else "GPU"):
             c.read(s, 3, out=(room.as_strided((2, 3, 2, 64), strides, 0), room.as_strided((2, 3, 2, 64), strides, off)))
+
+
+def test_negative_views(d):
+    """The imaginary part of a conjugate shares memory that holds the other sign."""
+    x = torch.zeros(4, 8, dtype=torch.complex64).conj().imag
+    assert x.is_neg()
+    page = d.KVCache.page_bytes(16, 2, 64, 4)
+    c = cache_in(d, torch.zeros(2 * page + 16, dtype=torch.uint8), 2)
+    k, s = torch.zeros(2, 3, 2, 64, dtype=torch.complex64).conj().imag, torch.zeros(2, dtype=torch.int32)
+    kept = d.ActCheckpoint((4, 8), torch.float32, torch.zeros(33, dtype=torch.uint8))
+    for f in (lambda: d.act_forward(x, "silu"), lambda: d.act_forward(x.resolve_neg(), "silu", up=x), lambda: d.act_save(x), lambda: d.act_backward(x, kept, "silu"),
+              lambda: c.write(k, k.resolve_neg(), s), lambda: c.write(k.resolve_neg(), k, s), lambda: c.read(s, 3, out=(k, k.resolve_neg()))):
+        with pytest.raises(ValueError, match="negative view"):
+            f()
