@@ -89,7 +89,7 @@ static int fits(const void* p, const long long* s, int size, unsigned bytes) {
     const uintptr_t m = bytes - 1;
     if ((uintptr_t)p & m) return 0;
     for (int i = 0; i < 3; i++)
-        if ((uintptr_t)(s[i] * size) & m) return 0;
+        if ((uintptr_t)s[i] * (uintptr_t)size & m) return 0;
     return 1;
 }
 
@@ -258,7 +258,7 @@ static int shape_of(const void* p, long long ld, long long rows, long long cols,
     if (!p) return 0;
     const int aligned = ((uintptr_t)p & 15u) == 0;
     if (aligned && (ld == cols || rows == 1)) return 0;
-    return aligned && cols % 8 == 0 && (ld * size) % 16 == 0 ? 1 : 2;
+    return aligned && cols % 8 == 0 && (uintptr_t)ld * (uintptr_t)size % 16 == 0 ? 1 : 2;
 }
 
 static int act_call(ActArgs* a, int back, void* stream) {
@@ -288,7 +288,7 @@ static int act_call(ActArgs* a, int back, void* stream) {
     if (mode == 0 && apart) {
         mode = 1;
         for (int i = 0; i < 5; i++)
-            if (arrays[i] && (a->cols % 8 || (a->rows > 1 && (lds[i] * size) % 16))) mode = 2;
+            if (arrays[i] && (a->cols % 8 || (a->rows > 1 && (uintptr_t)lds[i] * (uintptr_t)size % 16))) mode = 2;
     }
     a->mode = mode;
     a->n = a->rows * a->cols;

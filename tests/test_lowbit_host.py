@@ -119,3 +119,11 @@ def test_status_beside_a_capture(host):
     assert host.dc_kv_status(None, C.byref(word), 0) == ARG and host.stub_left() == 0
     host.stub_capture_beside(0)
     assert host.dc_kv_status(None, C.byref(word), 0) == 0
+
+
+def test_under_the_sanitizers(tmp_path):
+    """Arguments at and past every field's edges, in random combinations, under AddressSanitizer and UBSan: each call is taken
+    or refused."""
+    subprocess.check_call(["make", "-s", "-C", os.path.join(ROOT, "data-compression_amd"), f"B={tmp_path}", f"{tmp_path}/lowbit_asan_check"])
+    got = subprocess.run([str(tmp_path / "lowbit_asan_check")], capture_output=True, text=True, timeout=100, env=dict(os.environ, ASAN_OPTIONS="detect_leaks=0"))
+    assert got.returncode == 0 and got.stdout.startswith("fine: "), got.stdout + got.stderr
