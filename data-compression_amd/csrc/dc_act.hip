@@ -46,8 +46,9 @@ template <bool WIDE> static __device__ __forceinline__ float exp_of(float x, flo
 // keeps its precision down to the smallest normal result and no power overflows; 16 bits: from e^-x, whose reciprocal is 0
 // below -87 (results of less than 2^-119).
 // gelu: f = x Phi(x), f' = Phi(x) + x phi(x).  With t = 1 / (1 + c |x|) the upper tail is Phi(-|x|) = e^(-x^2/2) t p(t), p a
-// polynomial fitted to it, for f32 of degree 8 (relative error below 5e-8 for every x), for 16 bits of degree 5 (8e-6: the
-// forward pass is bound by its arithmetic, not by HBM, with the longer one).
+// polynomial fitted to it, for f32 of degree 8 (relative error below 6e-8 for every x), for 16 bits of degree 5 (8e-6: the
+// forward pass is bound by its arithmetic, not by HBM, with the longer one).  Both by iterated weighted least squares, as
+// tests/test_act_fit.py does again.
 template <int KIND, bool WIDE> static __device__ __forceinline__ void value_slope(float x, float& f, float& df) {
     if constexpr (KIND == DC_ACT_SILU && WIDE) {
         const float a = fabsf(x), unit = a > 64.0f ? 5.421010862427522e-20f : 1.0f;
