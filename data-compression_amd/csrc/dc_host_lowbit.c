@@ -137,9 +137,11 @@ int dc_kv_read_device(const dc_kv_cache* cache, const dc_kv_batch* at, int dtype
 /* How the attention is cut.  Query rows (tokens x the group that shares a head) in tiles of 16, or of as many as a wave's
  * registers hold where there are more.  The cache's positions in up to `splits` pieces a sequence, so that there are
  * about 768 workgroups, 3 per compute unit (with the join, 48 sequences of up to 8192 positions, 8 heads: 512 84 us, 768 76,
- * 1024 75, 2048 76; 20 of them: 38, 38, 40, 48; one of 262143, 2 heads: 21 to 22 for all), or half of that where a compute
- * unit holds two of them, wide tiles and long rows (16 sequences of 8192, heads of 256: 256 37 us, 384 32, 768 38; 8 queries
- * each, heads of 64: 256 31, 384 27, 768 33); up to twice the even number of pieces, for sequences longer than the others.
+ * 1024 75, 2048 76; 20 of them: 38, 38, 40, 48), or half of that where a compute unit holds two of them, wide tiles and long
+ * rows (16 sequences of 8192, heads of 256: 256 37 us, 384 32, 768 38; 8 queries each, heads of 64: 256 31, 384 27, 768
+ * 33); up to twice the even number of pieces, for sequences longer than the others.  At most 256 pieces, as the join takes a
+ * thread for each: one sequence of 1 or 2 heads then has 256 or 512 workgroups, whatever the aim (262143 positions, 2 heads:
+ * 21 us).
  * None up to 640 positions: there a second kernel, which joins the pieces, costs what they save (8 heads, 517 positions:
  * 9.6 us in one piece, 7.0 + 2.8 in three). */
 static int plan(const dc_kv_cache* c, int batch, int tokens, int q_heads, long long max_context, KvArgs* a) {

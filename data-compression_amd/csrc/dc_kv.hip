@@ -357,8 +357,9 @@ template <class E, int D, int BITS, bool VEC, bool PAST> __global__ __launch_bou
 // a reference M, and vs_t counts in 2^(R - 7), one power of two for a wave.  M is raised only by what its row sees (`refer`)
 // and so that the largest weight yet is 16 or more and below 2^15.  So 11 bits are kept down to 2^-14, fewer below: a weight
 // is off by 2^-11 of itself, half a unit of what f16 outputs round to, or by 2^-29 of its row's largest; whatever the steps
-// of tokens that a row does not see, or sees with no weight.  (Steps 2^-100 of the largest in a tile of rows lose bits.)  The
-// sum of p_t is kept in f32.
+// of tokens that a row does not see, or sees with no weight.  (As far as p_t may go: rows whose steps are 2^-80 of the largest
+// in their tile lose bits, as do those with scores above 2^20, for which the wave's largest step sets the unit.)  The sum of
+// p_t is kept in f32.
 // Queries are scaled to 2^14..2^15 by a power of two (exact); elements 2^-30 of a row's largest lose bits.
 //
 // A token's words are wanted by the 16 lanes that share its 4 tokens of a block: lane % 8 decodes one of the group's 8
@@ -368,10 +369,10 @@ template <class E, int D, int BITS, bool VEC, bool PAST> __global__ __launch_bou
 // a score's own; with the weights rounded two at a time and the values' operands made by one byte permute for four codes, a
 // step of 32 tokens x 32 queries of 64 values is 200 vector instructions (302 before), 16 of them exponentials.
 //
-// 48 sequences of up to 8192 positions, 8 heads of 128 in 4 bits: 61 us and 4.7 for the join, 5.0 TB/s; bound by HBM, in
-// pieces of 2 KiB.  One of 262143, 2 heads: 16.6 + 4.6 us, 4.2 TB/s.  517 positions: 9.2 us, the chain of lengths, pages,
-// codes, scores and sums.  Prompts (two of up to 509 queries behind 8192, 16 heads of 64, 8 bits): 64 to 80 us by their
-// lengths, 316 to 390 TFLOP/s, 84 % of the vector instructions' rate while the waves run; the longer one's workgroups are
+// 48 sequences of up to 8192 positions, 8 heads of 128 in 4 bits: 62 us and 4.7 for the join, 4.9 TB/s; bound by HBM, in
+// pieces of 2 KiB.  One of 262143, 2 heads: 17.4 + 4.0 us, 4.1 TB/s.  517 positions: 9.0 us, the chain of lengths, pages,
+// codes, scores and sums.  Prompts (two of up to 509 queries behind 8192, 16 heads of 64, 8 bits): 63 to 80 us by their
+// lengths, 316 to 400 TFLOP/s, 84 % of the vector instructions' rate while the waves run; the longer one's workgroups are
 // waited for (cut in pieces they cost their prologues and the join: 72 us, so 72 to 78).
 static __device__ __forceinline__ float over_groups_max(float x) {     // over the 4 groups of 16 lanes
     auto p = __builtin_amdgcn_permlane32_swap((int)asu(x), (int)asu(x), false, false);

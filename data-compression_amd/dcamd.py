@@ -1271,7 +1271,9 @@ class KVCache:
     Sequences are rows of a batch: `table` (batch, n) int32 names each one's pages (None: page b is sequence b's only one),
     `start` / `context` and `lens` are int32 of (batch,).  Rows from lens[b] on are padding and are not touched.
     Calls go to torch's current stream, allocate what they return (and the attention its workspace) from torch, and can be
-    captured into a graph.  They have no gradient."""
+    captured into a graph (but for the process's first call, which starts the library).  Tensors lie on one device, the
+    current one.  Outputs that are given must not share memory with one another or with inputs.  The calls have no
+    gradient."""
 
     def __init__(self, pages, page_size, heads, head_dim, bits=4, buffer=None, device="cuda"):
         self._native = native()
@@ -1312,7 +1314,8 @@ class KVCache:
     def attention(self, q, context, table=None, lens=None, scale=None, causal=True, max_context=None, out=None, lse=None):
         """softmax(scale q k^T) v over the first context[b] positions of each sequence, q (batch, tokens, q_heads, head_dim)
         in f16 or bf16 being its last lens[b] (None: all) tokens: causal, token i sees context[b] - lens[b] + 1 + i of
-        them.  scale: 1 / sqrt(head_dim).  max_context: the longest context expected (the table's capacity).  out: where
+        them.  scale: 1 / sqrt(head_dim).  max_context: the longest context expected (the table's capacity: where that is much
+        longer than the sequences, the split along them costs a second kernel that they do not need).  out: where
         to put the output (rows of padding keep what they have; in a new tensor they are 0); lse: an f32 tensor (batch,
         tokens, q_heads) for the log of each softmax's sum."""
         if max_context is None:

@@ -332,7 +332,8 @@ int dc_kv_read_device(const dc_kv_cache* cache, const dc_kv_batch* at, int dtype
  * full).  d_workspace: dc_kv_attention_workspace bytes (16-byte aligned; NULL where that is 0), in use until the call's work
  * is done: calls that may run at once need one each.  Outputs must not overlap the inputs.  Scores are formed in f32 from
  * queries and steps below 2^100.  A position's softmax weight times the step of its values is held to 2^-11 of itself or
- * 2^-29 of its query's largest, whichever is more; positions that a query does not see have no part in that. */
+ * 2^-29 of its query's largest, whichever is more (scores below 2^19, steps within 2^80 of one another); positions that a
+ * query does not see have no part in that.  Outputs beyond dtype's largest number are infinite. */
 size_t dc_kv_attention_workspace(const dc_kv_cache* cache, int batch, int tokens, int q_heads, long long max_context);
 int dc_kv_attention_device(const dc_kv_cache* cache, const dc_kv_batch* at, int dtype, int q_heads, const void* d_q,
                            const long long* q_strides, float scale, int causal, long long max_context, void* d_out,
@@ -348,7 +349,7 @@ int dc_kv_status(void* stream, unsigned* status_out, int reset);
  * (n <= 2^35 - 2048): */
 enum { DC_ACT_NONE = 0, DC_ACT_SILU = 1, DC_ACT_GELU = 2 };
 size_t dc_act_bytes(long long n);
-/* y = f(x) (d_up NULL) or f(x) up, and the checkpoints of x (and up); kind DC_ACT_NONE: the checkpoint alone (d_up and d_y
+/* y = f(x) (d_up NULL) or f(x) up, rounded to dtype (infinite beyond its largest number), and the checkpoints of x (and up); kind DC_ACT_NONE: the checkpoint alone (d_up and d_y
  * NULL).  ld*: elements between the starts of rows.  Checkpoints are 16-byte aligned. */
 int dc_act_forward_device(int kind, int dtype, long long rows, long long cols, const void* d_x, long long ldx,
                           const void* d_up, long long ldup, void* d_y, long long ldy, void* d_kept, void* d_kept_up,

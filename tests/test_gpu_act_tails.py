@@ -52,3 +52,21 @@ def test_16_bits(act, dtype):
         want, got = f_df(x.double(), kind)[0], y.cpu().double()
         tol = (torch.finfo(dtype).eps / 2 * 1.001 + 2.0 ** -15) * want.abs() + max(2.0 ** -119, torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2)
         assert bool(((got - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("kind", ["silu", "gelu"])
+def test_beyond_the_type(act, kind):
+    """Results beyond f16's largest number are infinite, as rounding them says; so is what an infinite input gives."""
+    x = torch.tensor([[1000.0, -1000.0, 3000.0, 60000.0, math.inf, 2.0, 300.0, 65504.0]], dtype=torch.float16)
+    up = torch.tensor([[100.0, 100.0, -30.0, 2.0, 1.0, 3e4, 200.0, 1.0]], dtype=torch.float16)
+    y, c = act.act_forward(x.to(DEV), kind, up=up.to(DEV))
+    assert y.cpu()[0, [0, 2, 3, 4]].tolist() == [math.inf, -math.inf, math.inf, math.inf] and bool(torch.isfinite(y.cpu()[0, [1, 5, 6, 7]]).all())
+    assert float(y[0, 7]) == 65504
+    dx, dup, back = act.act_backward(torch.full_like(x, 400.0).to(DEV), c, kind, recompute=True)
+    # at the kept values: infinite where the formula is beyond 65520.  (The gate's step is 2^8 and the input's 2^9: the
+    # recomputed output is within the type everywhere)
+    f = f_df(kept(x), kind)[0]
+    for got, want in ((dup, 400 * f), (back, f * kept(up))):
+        far = want.abs() >= 65520
+        assert bool(far.any()) == (got is dup) and torch.equal(got.cpu()[far].double(), want[far].sign() * math.inf)
+        assert bool(torch.isnan(got.cpu()[0, 4])) and bool(torch.isfinite(got.cpu()[0][~far[0] & ~torch.isnan(want[0])]).all())

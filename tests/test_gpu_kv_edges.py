@@ -140,3 +140,14 @@ def test_streams_of_all_kinds(kv):
         word = C.c_uint(7)
         L.check(L.L.dc_kv_status(stream, C.byref(word), 0), "status")                   # (waits for the stream)
         assert word.value == 0 and same(got[0], want[0]) and same(got[1], want[1])
+
+
+def test_outputs_beyond_the_type(kv):
+    """A mean beyond f16's largest number is infinite in f16 and what it is in bf16."""
+    g = gen(8)
+    k, v = torch.randn(1, 50, 1, 64, generator=g), torch.full((1, 50, 1, 64), 1e6)
+    f = filled(kv, k, v, 8)
+    q = torch.randn(1, 1, 2, 64, generator=g)
+    got = f.cache.attention(q.half().to(DEV), i32(50), table=f.table)
+    assert bool((got == math.inf).all())
+    check(f, q.bfloat16(), [50])
