@@ -509,7 +509,7 @@ static __device__ __forceinline__ void refer(const float (*ref)[8], const float*
             x = fmaxf(x, __builtin_amdgcn_exp2f(fmaf(ref[nt][t], unit[nt], -base)) * row_lane<t>(vr));
         });
         x = over_groups_max(x);
-        if (hi[nt] > m + 8.0f && x >= 16.0f) m = hi[nt];
+        if (hi[nt] - m > 8.0f && x >= 16.0f) m = hi[nt];
         if (x * __builtin_amdgcn_exp2f(base - m) > 32768.0f) m = base + (float)((int)(asu(x) >> 23) - 134);
         m = fmaxf(m, hi[nt] - 80.0f);
         const float al = M[nt] - m, be = __builtin_amdgcn_exp2f(al - (float)up);
@@ -575,7 +575,7 @@ static __device__ __forceinline__ void attend(Stage<D * BITS / 128>& c, const Fr
     // a score that passes its row's reference by 8, or a step as large as the unit (not a NaN): new references
     bool raise = vs >= R;
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) raise |= mx[nt] * unit[nt] > M[nt] + 8.0f;
+    for (int nt = 0; nt < NT; nt++) raise |= fmaf(mx[nt], unit[nt], -M[nt]) > 8.0f;    // (M + 8 is rounded above 2^27)
     if (__any(raise)) refer<NT, N>(ref, mx, unit, vs, acc, M, L, Z, R);
     const float vr = vs * asf(0x7F000000u - asu(R)) * 128.0f;       // 2^7 / R
     Frag w[NT];

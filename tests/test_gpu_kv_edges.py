@@ -151,3 +151,26 @@ def test_outputs_beyond_the_type(kv):
     got = f.cache.attention(q.half().to(DEV), i32(50), table=f.table)
     assert bool((got == math.inf).all())
     check(f, q.bfloat16(), [50])
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("k", [25, 26, 27, 28, 29, 30, 34])
+def test_scores_that_creep(kv, bits, k):
+    """Scores of about 2^k that rise by a few units of f32 from step to step of a wave (128
+    positions).  Which of the last ones share the weight is f32's rounding: the output is within what the last three steps'
+    positions hold, each row being one value."""
+    N, D, n = 1400, 64, 15 if bits == 4 else 255
+    key = torch.zeros(1, N, 1, D)
+    key[..., 0] = n                                                     # a step of 1, so the other value counts single codes
+    key[0, :, 0, 40] = (torch.arange(N) // 128).float()               # (added by a later instruction: to f32's last bit)
+    v = torch.arange(N)[None, :, None, None].float().expand(1, N, 1, D)
+    f = filled(kv, key, v, bits)
+    assert bool((f.ks == 1).all()) and bool((f.kz == 0).all())
+    held_rows = f.v[0, 1024:, 0, 0]
+    for rise in (2.0 ** -24, 1.5 * 2.0 ** -24, 2.0 ** -23, 1.5 * 2.0 ** -23, 2.0 ** -22, 2.0 ** -16):     # of a score, from code to code
+        q = torch.zeros(1, 1, 2, D)
+        q[..., 0], q[..., 40] = 1.0, rise * (n + 1)
+        for scale in (2.0 ** k / n, 2.0 ** k / n * 1.2, 2.0 ** k / n * 1.3):
+            got = f.cache.attention(q.bfloat16().to(DEV), i32(N), table=f.table, scale=scale).cpu().double()
+            assert bool(torch.isfinite(got).all()), (rise, scale, got[0, 0, 0, 0])
+            assert bool((got >= held_rows.min() * (1 - 2.0 ** -7)).all()) and bool((got <= held_rows.max() * (1 + 2.0 ** -7)).all()), (rise, scale, got[0, 0, 0, 0])
