@@ -315,8 +315,9 @@ typedef struct dc_kv_batch {
 size_t dc_kv_page_bytes(int page_size, int heads, int head_dim, int bits);
 /* Quantise keys and values [batch][tokens][heads][head_dim] (strides of batch, token and head in elements; the head's
  * values are consecutive) into the cache.  No two tokens of one call may have the same place (that place then holds a
- * mix).  Tokens at a position or in a page outside the cache are dropped (status bit 0).  batch x heads x (tokens + 30) / 16 is
- * below 2^25 (a read: 2^26; attention: batch x query rows / 16 below 2^24). */
+ * mix).  Tokens at a position or in a page outside the cache are dropped (status bit 0).  Calls of so many rows
+ * are taken: batch x heads x ((tokens + 30) / 16) at most 2^25 - 2 for a write, 2^26 - 4 for a read; batch x heads x
+ * ((tokens x q_heads / heads + 15) / 16) below 2^24 for the attention. */
 int dc_kv_write_device(const dc_kv_cache* cache, const dc_kv_batch* at, int dtype, const void* d_k,
                        const long long* k_strides, const void* d_v, const long long* v_strides, void* stream);
 /* Read them back (rounded to dtype, held at its largest finite value).  Positions and pages outside the cache read as
